@@ -6,13 +6,7 @@
 //     -log E is Gumbel-distributed for E = -log u.
 // The noise is a counter-based hash of (seed, request id, output position, vocabulary entry), so
 // a request's tokens do not depend on what else is in the batch or on how steps were cut.
-#include "common.cuh"
-
-__device__ __forceinline__ uint64_t mix64(uint64_t x) {
-    x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9ull;
-    x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
-    return x ^ (x >> 31);
-}
+#include "choice.cuh"
 
 // A row is cut into SAMPLE_PARTS slices, one block each; the blocks of a row form a thread-block cluster
 // and the first of them picks the winner out of the others' shared memory.  One block per row left the
@@ -20,10 +14,6 @@ __device__ __forceinline__ uint64_t mix64(uint64_t x) {
 // sampled row -- a hash and two logarithms per vocabulary entry -- one SM's work.
 #define SAMPLE_PARTS 8
 #define SAMPLE_THREADS 256
-
-__device__ __forceinline__ void take(float& bv, int& bi, float v, int i) {
-    if (v > bv || (v == bv && i < bi)) { bv = v; bi = i; }
-}
 
 template <bool CLUSTER>
 __global__ void __launch_bounds__(SAMPLE_THREADS)
@@ -40,18 +30,8 @@ sample_kernel(const float* __restrict__ logits, const float* __restrict__ temper
     const float* lg = logits + (int64_t)row * vocab;
     const float t = temperature[row];
     uint64_t key = 0;
-    if (t > 0.f) {
-        key = mix64(seed * 0x9E3779B97F4A7C15ull + (uint64_t)request[row]);
-        key = mix64(key ^ ((uint64_t)position[row] * 0xD1B54A32D192ED03ull));
-    }
-    auto score = [&](float v, int i) {
-        if (t > 0.f) {
-            const uint64_t h = mix64(key + (uint64_t)i);
-            const float u = ((float)(h >> 41) + 0.5f) * (1.0f / 8388608.0f);   // 23 bits + 0.5: never 0 or 1
-            v = v / t - logf(-logf(u));
-        }
-        return v;
-    };
+    if (t > 0.f) key = noise_key(seed, request[row], position[row]);
+    auto score = [&](float v, int i) { return t > 0.f ? noisy_score(v, t, key, i) : v; };
     // this block's slice: whole groups of four entries, so that aligned rows can be read 16 bytes at a time
     const int per = ((vocab + parts - 1) / parts + 3) & ~3;
     const int lo = min(vocab, part * per), hi = min(vocab, lo + per);

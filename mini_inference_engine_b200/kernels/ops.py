@@ -79,7 +79,7 @@ _RANGE_CODES = {1: "token id outside the vocabulary (or the fed-back tokens)", 2
 _RANGE_KERNELS = {1: "embedding", 2: "rope_cache", 3: "norm", 4: "attention_simt", 5: "attention_decode",
                   6: "attention_prefill", 7: "attention_prefill_tc", 8: "gemm_tcgen05 (q|k|v with rotation)",
                   9: "norm_group", 10: "qk_norm_rope", 11: "hyper_norm", 12: "latent_kv",
-                  13: "sandwich_norm", 14: "attention_f32"}
+                  13: "sandwich_norm", 14: "attention_f32", 15: "logit_rules"}
 _range_report: torch.Tensor | None = None
 _range_told: set = set()
 
@@ -761,15 +761,97 @@ def gemm_simt(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: torch.T
 
 # --------------------------------------------------------------------------- sampling
 
+class LogitRules:
+    """What holds for the logits of a step's rows beside the model: penalties for tokens that a row's text holds already, biases on single tokens,
+    a grammar's mask.  ``apply_logit_rules`` and ``sample`` take it.  Everything is on the device, int32 or float32 and contiguous; what is read is read
+    when the kernel runs, so the contents may change from step to step (in captured steps too).
+
+    ``history`` [slots, width]: a text a slot (prompt, then answer); ``slot`` [rows]: the row's slot (negative: no penalties and no biases);
+    ``prompt_len`` and ``total_len`` [rows]: tokens of the prompt, and of prompt and answer.  ``repetition``, ``presence``, ``frequency``
+    [rows] (or None: off): a token of the prompt or the answer has its logit x divided by ``repetition`` (multiplied where x is not positive); one of
+    the answer loses ``presence``, and ``frequency`` for every time that it stands there.  ``bias_tokens`` / ``bias_values`` [slots, n] and ``bias_len``
+    [rows] (None: all n of every row): token and what is added to its logit (-inf: a ban); a token named several times takes them all, in the list's order.
+    ``mask`` [masks, words >= ceil(vocab / 32)] and ``mask_row`` [rows] (negative: none): bit i % 32 of word i // 32 says whether entry i may
+    follow; the logits of the others become -inf, whatever they were.  In this order: repetition, presence and frequency, biases, mask."""
+
+    def __init__(self, history=None, slot=None, prompt_len=None, total_len=None, *, repetition=None, presence=None, frequency=None,
+                 bias_tokens=None, bias_values=None, bias_len=None, mask=None, mask_row=None):
+        rows = {t.numel() for t in (slot, prompt_len, total_len, repetition, presence, frequency, bias_len, mask_row) if t is not None}
+        _need(len(rows) == 1, "the rules of a step: one entry a row in slot, prompt_len, total_len, repetition, presence, frequency, bias_len and mask_row")
+        self.rows = rows.pop()
+        given = [t for t in (history, slot, prompt_len, total_len, repetition, presence, frequency, bias_tokens, bias_values, bias_len, mask, mask_row)
+                 if t is not None]
+        _need(len({t.device for t in given}) == 1, "the rules of a step are tensors of one device")
+        self.device = given[0].device
+        for t, name in ((slot, "slot"), (prompt_len, "prompt_len"), (total_len, "total_len"), (bias_len, "bias_len"), (mask_row, "mask_row"),
+                        (history, "history"), (bias_tokens, "bias_tokens"), (mask, "mask")):
+            if t is not None:
+                _i32(t, name)
+        for t, name in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency"), (bias_values, "bias_values")):
+            if t is not None:
+                _need(t.dtype == torch.float32 and t.is_contiguous(), f"{name} must be contiguous float32")
+        _need(history is None or (history.dim() == 2 and slot is not None and prompt_len is not None and total_len is not None),
+              "a history [slots, width] goes with slot, prompt_len and total_len")
+        _need(history is not None or (repetition is None and presence is None and frequency is None), "penalties need a history")
+        _need((bias_tokens is None) == (bias_values is None) and (bias_tokens is None or (slot is not None and bias_tokens.dim() == 2
+              and bias_tokens.shape == bias_values.shape)), "biases are tokens and values [slots, n], and a slot a row")
+        _need(bias_len is None or bias_tokens is not None, "bias_len without biases")
+        _need(history is None or bias_tokens is None or history.shape[0] == bias_tokens.shape[0], "history and biases have the same slots")
+        _need((mask is None) == (mask_row is None) and (mask is None or mask.dim() == 2), "a mask [masks, words] goes with mask_row")
+        if bias_tokens is not None and bias_tokens.shape[1] == 0:
+            bias_tokens = bias_values = bias_len = None
+        if mask is not None and mask.shape[0] == 0:
+            mask = mask_row = None
+        slots = history.shape[0] if history is not None else bias_tokens.shape[0] if bias_tokens is not None else 0
+        if slots == 0:
+            history = bias_tokens = bias_values = bias_len = slot = None
+        width = history.shape[1] if history is not None else 0
+        self.history, self.words = history, mask.shape[1] if mask is not None else None
+        self._kept = (slot, prompt_len, total_len, repetition, presence, frequency, bias_tokens, bias_values, bias_len, mask, mask_row)
+        self._args = (_ptr(history), ctypes.c_int64(width), slots, width, _ptr(slot), _ptr(prompt_len), _ptr(total_len), _ptr(repetition), _ptr(presence),
+                      _ptr(frequency), _ptr(bias_tokens), _ptr(bias_values), bias_tokens.shape[1] if bias_tokens is not None else 0, _ptr(bias_len),
+                      _ptr(mask), ctypes.c_int64(self.words or 0), mask.shape[0] if mask is not None else 0, _ptr(mask_row))
+
+    def args(self, logits: torch.Tensor):
+        """The kernel arguments of these rules for ``logits`` [rows, vocab] (entries of a row side by side, rows any distance apart)."""
+        _need(logits.dim() == 2 and logits.dtype == torch.float32 and (logits.stride(1) == 1 or logits.shape[1] <= 1), "logits must be float32 [rows, vocab], a row's entries side by side")
+        _need(logits.shape[0] == self.rows, f"rules of {self.rows} rows, logits of {logits.shape[0]}")
+        _need(logits.device == self.device and self.device.index == torch.cuda.current_device(), "logits and rules must be on the current device")
+        _need(self.words is None or self.words * 32 >= logits.shape[1], "a mask has a bit for every entry of the vocabulary")
+        return self._args
+
+
+RULE_SLICE = 16384          # entries of a row whose words a block of the rules' kernel holds at a time (csrc/logit_rules.cu)
+
+
+def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor) -> torch.Tensor:
+    """out[r] = logits[r] under ``rules`` (float32 [rows, vocab], ``out`` may be ``logits``; no other overlap).  See ``LogitRules``."""
+    args = rules.args(logits)
+    rows, vocab = logits.shape
+    _need(out.dtype == torch.float32 and out.shape == logits.shape and out.device == logits.device and (out.stride(1) == 1 or vocab <= 1),
+          "the output must be float32 of the logits' shape, a row's entries side by side")
+    _need(rows <= 1 or out.stride(0) >= vocab, "the output's rows must not overlap")
+    if rows == 0 or vocab == 0:
+        return out
+    parts = max(-(-vocab // RULE_SLICE), min(-(-4 * num_sms() // rows), vocab // 2048), 1)
+    _check(load("logit_rules").mie_apply_logit_rules(*args, _ptr(logits), ctypes.c_int64(logits.stride(0)), _ptr(out), ctypes.c_int64(out.stride(0)),
+                                                     rows, vocab, parts, _stream()), "apply_logit_rules")
+    return out
+
+
 def sample(logits: torch.Tensor, temperature, request, position, seed: int, out: torch.Tensor,
-           host_out: torch.Tensor | None = None, host_turn: torch.Tensor | None = None):
+           host_out: torch.Tensor | None = None, host_turn: torch.Tensor | None = None, *, rules: LogitRules | None = None,
+           logprob: torch.Tensor | None = None, append: bool = False):
     """Token ids [rows] from float32 logits [rows, vocab]; per-row temperature (0 = greedy), request
     id (int64) and output position (int32) key the noise.  ``host_out``: a pinned host tensor
     [turns, n >= rows] int32 that also receives the tokens, in row ``host_turn[0]`` (a device int32
     tensor; row 0 without it), written by the kernel itself (pinned memory is addressable from the
-    device), so that no copy has to follow."""
+    device), so that no copy has to follow.
+
+    ``rules``: the token is chosen from the logits under these rules (``LogitRules``; the logits stay as they are).  ``logprob`` (float32 [rows]):
+    receives log softmax of the logits (under the rules, before the temperature) at the token.  Rules that leave a row nothing make it token 0 with
+    -inf.  ``append``: the token joins the row's text in ``rules.history``, at place total_len (where there is room; a slot then serves one row)."""
     rows, vocab = logits.shape
-    _need(logits.dtype == torch.float32 and logits.is_contiguous(), "logits must be contiguous float32")
     _need(temperature.dtype == torch.float32 and request.dtype == torch.int64 and position.dtype == torch.int32
           and out.dtype == torch.int32, "sampling argument types")
     host_ptr, stride = ctypes.c_void_p(0), 0
@@ -779,11 +861,33 @@ def sample(logits: torch.Tensor, temperature, request, position, seed: int, out:
         if host_turn is not None:
             _need(host_turn.is_cuda and host_turn.dtype == torch.int32 and host_turn.numel() >= 1, "host_turn must be a device int32 tensor")
         host_ptr, stride = ctypes.c_void_p(host_out.data_ptr()), host_out.shape[1]
-    lib = build.load("sampling")
-    _check(lib.mie_sample(_ptr(logits), _ptr(temperature), _ptr(request), _ptr(position),
-                          ctypes.c_uint64(seed & ((1 << 64) - 1)), _ptr(out), rows, vocab, host_ptr,
-                          _ptr(host_turn) if host_out is not None else ctypes.c_void_p(0), stride, _stream()), "sample")
+    turn_ptr = _ptr(host_turn) if host_out is not None else ctypes.c_void_p(0)
+    if rules is None and logprob is None:
+        _need(not append, "append goes with rules")
+        _need(logits.dtype == torch.float32 and logits.is_contiguous(), "logits must be contiguous float32")
+        lib = build.load("sampling")
+        _check(lib.mie_sample(_ptr(logits), _ptr(temperature), _ptr(request), _ptr(position),
+                              ctypes.c_uint64(seed & ((1 << 64) - 1)), _ptr(out), rows, vocab, host_ptr, turn_ptr, stride, _stream()), "sample")
+        return out
+    if rules is None:
+        _need(logits.dtype == torch.float32 and (logits.stride(1) == 1 or vocab <= 1), "logits must be float32, a row's entries side by side")
+        args = _NO_RULES
+    else:
+        args = rules.args(logits)
+    _need(vocab > 0, "an empty vocabulary has no token")
+    for t, name in ((temperature, "temperature"), (request, "request"), (position, "position"), (out, "out"), (logprob, "logprob")):
+        if t is not None:
+            _need(t.is_contiguous() and t.numel() >= rows, f"{name} must be contiguous, one entry a row")
+    _need(logprob is None or logprob.dtype == torch.float32, "logprob must be float32")
+    _need(not append or (rules is not None and rules.history is not None), "append goes with rules that have a history")
+    _ptr(logits)                                               # (refuses what is not on a CUDA device)
+    _check(load("logit_rules").mie_sample_rules(*args, _ptr(logits), ctypes.c_int64(logits.stride(0)), _ptr(temperature), _ptr(request), _ptr(position),
+                                                ctypes.c_uint64(seed & ((1 << 64) - 1)), _ptr(out), _ptr(logprob), _ptr(rules.history) if append else ctypes.c_void_p(0),
+                                                rows, vocab, host_ptr, turn_ptr, stride, _stream()), "sample with rules")
     return out
+
+
+_NO_RULES = (None, ctypes.c_int64(0), 0, 0, None, None, None, None, None, None, None, None, 0, None, None, ctypes.c_int64(0), 0, None)
 
 
 # --------------------------------------------------------------------------- post-norm stream, grouped statistics
