@@ -1,12 +1,14 @@
 // The decode attention kernel, its parameter block and its launch by head size, shared by the
 // entry points that differ in where the scratch memory comes from (attention_decode.cu: the
 // caller's; attention_decode_static.cu: a fixed array inside the library) and in whether a window keeps
-// the first keys in sight (attention_decode_kept.cu: the KEEP instances, compiled where a model asks for them).
+// the first keys in sight (attention_decode_kept.cu: the KEEP instances, compiled where a model asks for them), and for rows whose
+// first keys another kernel has dealt with (attention_decode_shared.cu: the SHARED instances).
 #pragma once
 #include "mma_common.cuh"
 #include "tcgen05_common.cuh"      // mbarrier, TMA copies, bounded waits, the tensor-map encoder
 #include "range_check.cuh"
 #include "rope_math.cuh"
+#include "prefix_plan.cuh"
 
 #define DEC_WARPS 4
 #define DEC_TILE 64
@@ -39,6 +41,8 @@ struct DecodeParams {
     float scale;             // the scale without the base-2 factor, for scores that are modified before the softmax
     ScoreMods mods;          // cap, bias by distance, sink (common.cuh); all off: the plain softmax
     int modded;
+    // SHARED: the rows' groups, and what attention over a group's prefix left for each of its rows (attention_prefix.cu)
+    PrefixGroups groups; const float* pre_o; const float* pre_lse; int64_t pre_slots;
 };
 
 // Where the 16-byte piece `chunk` of key row `row` lies inside a tile that TMA wrote with the
@@ -64,7 +68,9 @@ __device__ __forceinline__ uint32_t swz_tile_off(int row, int chunk) {
 // blocks than fit beside one another it is the faster way (128 requests x 512 keys 20.6 -> 14.9 us,
 // 256 x 512 34.4 -> 29.2 us, 256 x 2048 101 -> 96 us = 5.6 TB/s); where a block walks a long part
 // alone it is not (64 x 2048: 40.0 -> 42.9 us), so the caller chooses (ops.decode_uses_tma).
-template <int D, int NSTAGE, bool TMA, bool KEEP>
+// SHARED: a row of a group with a shared prefix walks its own keys only, those from the prefix's end on, and joins them with the partial
+// results that attention_prefix.cu left for the prefix (the splits merge through scratch memory then, never in a cluster).
+template <int D, int NSTAGE, bool TMA, bool KEEP, bool SHARED>
 __global__ void __launch_bounds__(DEC_WARPS * 32)
 decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const DecodeParams p) {
@@ -110,9 +116,22 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int quad = lane >> 2, tq = lane & 3;
 
+    __shared__ PrefixPart s_part;                                  // SHARED: the row's group (rows 0: it has none)
+    int prefix = 0;
+    if (SHARED) {
+        for (int g = 0; g < p.groups.groups; ++g) {
+            const PrefixPart t = prefix_group(p.groups, g);
+            if (row >= t.first_row && row < t.first_row + t.rows) { prefix = t.keys; break; }
+        }
+        if (prefix > ctx) {                                        // a context that ends inside its prefix
+            if (threadIdx.x == 0 && split == 0 && blockIdx.y == 0) range_report(p.report, MIE_RANGE_POSITION, MIE_K_ATTENTION_DECODE, row, prefix);
+            prefix = ctx;
+        }
+    }
     // this block's part of the context: the range [lo, ctx) cut into `splits` parts of whole tiles
-    const int first_key = mask_first_key(ctx - 1, p.window);      // sliding window, or the start of the query's block of positions
-    const int lo = first_key & ~(DEC_TILE - 1);
+    const int first_key = SHARED ? prefix : mask_first_key(ctx - 1, p.window);      // sliding window, or the start of the query's block of positions
+    // (own keys: tiles from the start of their first page on, so that no earlier page of the row's table is asked for)
+    const int lo = SHARED ? prefix & ~(min(p.page_size, DEC_TILE) - 1) : first_key & ~(DEC_TILE - 1);
     const int kept = KEEP ? mask_kept_tiles(p.keep, lo, DEC_TILE) : 0;       // tiles of kept keys in front of the window's
     const int tiles_total = kept + (ctx - lo + DEC_TILE - 1) / DEC_TILE;
     // The grid is laid out for the longest context the launch may meet; a row is cut into as many parts as
@@ -207,7 +226,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         for (int idx = threadIdx.x; idx < DEC_TILE * CHUNKS_PER_ROW; idx += DEC_WARPS * 32) {
             const int r = idx / CHUNKS_PER_ROW, c = (idx - r * CHUNKS_PER_ROW) * 8;
             const int key = k0 + r;
-            if (key < ctx) {
+            if (key < ctx && (!SHARED || key >= first_key)) {
                 const int page = page_at(key, base);
                 const int64_t src = (((int64_t)page * p.num_kv_heads + kvh) * p.page_size + (key & (p.page_size - 1))) * D + c;
                 cp_async16(kd + r * DP + c, p.k_cache + src);
@@ -223,6 +242,10 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     for (int t = 0; t < NSTAGE - 1; ++t) {
         if (t < ntiles) load_tile(t, t);
         cp_async_commit();
+    }
+    if (SHARED && warp == DEC_WARPS - 1) {                         // how the row's prefix was cut, under the copies (read behind the tiles' barriers)
+        const PrefixPart t = prefix_find(p.groups, prefix_chunk(p.groups), row, true);
+        if (lane == 0) s_part = t;
     }
     pdl_wait();                                                    // q and the newest key and value are the previous kernel's
     const int newest = ctx - 1;                                    // the only cached position written during this step
@@ -304,6 +327,11 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
                 if (TMA) *reinterpret_cast<uint4*>(tma_tiles + (size_t)stage * 2 * KV_TILE_BYTES + which * KV_TILE_BYTES + swz_tile_off(r, c / 8)) = v;
                 else *reinterpret_cast<uint4*>((which ? v_s : k_s) + stage * DEC_TILE * DP + r * DP + c) = v;
             }
+            __syncthreads();
+        }
+        if (SHARED && TMA && tile0 + t == 0 && lo < first_key) {   // the first page's slots in front of the own keys may hold anything: 0 * NaN is NaN
+            for (int i = threadIdx.x; i < (first_key - lo) * CHUNKS_PER_ROW; i += DEC_WARPS * 32)
+                *reinterpret_cast<uint4*>(tma_tiles + (size_t)stage * 2 * KV_TILE_BYTES + KV_TILE_BYTES + swz_tile_off(i / CHUNKS_PER_ROW, i % CHUNKS_PER_ROW)) = make_uint4(0, 0, 0, 0);
             __syncthreads();
         }
         const bf16* kt = k_s + stage * DEC_TILE * DP + warp * 16 * DP;
@@ -457,6 +485,23 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
             val.x += f * v.x; val.y += f * v.y; val.z += f * v.z; val.w += f * v.w;
         }
         const int head = kvh * G + g0 + g;
+        if (SHARED && eff == 1 && s_part.rows > 0 && s_part.splits > 0) {
+            const int64_t at = s_part.slot0 + (int64_t)(row - s_part.first_row) * s_part.splits;
+            const int S2 = at + s_part.splits <= p.pre_slots ? s_part.splits : 0;
+            float mm = c_lse[g];
+            for (int s2 = 0; s2 < S2; ++s2) mm = fmaxf(mm, __ldcg(p.pre_lse + (at + s2) * p.num_heads + head));
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            float w = fast_exp2(c_lse[g] - ref), wsum = w;
+            val.x *= w; val.y *= w; val.z *= w; val.w *= w;
+            for (int s2 = 0; s2 < S2; ++s2) {
+                w = fast_exp2(__ldcg(p.pre_lse + (at + s2) * p.num_heads + head) - ref);
+                const float4 part = __ldcg(reinterpret_cast<const float4*>(p.pre_o + ((at + s2) * p.num_heads + head) * D + d));
+                val.x += w * part.x; val.y += w * part.y; val.z += w * part.z; val.w += w * part.w;
+                wsum += w;
+            }
+            const float inv = wsum > 0.f ? __frcp_rn(wsum) : 0.f;
+            val.x *= inv; val.y *= inv; val.z *= inv; val.w *= inv;
+        }
         if (eff == 1) {
             if (p.out32) {
                 *reinterpret_cast<float4*>(p.out32 + ((int64_t)token * p.num_heads + head) * D + d) = val;
@@ -529,7 +574,21 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         const int64_t base = ((int64_t)row * p.num_heads + head) * p.splits;
         float mm = -INFINITY;
         for (int s2 = 0; s2 < eff; ++s2) mm = fmaxf(mm, __ldcg(p.part_lse + base + s2));
+        int64_t at = 0;                                            // SHARED: the row's results of its prefix come first
+        int S2 = 0;
+        if (SHARED && s_part.rows > 0) {
+            at = s_part.slot0 + (int64_t)(row - s_part.first_row) * s_part.splits;
+            S2 = at + s_part.splits <= p.pre_slots ? s_part.splits : 0;
+            for (int s2 = 0; s2 < S2; ++s2) mm = fmaxf(mm, __ldcg(p.pre_lse + (at + s2) * p.num_heads + head));
+        }
         float acc = 0.f, wsum = 0.f;
+        if (SHARED) {
+            for (int s2 = 0; s2 < S2; ++s2) {
+                const float w = fast_exp2(__ldcg(p.pre_lse + (at + s2) * p.num_heads + head) - (mm == -INFINITY ? 0.f : mm));
+                acc += w * __ldcg(p.pre_o + ((at + s2) * p.num_heads + head) * D + d);
+                wsum += w;
+            }
+        }
         for (int s2 = 0; s2 < eff; ++s2) {
             const float lse = __ldcg(p.part_lse + base + s2);
             if (lse == -INFINITY) continue;
@@ -557,7 +616,7 @@ static int make_decode_map(CUtensorMap* map, const void* ptr, uint64_t rows, int
     return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
 }
 
-template <int D, int NSTAGE, bool TMA, bool KEEP>
+template <int D, int NSTAGE, bool TMA, bool KEEP, bool SHARED>
 static int launch_decode_stages(const DecodeParams& p, const DecodeMaps& maps, int num_rows, cudaStream_t stream) {
     // at least the four-warp merge buffer (4 x 16 x D float32) must fit
     size_t smem = TMA ? (size_t)NSTAGE * 2 * ((D + 63) / 64) * 8192 + 1024 : (size_t)NSTAGE * 2 * DEC_TILE * (D + 8) * sizeof(bf16);
@@ -566,36 +625,36 @@ static int launch_decode_stages(const DecodeParams& p, const DecodeMaps& maps, i
     DecodeParams pp = p;
     pp.recv_offset = (uint32_t)((smem + 15) & ~size_t(15));
     if (p.cluster) smem = pp.recv_offset + (16 * (D / 4) + 8) * sizeof(float4) + 8 * 16 * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(decode_attention_kernel<D, NSTAGE, TMA, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(decode_attention_kernel<D, NSTAGE, TMA, KEEP, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
     const dim3 grid(p.splits, p.num_kv_heads * p.chunks, num_rows);
     const dim3 cluster(p.cluster ? p.splits : 1, 1, 1);
-    return launch_kernel_cluster(decode_attention_kernel<D, NSTAGE, TMA, KEEP>, grid, dim3(DEC_WARPS * 32), smem, stream, cluster,
+    return launch_kernel_cluster(decode_attention_kernel<D, NSTAGE, TMA, KEEP, SHARED>, grid, dim3(DEC_WARPS * 32), smem, stream, cluster,
                                  maps.k, maps.v, pp);
 }
 
 // Tiles in flight per block.  Few tiles per block (short contexts, many splits): two stages, so that
 // more blocks share an SM and hide one another's latencies.  Many tiles per block: a deeper ring.
-template <int D, bool TMA, bool KEEP>
+template <int D, bool TMA, bool KEEP, bool SHARED>
 static int launch_decode_tma(const DecodeParams& p, const DecodeMaps& maps, int num_rows, cudaStream_t stream) {
-    if (p.stages <= 2) return launch_decode_stages<D, 2, TMA, KEEP>(p, maps, num_rows, stream);
-    if (p.stages == 3 || D > 64) return launch_decode_stages<D, 3, TMA, KEEP>(p, maps, num_rows, stream);
-    return launch_decode_stages<D, 4, TMA, KEEP>(p, maps, num_rows, stream);
+    if (p.stages <= 2) return launch_decode_stages<D, 2, TMA, KEEP, SHARED>(p, maps, num_rows, stream);
+    if (p.stages == 3 || D > 64) return launch_decode_stages<D, 3, TMA, KEEP, SHARED>(p, maps, num_rows, stream);
+    return launch_decode_stages<D, 4, TMA, KEEP, SHARED>(p, maps, num_rows, stream);
 }
 
-template <int D, bool KEEP>
+template <int D, bool KEEP, bool SHARED>
 static int launch_decode(const DecodeParams& p, const DecodeMaps& maps, int num_rows, cudaStream_t stream) {
     if constexpr (D == 64 || D == 128) {
-        if (maps.use) return launch_decode_tma<D, true, KEEP>(p, maps, num_rows, stream);
+        if (maps.use) return launch_decode_tma<D, true, KEEP, SHARED>(p, maps, num_rows, stream);
     }
-    return launch_decode_tma<D, false, KEEP>(p, maps, num_rows, stream);
+    return launch_decode_tma<D, false, KEEP, SHARED>(p, maps, num_rows, stream);
 }
 
 
 // Checks the sizes, fills the parameter block and launches.  With splits > 1 and all three scratch
 // pointers null, the splits (2, 4 or 8) form a thread-block cluster and merge through distributed
 // shared memory; with scratch given, any number of splits merges through it.
-template <bool KEEP>
+template <bool KEEP, bool SHARED = false>
 static int decode_attention_launch(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
                                    const int* block_tables, int table_stride, const int* row_q_start,
                                    const int* row_q_len, const int* row_ctx_len, int num_rows, void* out,
@@ -604,12 +663,14 @@ static int decode_attention_launch(const void* q, int64_t q_stride, const void* 
                                    cudaStream_t stream, int stages = 0, int64_t num_pages = 0,
                                    int64_t check_pages = 0, int* report = nullptr, int min_part_tiles = 0,
                                    const float* cos_t = nullptr, const float* sin_t = nullptr, int max_pos = 0, bool out_f32 = false,
-                                   const ScoreMods* mods = nullptr, int keep = 0) {
+                                   const ScoreMods* mods = nullptr, int keep = 0, const PrefixGroups* groups = nullptr,
+                                   const float* pre_o = nullptr, const float* pre_lse = nullptr, int64_t pre_slots = 0) {
     if (num_rows <= 0) return 0;
     if (head_dim < 16 || head_dim > DEC_MAX_D || head_dim % 16) return MIE_ERR_BAD_ARG;
     if (num_kv_heads <= 0 || num_heads % num_kv_heads) return MIE_ERR_BAD_ARG;
     if (page_size < 1 || (page_size & (page_size - 1))) return MIE_ERR_BAD_ARG;
     const bool cluster = splits > 1 && !part_o && !part_lse && !counters;     // no scratch given: merge inside a cluster
+    if (SHARED && (cluster || !groups || window != 0)) return MIE_ERR_BAD_ARG;
     if (splits < 1 || (splits > 1 && !cluster && (!part_o || !part_lse || !counters))) return MIE_ERR_BAD_ARG;
     if (cluster && splits != 2 && splits != 4 && splits != 8) return MIE_ERR_BAD_ARG;
     if (num_rows > 65535) return MIE_ERR_TOO_LARGE;
@@ -633,6 +694,8 @@ static int decode_attention_launch(const void* q, int64_t q_stride, const void* 
     if (p.mods.dist_bias && p.mods.dist_len <= 0) return MIE_ERR_BAD_ARG;
     p.modded = p.mods.softcap > 0.f || p.mods.dist_bias != nullptr || p.mods.slope != nullptr;
     p.check_pages = check_pages; p.report = report;
+    p.groups = groups ? *groups : PrefixGroups{};
+    p.pre_o = pre_o; p.pre_lse = pre_lse; p.pre_slots = pre_slots;
     if ((cos_t != nullptr) != (sin_t != nullptr) || (cos_t && (head_dim % 32 || max_pos <= 0))) return MIE_ERR_BAD_ARG;
     p.cos_t = cos_t; p.sin_t = sin_t; p.max_pos = max_pos;
     // TMA copies (see the kernel): head sizes 64 and 128, pages of 8 positions or more, a caller that says
@@ -651,14 +714,14 @@ static int decode_attention_launch(const void* q, int64_t q_stride, const void* 
         p.error = g_error_dev;
     }
     switch (head_dim) {
-        case 16: return launch_decode<16, KEEP>(p, maps, num_rows, stream);
-        case 32: return launch_decode<32, KEEP>(p, maps, num_rows, stream);
-        case 48: return launch_decode<48, KEEP>(p, maps, num_rows, stream);
-        case 64: return launch_decode<64, KEEP>(p, maps, num_rows, stream);
-        case 80: return launch_decode<80, KEEP>(p, maps, num_rows, stream);
-        case 96: return launch_decode<96, KEEP>(p, maps, num_rows, stream);
-        case 112: return launch_decode<112, KEEP>(p, maps, num_rows, stream);
-        case 128: return launch_decode<128, KEEP>(p, maps, num_rows, stream);
+        case 16: return launch_decode<16, KEEP, SHARED>(p, maps, num_rows, stream);
+        case 32: return launch_decode<32, KEEP, SHARED>(p, maps, num_rows, stream);
+        case 48: return launch_decode<48, KEEP, SHARED>(p, maps, num_rows, stream);
+        case 64: return launch_decode<64, KEEP, SHARED>(p, maps, num_rows, stream);
+        case 80: return launch_decode<80, KEEP, SHARED>(p, maps, num_rows, stream);
+        case 96: return launch_decode<96, KEEP, SHARED>(p, maps, num_rows, stream);
+        case 112: return launch_decode<112, KEEP, SHARED>(p, maps, num_rows, stream);
+        case 128: return launch_decode<128, KEEP, SHARED>(p, maps, num_rows, stream);
     }
     return MIE_ERR_BAD_ARG;
 }

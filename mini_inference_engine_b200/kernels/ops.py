@@ -6,6 +6,7 @@ other path: a tensor that is not on a CUDA device is refused.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -79,7 +80,7 @@ _RANGE_CODES = {1: "token id outside the vocabulary (or the fed-back tokens)", 2
 _RANGE_KERNELS = {1: "embedding", 2: "rope_cache", 3: "norm", 4: "attention_simt", 5: "attention_decode",
                   6: "attention_prefill", 7: "attention_prefill_tc", 8: "gemm_tcgen05 (q|k|v with rotation)",
                   9: "norm_group", 10: "qk_norm_rope", 11: "hyper_norm", 12: "latent_kv",
-                  13: "sandwich_norm", 14: "attention_f32", 15: "logit_rules"}
+                  13: "sandwich_norm", 14: "attention_f32", 15: "logit_rules", 16: "attention_prefix"}
 _range_report: torch.Tensor | None = None
 _range_told: set = set()
 
@@ -522,7 +523,7 @@ def set_prefill_pairs(mode: int = -1) -> None:
 def check_tc_errors() -> None:
     """Raises if a block of a tensor-core kernel gave up a bounded wait (call after a synchronise)."""
     for name, fn in (("attention_prefill_tc", "mie_prefill_attention_tc"), ("attention_decode", "mie_decode_attention"),
-                     ("attention_decode_kept", "mie_decode_attention_kept")):
+                     ("attention_decode_kept", "mie_decode_attention_kept"), ("attention_decode_shared", "mie_decode_attention_shared")):
         lib = build._libs.get(name)
         if lib is not None and getattr(lib, fn + "_error")():
             getattr(lib, fn + "_clear_error")()
@@ -728,6 +729,96 @@ def decode_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, block_tab
                                     _ptr(cos), _ptr(sin), int(cos.shape[0]) if cos is not None else 0,
                                     int(out.dtype == torch.float32), *(mods or _NO_MODS).args(num_heads), _stream()),
            "decode_attention")
+    return out
+
+
+@functools.lru_cache(maxsize=None)
+def _prefix_layout(rows: int, num_heads: int, num_kv_heads: int, head_dim: int, sms: int):
+    """How the prefix kernel cuts (row, head) pairs, as its library says, and the most slots of partial results that it writes."""
+    layout = (ctypes.c_int * 4)()
+    fn = load("attention_prefix").mie_prefix_layout
+    fn.restype = ctypes.c_longlong
+    slots = fn(rows, num_heads, num_kv_heads, head_dim, sms, layout)
+    _need(slots >= 0, f"{num_heads} heads of {head_dim} on {num_kv_heads}: the prefix kernel takes head sizes in steps of 16 up to 128")
+    return layout, slots
+
+
+def own_keys_plan(rows: int, kv_units: int, max_own: int, tma_ok: bool, head_dim: int) -> tuple[int, int]:
+    """(splits, min_part_tiles) for the rows' own keys behind a shared prefix: parts of at least two tiles of 64 keys while the batch alone leaves
+    places on the GPU free, and those of ``decode_plan`` for long ones.  A row is cut by its own length on the device."""
+    units, tiles = max(1, rows * kv_units), -(-max(1, max_own) // 64)
+    places = decode_blocks_per_sm(head_dim) * num_sms() // units
+    if tma_ok and units >= 64 and tiles >= 2 * LONG_PART_TILES:
+        parts = min(places, tiles // LONG_PART_TILES, 8 if head_dim <= 64 else 16)
+        if parts >= 2:
+            return parts, LONG_PART_TILES
+    return max(1, min(8, places, tiles // 2)), 2
+
+
+def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, block_tables, row_q_start, row_q_len, row_ctx_len, group_start,
+                            group_prefix, out: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, scale: float, *,
+                            max_prefix: int | None = None, max_own: int | None = None) -> torch.Tensor:
+    """Attention of rows with exactly one new token of which groups share their first keys (answers to one prompt, requests behind one system
+    prompt): the shared keys and values are read once a group, not once a row.  bfloat16 (the output bfloat16 or float32), head sizes in steps of
+    16 up to 128, no window and no score modifiers; otherwise arguments and result are ``decode_attention``'s.
+
+    ``group_start`` int32 [groups + 1]: group g is the rows group_start[g] .. group_start[g + 1] - 1; ``group_prefix`` int32 [groups]: its rows share that
+    many first keys, which lie where the block table of the group's FIRST row says (the other rows' table entries for them are not followed, but
+    where a prefix ends inside a page every row's own entry for that page holds its keys from there on).  0: the rows share nothing.  Groups do not
+    overlap; rows of no group share nothing.  A row's context (``row_ctx_len``) includes its prefix.  ``max_prefix`` and ``max_own``: bounds on the
+    prefixes and on the keys behind them, for planning (a captured step's may be shorter); without them the block table's width bounds both.
+
+    Two launches: the groups' (row, head) pairs against the prefixes in tiles, then the rows' own keys, joined with those.  Rows with more than
+    one new token are skipped.  Slots of a row's last page behind its context must hold finite values (see ``decode_uses_tma``)."""
+    _need(q.dtype == torch.bfloat16 == k_cache.dtype == v_cache.dtype and out.dtype in (torch.bfloat16, torch.float32),
+          "attention over shared prefixes is bfloat16 (its output bfloat16 or float32)")
+    for t, n in ((block_tables, "block_tables"), (row_q_start, "row_q_start"), (row_q_len, "row_q_len"), (row_ctx_len, "row_ctx_len"),
+                 (group_start, "group_start"), (group_prefix, "group_prefix")):
+        _i32(t, n)
+    rows, groups = row_q_len.numel(), group_prefix.numel()
+    _need(num_kv_heads > 0 and num_heads % num_kv_heads == 0, "query heads must be a multiple of kv heads")
+    _need(head_dim % 16 == 0 and 16 <= head_dim <= 128, f"head_dim {head_dim}: attention over shared prefixes takes multiples of 16 from 16 to 128")
+    _need(page_size >= 1 and page_size & (page_size - 1) == 0, "the page size must be a power of two")
+    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and tuple(k_cache.shape[1:]) == (num_kv_heads, page_size, head_dim)
+          and k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous [pages, kv heads, page size, head_dim]")
+    _need(block_tables.dim() == 2 and block_tables.shape[0] >= rows and row_q_start.numel() >= rows and row_ctx_len.numel() >= rows,
+          "block_tables, row_q_start and row_ctx_len need an entry for every row")
+    _need(group_start.numel() == groups + 1, "group_start has one entry more than group_prefix")
+    _need(q_stride % 8 == 0 and q.data_ptr() % 16 == 0 and k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0, "rows of q and the caches must begin on 16 bytes")
+    _need(out.is_contiguous() and out.data_ptr() % 16 == 0, "the output must be contiguous [tokens, heads, head_dim], 16-byte aligned")
+    _need(q.device.index == torch.cuda.current_device() if q.is_cuda else True, "the tensors must be on the current device")
+    if rows == 0:
+        return out
+    covered = block_tables.shape[1] * page_size
+    max_own = covered if max_own is None else max(1, min(max_own, covered))
+    chunks = -(-(num_heads // num_kv_heads) // 16)
+    units = num_kv_heads * chunks
+    tma_ok = head_dim in (64, 128) and page_size >= 8
+    splits, part_tiles = own_keys_plan(rows, units, max_own, tma_ok, head_dim)
+    blocks = rows * units * splits
+    tma = tma_ok and decode_uses_tma(blocks, head_dim)
+    stages = decode_stages(blocks, max_own, splits, tma, head_dim, clustered=False)
+    part_o = part_lse = counters = None
+    if splits > 1:
+        part_o = _workspace(q.device, "decode_part_o", rows * num_heads * splits * head_dim, torch.float32)
+        part_lse = _workspace(q.device, "decode_part_lse", rows * num_heads * splits, torch.float32)
+        counters = _workspace(q.device, "decode_counters", rows * units, torch.int32)
+    shared = groups > 0 and max_prefix != 0
+    layout, slots = _prefix_layout(rows, num_heads, num_kv_heads, head_dim, num_sms(q.device))
+    pre_o = pre_lse = None
+    if shared:
+        pre_o = _workspace(q.device, "prefix_o", slots * num_heads * head_dim, torch.float32)
+        pre_lse = _workspace(q.device, "prefix_lse", slots * num_heads, torch.float32)
+        _check(load("attention_prefix").mie_prefix_attention(
+            _ptr(q), ctypes.c_int64(q_stride), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(row_q_start), _ptr(row_q_len),
+            rows, _ptr(group_start), _ptr(group_prefix), groups, num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale), layout, _ptr(pre_o),
+            _ptr(pre_lse), ctypes.c_longlong(slots), ctypes.c_longlong(k_cache.shape[0]), _stream()), "shared_prefix_attention (prefixes)")
+    _check(load("attention_decode_shared").mie_decode_attention_shared(
+        _ptr(q), ctypes.c_int64(q_stride), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(row_q_start), _ptr(row_q_len),
+        _ptr(row_ctx_len), rows, _ptr(group_start), _ptr(group_prefix), groups if shared else 0, layout, _ptr(pre_o), _ptr(pre_lse),
+        ctypes.c_longlong(slots), _ptr(out), num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale), int(splits), _ptr(part_o),
+        _ptr(part_lse), _ptr(counters), int(stages), ctypes.c_int64(k_cache.shape[0] if tma else 0), ctypes.c_int64(k_cache.shape[0]), int(part_tiles),
+        int(out.dtype == torch.float32), _stream()), "shared_prefix_attention (own keys)")
     return out
 
 
