@@ -912,9 +912,6 @@ class LogitRules:
         return self._args
 
 
-RULE_SLICE = 16384          # entries of a row whose words a block of the rules' kernel holds at a time (csrc/logit_rules.cu)
-
-
 def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor) -> torch.Tensor:
     """out[r] = logits[r] under ``rules`` (float32 [rows, vocab], ``out`` may be ``logits``; no other overlap).  See ``LogitRules``."""
     args = rules.args(logits)
@@ -924,9 +921,8 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     _need(rows <= 1 or out.stride(0) >= vocab, "the output's rows must not overlap")
     if rows == 0 or vocab == 0:
         return out
-    parts = max(-(-vocab // RULE_SLICE), min(-(-4 * num_sms() // rows), vocab // 2048), 1)
     _check(load("logit_rules").mie_apply_logit_rules(*args, _ptr(logits), ctypes.c_int64(logits.stride(0)), _ptr(out), ctypes.c_int64(out.stride(0)),
-                                                     rows, vocab, parts, _stream()), "apply_logit_rules")
+                                                     rows, vocab, _stream()), "apply_logit_rules")
     return out
 
 
