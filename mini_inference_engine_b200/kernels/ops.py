@@ -523,7 +523,7 @@ def set_prefill_pairs(mode: int = -1) -> None:
 def check_tc_errors() -> None:
     """Raises if a block of a tensor-core kernel gave up a bounded wait (call after a synchronise)."""
     for name, fn in (("attention_prefill_tc", "mie_prefill_attention_tc"), ("attention_decode", "mie_decode_attention"),
-                     ("attention_decode_kept", "mie_decode_attention_kept"), ("attention_decode_shared", "mie_decode_attention_shared")):
+                     ("attention_decode_kept", "mie_decode_attention_kept"), ("attention_decode_shared", "mie_decode_attention_shared"), ("attention_prefix", "mie_prefix_attention")):
         lib = build._libs.get(name)
         if lib is not None and getattr(lib, fn + "_error")():
             getattr(lib, fn + "_clear_error")()
@@ -733,12 +733,12 @@ def decode_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, block_tab
 
 
 @functools.lru_cache(maxsize=None)
-def _prefix_layout(rows: int, num_heads: int, num_kv_heads: int, head_dim: int, sms: int):
+def _prefix_layout(rows: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, sms: int):
     """How the prefix kernel cuts (row, head) pairs, as its library says, and the most slots of partial results that it writes."""
-    layout = (ctypes.c_int * 4)()
+    layout = (ctypes.c_int * 5)()
     fn = load("attention_prefix").mie_prefix_layout
     fn.restype = ctypes.c_longlong
-    slots = fn(rows, num_heads, num_kv_heads, head_dim, sms, layout)
+    slots = fn(rows, num_heads, num_kv_heads, head_dim, page_size, sms, layout)
     _need(slots >= 0, f"{num_heads} heads of {head_dim} on {num_kv_heads}: the prefix kernel takes head sizes in steps of 16 up to 128")
     return layout, slots
 
@@ -786,6 +786,8 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     _need(group_start.numel() == groups + 1, "group_start has one entry more than group_prefix")
     _need(q_stride % 8 == 0 and q.data_ptr() % 16 == 0 and k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0, "rows of q and the caches must begin on 16 bytes")
     _need(out.is_contiguous() and out.data_ptr() % 16 == 0, "the output must be contiguous [tokens, heads, head_dim], 16-byte aligned")
+    _need(k_cache.shape[0] * num_kv_heads * page_size < 1 << 31, "caches of 2^31 key rows and more are not taken")
+    _need(scale > 0, "the scale of the scores must be positive")
     _need(q.device.index == torch.cuda.current_device() if q.is_cuda else True, "the tensors must be on the current device")
     if rows == 0:
         return out
@@ -804,7 +806,7 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
         part_lse = _workspace(q.device, "decode_part_lse", rows * num_heads * splits, torch.float32)
         counters = _workspace(q.device, "decode_counters", rows * units, torch.int32)
     shared = groups > 0 and max_prefix != 0
-    layout, slots = _prefix_layout(rows, num_heads, num_kv_heads, head_dim, num_sms(q.device))
+    layout, slots = _prefix_layout(rows, num_heads, num_kv_heads, head_dim, page_size, num_sms(q.device))
     pre_o = pre_lse = None
     if shared:
         pre_o = _workspace(q.device, "prefix_o", slots * num_heads * head_dim, torch.float32)
