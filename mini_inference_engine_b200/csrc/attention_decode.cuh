@@ -42,7 +42,7 @@ struct DecodeParams {
     ScoreMods mods;          // cap, bias by distance, sink (common.cuh); all off: the plain softmax
     int modded;
     // SHARED: the rows' groups, and what attention over a group's prefix left for each of its rows (attention_prefix.cu)
-    PrefixGroups groups; const float* pre_o; const float* pre_lse; int64_t pre_slots;
+    PrefixGroups groups; const float* pre_o; const float* pre_lse; const int* pre_chunk; int64_t pre_slots;
 };
 
 // Where the 16-byte piece `chunk` of key row `row` lies inside a tile that TMA wrote with the
@@ -243,11 +243,11 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         if (t < ntiles) load_tile(t, t);
         cp_async_commit();
     }
-    if (SHARED && warp == DEC_WARPS - 1) {                         // how the row's prefix was cut, under the copies (read behind the tiles' barriers)
-        const PrefixPart t = prefix_find(p.groups, prefix_chunk(p.groups), row, true);
+    pdl_wait();                                                    // q and the newest key and value are the previous kernel's
+    if (SHARED && warp == DEC_WARPS - 1) {                         // how the row's prefix was cut (read behind the tiles' barriers)
+        const PrefixPart t = p.groups.groups > 0 ? prefix_find(p.groups, max(1, __ldcg(p.pre_chunk)), row, true) : PrefixPart{};
         if (lane == 0) s_part = t;
     }
-    pdl_wait();                                                    // q and the newest key and value are the previous kernel's
     const int newest = ctx - 1;                                    // the only cached position written during this step
     if (p.cos_t && range_position(newest, p.max_pos) != MIE_RANGE_OK) {   // no row of the tables for this position
         // reported; the block goes on without rotating (it takes part in the merge's barriers and counters)
@@ -475,6 +475,28 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         }
     }
     __syncthreads();
+    // SHARED, a row left whole: the weights of its own part and of its prefix's ranges, a warp a head
+    __shared__ float pre_w[SHARED ? 16 : 1][SHARED ? PREFIX_MAX_SPLITS : 1], pre_own[16];
+    int64_t pre_at = 0;
+    int pre_n = 0;
+    if (SHARED && s_part.rows > 0) {
+        pre_at = s_part.slot0 + (int64_t)(row - s_part.first_row) * s_part.splits;
+        pre_n = s_part.splits <= PREFIX_MAX_SPLITS && pre_at + s_part.splits <= p.pre_slots ? s_part.splits : 0;
+    }
+    if (SHARED && eff == 1 && pre_n > 0) {
+        for (int g = warp; g < gn; g += DEC_WARPS) {
+            const float* lse = p.pre_lse + pre_at * p.num_heads + kvh * G + g0 + g;
+            const float a = lane < pre_n ? __ldcg(lse + (int64_t)lane * p.num_heads) : -INFINITY;
+            const float b = lane + 32 < pre_n ? __ldcg(lse + (int64_t)(lane + 32) * p.num_heads) : -INFINITY;
+            const float mm = fmaxf(warp_max(fmaxf(a, b)), c_lse[g]), ref = mm == -INFINITY ? 0.f : mm;
+            const float own = fast_exp2(c_lse[g] - ref), wa = fast_exp2(a - ref), wb = fast_exp2(b - ref);
+            const float sum = warp_sum(wa + wb) + own, inv = sum > 0.f ? __frcp_rn(sum) : sum == 0.f ? 0.f : sum;
+            if (lane < pre_n) pre_w[g][lane] = wa * inv;
+            if (lane + 32 < pre_n) pre_w[g][lane + 32] = wb * inv;
+            if (lane == 0) pre_own[g] = own * inv;
+        }
+        __syncthreads();
+    }
     for (int idx = threadIdx.x; idx < gn * (D / 4); idx += DEC_WARPS * 32) {      // one thread: one head, four dimensions
         const int g = idx / (D / 4), d = (idx - g * (D / 4)) * 4;
         float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -485,22 +507,16 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
             val.x += f * v.x; val.y += f * v.y; val.z += f * v.z; val.w += f * v.w;
         }
         const int head = kvh * G + g0 + g;
-        if (SHARED && eff == 1 && s_part.rows > 0 && s_part.splits > 0) {
-            const int64_t at = s_part.slot0 + (int64_t)(row - s_part.first_row) * s_part.splits;
-            const int S2 = at + s_part.splits <= p.pre_slots ? s_part.splits : 0;
-            float mm = c_lse[g];
-            for (int s2 = 0; s2 < S2; ++s2) mm = fmaxf(mm, __ldcg(p.pre_lse + (at + s2) * p.num_heads + head));
-            const float ref = mm == -INFINITY ? 0.f : mm;
-            float w = fast_exp2(c_lse[g] - ref), wsum = w;
-            val.x *= w; val.y *= w; val.z *= w; val.w *= w;
-            for (int s2 = 0; s2 < S2; ++s2) {
-                w = fast_exp2(__ldcg(p.pre_lse + (at + s2) * p.num_heads + head) - ref);
-                const float4 part = __ldcg(reinterpret_cast<const float4*>(p.pre_o + ((at + s2) * p.num_heads + head) * D + d));
+        if (SHARED && eff == 1 && pre_n > 0) {                     // what is left of the row's prefix, range by range, by the weights worked out above
+            const float w0 = pre_own[g];
+            val.x *= w0; val.y *= w0; val.z *= w0; val.w *= w0;
+            const float* from = p.pre_o + (pre_at * p.num_heads + head) * D + d;
+#pragma unroll 6
+            for (int s2 = 0; s2 < pre_n; ++s2) {
+                const float w = pre_w[g][s2];
+                const float4 part = __ldcg(reinterpret_cast<const float4*>(from + (int64_t)s2 * p.num_heads * D));
                 val.x += w * part.x; val.y += w * part.y; val.z += w * part.z; val.w += w * part.w;
-                wsum += w;
             }
-            const float inv = wsum > 0.f ? __frcp_rn(wsum) : 0.f;
-            val.x *= inv; val.y *= inv; val.z *= inv; val.w *= inv;
         }
         if (eff == 1) {
             if (p.out32) {
@@ -574,18 +590,13 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         const int64_t base = ((int64_t)row * p.num_heads + head) * p.splits;
         float mm = -INFINITY;
         for (int s2 = 0; s2 < eff; ++s2) mm = fmaxf(mm, __ldcg(p.part_lse + base + s2));
-        int64_t at = 0;                                            // SHARED: the row's results of its prefix come first
-        int S2 = 0;
-        if (SHARED && s_part.rows > 0) {
-            at = s_part.slot0 + (int64_t)(row - s_part.first_row) * s_part.splits;
-            S2 = at + s_part.splits <= p.pre_slots ? s_part.splits : 0;
-            for (int s2 = 0; s2 < S2; ++s2) mm = fmaxf(mm, __ldcg(p.pre_lse + (at + s2) * p.num_heads + head));
-        }
+        if (SHARED) for (int s2 = 0; s2 < pre_n; ++s2) mm = fmaxf(mm, __ldcg(p.pre_lse + (pre_at + s2) * p.num_heads + head));      // the row's prefix's results come first
         float acc = 0.f, wsum = 0.f;
         if (SHARED) {
-            for (int s2 = 0; s2 < S2; ++s2) {
-                const float w = fast_exp2(__ldcg(p.pre_lse + (at + s2) * p.num_heads + head) - (mm == -INFINITY ? 0.f : mm));
-                acc += w * __ldcg(p.pre_o + ((at + s2) * p.num_heads + head) * D + d);
+#pragma unroll 4
+            for (int s2 = 0; s2 < pre_n; ++s2) {
+                const float w = fast_exp2(__ldcg(p.pre_lse + (pre_at + s2) * p.num_heads + head) - (mm == -INFINITY ? 0.f : mm));
+                acc += w * __ldcg(p.pre_o + ((pre_at + s2) * p.num_heads + head) * D + d);
                 wsum += w;
             }
         }
@@ -664,13 +675,14 @@ static int decode_attention_launch(const void* q, int64_t q_stride, const void* 
                                    int64_t check_pages = 0, int* report = nullptr, int min_part_tiles = 0,
                                    const float* cos_t = nullptr, const float* sin_t = nullptr, int max_pos = 0, bool out_f32 = false,
                                    const ScoreMods* mods = nullptr, int keep = 0, const PrefixGroups* groups = nullptr,
-                                   const float* pre_o = nullptr, const float* pre_lse = nullptr, int64_t pre_slots = 0) {
+                                   const float* pre_o = nullptr, const float* pre_lse = nullptr, const int* pre_chunk = nullptr,
+                                   int64_t pre_slots = 0) {
     if (num_rows <= 0) return 0;
     if (head_dim < 16 || head_dim > DEC_MAX_D || head_dim % 16) return MIE_ERR_BAD_ARG;
     if (num_kv_heads <= 0 || num_heads % num_kv_heads) return MIE_ERR_BAD_ARG;
     if (page_size < 1 || (page_size & (page_size - 1))) return MIE_ERR_BAD_ARG;
     const bool cluster = splits > 1 && !part_o && !part_lse && !counters;     // no scratch given: merge inside a cluster
-    if (SHARED && (cluster || !groups || window != 0)) return MIE_ERR_BAD_ARG;
+    if (SHARED && (cluster || !groups || window != 0 || (groups->groups > 0 && (!pre_o || !pre_lse || !pre_chunk)))) return MIE_ERR_BAD_ARG;
     if (splits < 1 || (splits > 1 && !cluster && (!part_o || !part_lse || !counters))) return MIE_ERR_BAD_ARG;
     if (cluster && splits != 2 && splits != 4 && splits != 8) return MIE_ERR_BAD_ARG;
     if (num_rows > 65535) return MIE_ERR_TOO_LARGE;
@@ -695,7 +707,7 @@ static int decode_attention_launch(const void* q, int64_t q_stride, const void* 
     p.modded = p.mods.softcap > 0.f || p.mods.dist_bias != nullptr || p.mods.slope != nullptr;
     p.check_pages = check_pages; p.report = report;
     p.groups = groups ? *groups : PrefixGroups{};
-    p.pre_o = pre_o; p.pre_lse = pre_lse; p.pre_slots = pre_slots;
+    p.pre_o = pre_o; p.pre_lse = pre_lse; p.pre_chunk = pre_chunk; p.pre_slots = pre_slots;
     if ((cos_t != nullptr) != (sin_t != nullptr) || (cos_t && (head_dim % 32 || max_pos <= 0))) return MIE_ERR_BAD_ARG;
     p.cos_t = cos_t; p.sin_t = sin_t; p.max_pos = max_pos;
     // TMA copies (see the kernel): head sizes 64 and 128, pages of 8 positions or more, a caller that says

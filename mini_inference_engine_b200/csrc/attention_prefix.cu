@@ -21,7 +21,7 @@ struct PrefixParams {
     const int* block_tables; int table_stride;
     const int* row_q_start; const int* row_q_len;
     PrefixGroups groups;
-    float* part_o; float* part_lse; int64_t most_slots;
+    float* part_o; float* part_lse; int64_t most_slots; int* chunk;       // chunk: how the prefixes are cut, for the kernel behind
     int num_heads, num_kv_heads, page_size, page_shift, chunks, chunk_heads;       // a unit: up to chunk_heads query heads of a key head, `chunks` units each
     float scale_log2e;
     int64_t num_pages; int* report; int* error;
@@ -41,16 +41,19 @@ prefix_attention_kernel(const PrefixParams p) {
     bf16* k_s = reinterpret_cast<bf16*>(smem_raw);         // [2][64][DP]
     bf16* v_s = k_s + 2 * PFX_TILE * DP;
     __shared__ PrefixPart s_part;
+    __shared__ int s_chunk;
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, tq = lane & 3;
     if (warp == 0) {
-        const PrefixPart t = prefix_find(p.groups, prefix_chunk(p.groups), (int)blockIdx.x, false);
-        if (lane == 0) s_part = t;
+        const int chunk = prefix_chunk(p.groups);
+        const PrefixPart t = prefix_find(p.groups, chunk, (int)blockIdx.x, false);
+        if (lane == 0) { s_part = t; s_chunk = chunk; }
     }
     __syncthreads();
     const PrefixPart t = s_part;
     if (t.rows == 0 || t.splits == 0) {
         pdl_wait();                                        // a block without work waits too: see common.cuh
+        if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = s_chunk;
         return;
     }
     int index = (int)blockIdx.x - t.item0;
@@ -87,6 +90,7 @@ prefix_attention_kernel(const PrefixParams p) {
     load_tile(0, 0);                                       // the prefix is older than the step: before the wait
     cp_async_commit();
     pdl_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = s_chunk;
 
     unsigned qf[KSTEPS][4];
     const bf16* q_of[2];                                   // this lane's two pairs: quad and quad + 8 of the warp's sixteen
@@ -232,6 +236,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
     __shared__ PrefixPart s_part;
+    __shared__ int s_chunk;
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char* tiles = smem_dyn + (base - smem_u32(smem_dyn));
     auto q_off = [&](int u) { return (uint32_t)u * TILE; };
@@ -240,13 +245,15 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        const PrefixPart t = prefix_find(p.groups, prefix_chunk(p.groups), (int)blockIdx.x, false);
-        if (lane == 0) s_part = t;
+        const int chunk = prefix_chunk(p.groups);
+        const PrefixPart t = prefix_find(p.groups, chunk, (int)blockIdx.x, false);
+        if (lane == 0) { s_part = t; s_chunk = chunk; }
     }
     __syncthreads();
     const PrefixPart t = s_part;
     if (t.rows == 0 || t.splits == 0) {
         pdl_wait();                                        // a block without work waits too: see common.cuh
+        if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = s_chunk;
         return;
     }
     int index = (int)blockIdx.x - t.item0;
@@ -310,6 +317,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     // Tensor memory is taken behind the wait, and the next kernel let in behind that: a block that held it before the kernels in front are done could keep
     // it from a block of theirs, and one that came later from this one.
     pdl_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = s_chunk;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -558,14 +566,14 @@ extern "C" long long mie_prefix_layout(int num_rows, int num_heads, int num_kv_h
 extern "C" int mie_prefix_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const int* block_tables, int table_stride,
                                     const int* row_q_start, const int* row_q_len, int num_rows, const int* group_start, const int* group_prefix, int groups,
                                     int num_heads, int num_kv_heads, int head_dim, int page_size, float scale, const int* layout, float* part_o,
-                                    float* part_lse, long long most_slots, long long num_pages, cudaStream_t stream) {
+                                    float* part_lse, int* chunk, long long most_slots, long long num_pages, cudaStream_t stream) {
     if (num_rows <= 0 || groups <= 0) return 0;
     if (num_kv_heads <= 0 || num_heads % num_kv_heads) return MIE_ERR_BAD_ARG;
     if (page_size < 1 || (page_size & (page_size - 1))) return MIE_ERR_BAD_ARG;
     PrefixParams p = {};
     p.q = (const bf16*)q; p.q_stride = q_stride; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache;
     p.block_tables = block_tables; p.table_stride = table_stride; p.row_q_start = row_q_start; p.row_q_len = row_q_len;
-    p.part_o = part_o; p.part_lse = part_lse; p.most_slots = most_slots;
+    p.part_o = part_o; p.part_lse = part_lse; p.most_slots = most_slots; p.chunk = chunk;
     p.num_heads = num_heads; p.num_kv_heads = num_kv_heads; p.page_size = page_size;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     p.chunk_heads = layout[0]; p.chunks = layout[1];

@@ -1,6 +1,6 @@
 // How the work on shared prefixes is cut up, decided on the device from the step's groups alone, so that a captured step follows whatever groups
-// and lengths its inputs hold.  Two kernels ask and have to agree: the one that attends over the prefixes and the one that joins its results
-// with the rows' own keys.
+// and lengths its inputs hold.  The kernel that attends over the prefixes decides and leaves the length of its ranges (`chunk`) to the one that joins its
+// results with the rows' own keys.
 //
 // Group g is the rows start[g] .. start[g + 1] - 1; they share their first prefix[g] keys.  For a unit (a key head, or a part of its query heads)
 // the (row, head) pairs of a group go in tiles of up to `tile_rows` rows, and the prefix, counted in steps of PREFIX_STEP keys, is cut
@@ -71,36 +71,79 @@ __host__ __device__ __forceinline__ long long prefix_most_slots(int rows, int un
 }
 
 #ifdef __CUDACC__
-// Steps a range, for every lane the same; by a whole warp: lane l weighs up cutting the longest prefix into l + 1 and l + 33 ranges.
+// Steps a range, for every lane the same; by a whole warp: lane l weighs up cutting the longest prefix into l + 1 and l + 33 ranges.  A lane holds a
+// group (of up to 32: the host's arithmetic above for more); 13.3 -> 10 us for the two launches of a step of two rows behind 208 keys against every
+// lane reading every group.
 __device__ __forceinline__ int prefix_chunk(const PrefixGroups& p) {
-    const int lane = threadIdx.x & 31, most = prefix_most_steps(p);
-    long long best = 0x7fffffffffffffffll;
+    const int lane = threadIdx.x & 31;
+    const bool few = p.groups <= 32;
+    PrefixPart mine = {};
+    if (few && lane < p.groups) mine = prefix_group(p, lane);
+    int most;
+    if (few) {
+        most = mine.tiles ? mine.steps : 1;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    } else most = prefix_most_steps(p);
+    const unsigned whole = mine.tiles ? (unsigned)p.units * mine.tiles : 0u;
+    unsigned best = 0xffffffffu;
     int chunk = most;
-#pragma unroll 1
-    for (int s = lane + 1; s <= PREFIX_MAX_SPLITS && s < most + 32; s += 32) {
-        int c;
-        const long long cost = prefix_cost(p, most, s, c);
-        if (cost >= 0 && cost < best) { best = cost; chunk = c; }
+#pragma unroll
+    for (int turn = 0; turn < 2; ++turn) {
+        const int s = lane + 1 + 32 * turn;
+        if (turn && most <= 32) break;
+        unsigned cost = 0xffffffffu;
+        int c = max(1, (most + s - 1) / s);
+        if (few) {
+            unsigned long long items = 0;
+            for (int g = 0; g < p.groups; ++g) {
+                const int steps = __shfl_sync(0xffffffffu, mine.steps, g);
+                items += (unsigned long long)__shfl_sync(0xffffffffu, whole, g) * prefix_splits(steps, c);
+            }
+            const unsigned n = (unsigned)min(items, 0x3fffffffull);
+            if (s == 1 || n <= 2u * p.places) cost = ((n + p.places - 1) / p.places) * (unsigned)(c + PREFIX_COST_START);
+        } else {
+            const long long l = prefix_cost(p, most, s, c);
+            if (l >= 0) cost = (unsigned)min(l, 0xfffffffell);
+        }
+        if (s < most + 32 && cost < best) { best = cost; chunk = c; }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const long long ob = __shfl_xor_sync(0xffffffffu, best, o);
+        const unsigned ob = __shfl_xor_sync(0xffffffffu, best, o);
         const int oc = __shfl_xor_sync(0xffffffffu, chunk, o);
         if (ob < best || (ob == best && oc > chunk)) { best = ob; chunk = oc; }
     }
     return chunk;
 }
-// The group that item `item` (or, with by_row, row `item`) belongs to; rows 0 where there is none.
+// The group that item `item` (or, with by_row, row `item`) belongs to; rows 0 where there is none.  By a whole warp, for every lane the same.
 __device__ __forceinline__ PrefixPart prefix_find(const PrefixGroups& p, int chunk, int item, bool by_row) {
+    const int lane = threadIdx.x & 31;
     int items = 0, slots = 0;
-    for (int g = 0; g < p.groups; ++g) {
-        PrefixPart t = prefix_group(p, g);
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+        PrefixPart t = {};
+        if (g0 + lane < p.groups) t = prefix_group(p, g0 + lane);
         t.splits = t.tiles ? prefix_splits(t.steps, chunk) : 0;
-        t.item0 = items;
-        t.slot0 = slots;
-        items += p.units * t.tiles * t.splits;
-        slots += t.rows * t.splits;
-        if (by_row ? item >= t.first_row && item < t.first_row + t.rows : item < items) return t;
+        const int n = p.units * t.tiles * t.splits, k = t.rows * t.splits;
+        int ni = n, ki = k;                                // sums up to this lane's group
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int a = __shfl_up_sync(0xffffffffu, ni, o), b = __shfl_up_sync(0xffffffffu, ki, o);
+            if (lane >= o) { ni += a; ki += b; }
+        }
+        t.item0 = items + ni - n;
+        t.slot0 = slots + ki - k;
+        const unsigned hit = __ballot_sync(0xffffffffu, by_row ? item >= t.first_row && item < t.first_row + t.rows : item >= t.item0 && item < t.item0 + n);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            t.first_row = __shfl_sync(0xffffffffu, t.first_row, l); t.rows = __shfl_sync(0xffffffffu, t.rows, l);
+            t.keys = __shfl_sync(0xffffffffu, t.keys, l); t.tiles = __shfl_sync(0xffffffffu, t.tiles, l);
+            t.steps = __shfl_sync(0xffffffffu, t.steps, l); t.splits = __shfl_sync(0xffffffffu, t.splits, l);
+            t.slot0 = __shfl_sync(0xffffffffu, t.slot0, l); t.item0 = __shfl_sync(0xffffffffu, t.item0, l);
+            return t;
+        }
+        items += __shfl_sync(0xffffffffu, ni, 31);
+        slots += __shfl_sync(0xffffffffu, ki, 31);
     }
     return PrefixPart{};
 }

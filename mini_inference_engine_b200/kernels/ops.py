@@ -807,18 +807,19 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
         counters = _workspace(q.device, "decode_counters", rows * units, torch.int32)
     shared = groups > 0 and max_prefix != 0
     layout, slots = _prefix_layout(rows, num_heads, num_kv_heads, head_dim, page_size, num_sms(q.device))
-    pre_o = pre_lse = None
+    pre_o = pre_lse = pre_chunk = None
     if shared:
         pre_o = _workspace(q.device, "prefix_o", slots * num_heads * head_dim, torch.float32)
         pre_lse = _workspace(q.device, "prefix_lse", slots * num_heads, torch.float32)
+        pre_chunk = _workspace(q.device, "prefix_chunk", 1, torch.int32)
         _check(load("attention_prefix").mie_prefix_attention(
             _ptr(q), ctypes.c_int64(q_stride), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(row_q_start), _ptr(row_q_len),
             rows, _ptr(group_start), _ptr(group_prefix), groups, num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale), layout, _ptr(pre_o),
-            _ptr(pre_lse), ctypes.c_longlong(slots), ctypes.c_longlong(k_cache.shape[0]), _stream()), "shared_prefix_attention (prefixes)")
+            _ptr(pre_lse), _ptr(pre_chunk), ctypes.c_longlong(slots), ctypes.c_longlong(k_cache.shape[0]), _stream()), "shared_prefix_attention (prefixes)")
     _check(load("attention_decode_shared").mie_decode_attention_shared(
         _ptr(q), ctypes.c_int64(q_stride), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(row_q_start), _ptr(row_q_len),
         _ptr(row_ctx_len), rows, _ptr(group_start), _ptr(group_prefix), groups if shared else 0, layout, _ptr(pre_o), _ptr(pre_lse),
-        ctypes.c_longlong(slots), _ptr(out), num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale), int(splits), _ptr(part_o),
+        _ptr(pre_chunk), ctypes.c_longlong(slots), _ptr(out), num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale), int(splits), _ptr(part_o),
         _ptr(part_lse), _ptr(counters), int(stages), ctypes.c_int64(k_cache.shape[0] if tma else 0), ctypes.c_int64(k_cache.shape[0]), int(part_tiles),
         int(out.dtype == torch.float32), _stream()), "shared_prefix_attention (own keys)")
     return out
