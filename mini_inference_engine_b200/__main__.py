@@ -65,10 +65,14 @@ def cmd_generate(args):
     else:
         rng = random.Random(args.seed)
         prompts = [[rng.randrange(eng.vocab_size) for _ in range(args.prompt_len)] for _ in range(args.num_prompts)]
-    sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, ignore_eos=args.ignore_eos)
-    for o in eng.generate(prompts, sp):
-        print(json.dumps({"seq_id": o.seq_id, "prompt_len": o.prompt_len, "output_ids": o.output_ids,
-                          "ttft": o.ttft, "latency": o.latency}))
+    sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, ignore_eos=args.ignore_eos,
+                        repetition_penalty=args.repetition_penalty, presence_penalty=args.presence_penalty,
+                        frequency_penalty=args.frequency_penalty, logprobs=args.logprobs)
+    for o in eng.generate(prompts, sp, n=args.n):
+        line = {"seq_id": o.seq_id, "prompt_len": o.prompt_len, "output_ids": o.output_ids, "ttft": o.ttft, "latency": o.latency}
+        if o.logprobs is not None:
+            line["logprobs"] = o.logprobs
+        print(json.dumps(line))
 
 
 def decode_latency(eng, batch: int, prompt: int, steps: int) -> float:
@@ -237,6 +241,11 @@ def main(argv=None):
     g.add_argument("--max-tokens", type=int, default=128)
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--ignore-eos", action="store_true")
+    g.add_argument("--n", type=int, default=1, help="answers to every prompt (they share its pages)")
+    g.add_argument("--repetition-penalty", type=float, default=1.0)
+    g.add_argument("--presence-penalty", type=float, default=0.0)
+    g.add_argument("--frequency-penalty", type=float, default=0.0)
+    g.add_argument("--logprobs", action="store_true", help="print every token's log-probability")
     g.set_defaults(fn=cmd_generate)
 
     l = sub.add_parser("latency", help="median ms per pure-decode step at several batch sizes")

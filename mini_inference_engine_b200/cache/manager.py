@@ -46,6 +46,7 @@ class RequestCache:
     first_live: list = field(default_factory=list)
     state_slot: int = 0
     num_computed: int = 0
+    shared: int = 0                   # the first that many pages of every table belong to a prefix that the request shares
     version: int = 0                  # counts the changes of ``tables`` (the manager bumps it)
     _arrays: tuple = field(default=(-1, None), repr=False, compare=False)
 
@@ -67,6 +68,7 @@ class CacheManager:
         counts = num_pages if isinstance(num_pages, (list, tuple)) else [num_pages] * len(groups)
         self.pools = [PagePool(n) for n in counts]
         self._windowed = any(g.window is not None or g.chunk is not None for g in self.groups)
+        self.pinned = [0] * len(self.groups)          # pages that prefixes hold: no request's end gives them back
         # slot 0 is the scratch slot of padding rows, like page 0
         self.state_pool = PagePool(num_state_slots + 1) if num_state_slots > 0 else None
 
@@ -101,6 +103,29 @@ class CacheManager:
             rc.tables = [[] for _ in self.groups]
             rc.version += 1
             rc.first_live = [0 for _ in self.groups]
+
+    # ------------------------------------------------------------------ shared prefixes
+    def can_share(self) -> bool:
+        """Whether requests can share the pages of a prefix: every layer keeps all positions.  (What a layer keeps of a request beside its pages is not
+        shared: a caller whose model has such a state does not.)"""
+        return not self._windowed
+
+    def adopt(self, rc: RequestCache, source: RequestCache, pages: int) -> None:
+        """``rc``, which holds nothing yet, begins with the first ``pages`` pages of ``source``: their positions count as computed, and the pages stay
+        ``source``'s (``free`` leaves them alone)."""
+        if any(rc.tables) or rc.num_computed:
+            raise PageError("a request that holds pages already cannot begin with another's")
+        if pages * self.block_size > source.num_computed:
+            raise PageError(f"{pages} pages of a prefix of {source.num_computed} positions")
+        rc.tables = [list(t[:pages]) for t in source.tables]
+        rc.first_live = [0 for _ in self.groups]
+        rc.version += 1
+        rc.shared, rc.num_computed = pages, pages * self.block_size
+
+    def pin(self, rc: RequestCache, on: bool = True) -> None:
+        """Counts the pages that ``rc`` (a prefix) holds as given away for as long as it lives."""
+        for g, t in enumerate(rc.tables):
+            self.pinned[g] += len(t) if on else -len(t)
 
     # ------------------------------------------------------------------ reserve / advance / free
     def can_reserve(self, rc: RequestCache, n_new: int, watermark: int = 0) -> bool:
@@ -155,11 +180,11 @@ class CacheManager:
         """Everything the request holds goes back (end of the request, or preemption)."""
         self._ensure_tables(rc)
         for g in range(len(self.groups)):
-            self.pools[g].give_back([p for p in rc.tables[g] if p != RELEASED])
+            self.pools[g].give_back([p for p in rc.tables[g][rc.shared:] if p != RELEASED])
         rc.tables = [[] for _ in self.groups]
         rc.version += 1
         rc.first_live = [0 for _ in self.groups]
-        rc.num_computed = 0
+        rc.num_computed = rc.shared = 0
         if self.state_pool is not None and rc.state_slot:
             self.state_pool.give_back([rc.state_slot])
         rc.state_slot = 0

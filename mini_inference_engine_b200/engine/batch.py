@@ -15,7 +15,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from ..parts.base import StepContext
+from ..parts.base import PrefixGroups, StepContext
 
 
 @dataclass
@@ -45,12 +45,14 @@ class BatchBuilder:
 
     # ------------------------------------------------------------------ packing
     def pack(self, rows: list[BatchRow], pad_rows: int | None = None, table_width: int | None = None,
-             extras: dict | None = None):
+             extras: dict | None = None, shared: list | None = None, most_groups: int = 0):
         """Returns (numpy int32 buffer, layout dict).  ``pad_rows`` pads with scratch rows (one
         token at position 0 in page 0, state slot 0) up to that many rows, and ``table_width`` fixes
         the block-table width -- both for steps replayed from a captured graph, whose shapes are
         static.  ``extras`` are small per-step arrays of 4- or 8-byte elements (sampling inputs)
-        that ride in the same transfer; they come back as ``ctx.extras[name]`` on the device."""
+        that ride in the same transfer; they come back as ``ctx.extras[name]`` on the device.  ``shared``: groups of
+        rows that share a prefix as (rows, first row, positions), in row order; ``most_groups`` fixes how many there is room for.
+        They come back as ``ctx.prefix``."""
         R_real = len(rows)
         R = max(R_real, pad_rows or 0)
         lens = [len(r.tokens) for r in rows]
@@ -82,6 +84,11 @@ class BatchBuilder:
         for g in range(self.num_groups):
             off[f"tables{g}"] = (n, R * width)
             n = _align(n + R * width)
+        num_groups = max(most_groups, len(shared)) if shared is not None else 0
+        if shared is not None:
+            for name, size in (("group_start", 2 * num_groups + 1), ("group_prefix", 2 * num_groups)):
+                off[name] = (n, size)
+                n = _align(n + size)
         extra_off = {}
         for name, arr in (extras or {}).items():
             arr = np.ascontiguousarray(arr)
@@ -98,6 +105,17 @@ class BatchBuilder:
             o, s = off[name]
             return buf[o:o + s]
 
+        if shared is not None:
+            # every group's rows, and those between it and the next as a group without a prefix
+            gs, gp = seg("group_start"), seg("group_prefix")
+            at = 0
+            for i, (count, first, positions) in enumerate(shared):
+                if first < at or first + count > R_real:
+                    raise ValueError("groups of shared prefixes lie one behind another within the rows")
+                gs[2 * i:2 * i + 2] = first, first + count
+                gp[2 * i] = positions
+                at = first + count
+            gs[2 * len(shared):] = at
         seg("row_q_start")[:] = q_start[:R]
         seg("row_q_len")[:] = q_len
         seg("row_ctx_len")[:] = ctx_len
@@ -141,6 +159,7 @@ class BatchBuilder:
         layout = dict(off=off, T=T, R=R, W=W, width=width, size=n, real_rows=R_real,
                       extras={k: v[:3] for k, v in extra_off.items()},
                       max_q_len=int(q_len.max()) if R else 0, max_ctx_len=int(ctx_len.max()) if R else 0,
+                      shared=shared is not None,
                       q_len=q_len.tolist(), ctx_len=ctx_len.tolist(), q_start=q_start[:R].tolist(),
                       state_slots=[r.state_slot for r in rows] + [0] * (R - R_real))
         return buf, layout
@@ -179,7 +198,11 @@ class BatchBuilder:
             o, s = off[name]
             return dev[o:o + s]
 
+        prefix = None
+        if layout.get("shared"):
+            prefix = PrefixGroups(seg("group_start"), seg("group_prefix"), layout["max_ctx_len"], layout["max_ctx_len"])
         return StepContext(
+            prefix=prefix,
             num_tokens=T, num_rows=R, token_ids=seg("token_ids"), positions=seg("positions"),
             token_row=seg("token_row"), row_q_start=seg("row_q_start"), row_q_len=seg("row_q_len"),
             row_ctx_len=seg("row_ctx_len"), state_slots=seg("state_slots"),

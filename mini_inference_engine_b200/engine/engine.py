@@ -19,12 +19,14 @@ import torch
 
 from ..config import EngineConfig, load_config
 from ..kernels import gemm_tc, ops
-from ..kernels.attention import captured_context_bounds
+from ..kernels.attention import captured_context_bounds, sharing_pays
 from ..models.decoder import DecoderModel
 from ..parts.base import Runtime
 from ..sampling.params import SamplingParams
+from ..sampling.rules import RuleBook, mask_words
 from ..sampling.sampler import Sampler
 from ..weights import read_model_folder
+from .prefix import Prefix, shared_groups
 from .runner import ModelRunner
 from .scheduler import Scheduler
 from .sequence import Sequence
@@ -40,6 +42,7 @@ class RequestOutput:
     text: str | None
     ttft: float | None          # seconds from arrival to the first generated token
     latency: float | None       # seconds from arrival to the end
+    logprobs: list | None = None        # of the output's tokens, where the request asked for them
 
 
 PENDING = -1          # in token_ids: a token that the step in flight is sampling
@@ -49,8 +52,9 @@ class _InFlight:
     """A launched step whose sampled tokens the host has not read yet.  ``sources``: (pinned row, count)
     in the order of ``seqs`` -- one entry, or two when the step ran as two graphs."""
 
-    def __init__(self, seqs, places, ending, sources, event):
+    def __init__(self, seqs, places, ending, sources, logprob_sources, event):
         self.seqs, self.places, self.ending, self.sources, self.event = seqs, places, ending, sources, event
+        self.logprob_sources = logprob_sources        # (pinned row or None, count), as ``sources``
 
     def tokens(self) -> list:
         out = []
@@ -58,11 +62,27 @@ class _InFlight:
             out += row[:n].tolist()
         return out
 
+    def logprobs(self) -> list:
+        out = []
+        for row, n in self.logprob_sources:
+            out += [None] * n if row is None else row[:n].tolist()
+        return out
+
+
+class _DeviceMemory:
+    """Memory that a captured graph writes, for ``torch.as_tensor``: a view that does not own it.  A tensor that did would keep the graphs captured
+    after this one from using the memory again, as they may: what one replay leaves is read before the next."""
+
+    def __init__(self, t):
+        self.__cuda_array_interface__ = dict(shape=tuple(t.shape), typestr="<f4", data=(t.data_ptr(), False), version=2)
+
 
 class _DecodeGraph:
-    def __init__(self, graph, layout, buffer, tokens, kernels):
+    def __init__(self, graph, layout, buffer, tokens, kernels, ctx, logits):
         self.graph, self.layout, self.buffer, self.tokens = graph, layout, buffer, tokens
         self.kernels = kernels        # kernels of this package inside the captured step
+        self.ctx = ctx
+        self.logits = torch.as_tensor(_DeviceMemory(logits), device=logits.device) if logits.numel() else logits      # what a replay leaves
 
 
 def _nvtx_range(name):
@@ -130,6 +150,13 @@ class LLMEngine:
         self._sampled = torch.zeros(most + 8, dtype=torch.int32, device=self.device)   # the last step's tokens, on the device
         self._turn = 0
         self._in_flight = None
+        self.rules = RuleBook(self.device, self.cfg.max_model_len, self.vocab_size)
+        self._logprobs = self._pinned_logprobs = None        # made when a request first asks for them
+        self.can_share = self.cache.can_share() and not layout.state         # whether requests can share pages
+        self.prefixes: list = []                 # the prefixes that requests may begin with (``add_prefix``)
+        self._shared_graphs: dict = {}           # (bucket, context bound) -> captured decode step over shared prefixes, or None: it has run once
+        self._bytes_per_key = max((2 * n.num_kv_heads * n.head_dim * torch.empty((), dtype=dtype).element_size()
+                                   for _, n in layout.kv.values()), default=0)
         self.graphs: dict = {}                   # (bucket, context bound) -> captured decode step
         self.graph_sizes: list = []
         self.graph_bounds: list = []             # the context bounds the buckets were captured for, ascending
@@ -171,13 +198,35 @@ class LLMEngine:
 
     # ------------------------------------------------------------------ CUDA graphs of decode steps
     def _forward_and_sample(self, ctx, tokens_out=None, host_out=None, seed=None):
+        """Returns the step's logits; the tokens go to ``tokens_out``."""
         logits = self.model.step(ctx)
-        if logits.shape[0] == 0:
+        if logits.shape[0]:
+            self.sampler.sample(logits, ctx.extras["temperature"], ctx.extras["request"],
+                                ctx.extras["out_position"], out=tokens_out, seed=seed,
+                                host_out=self._pinned_tokens if host_out is None else host_out,
+                                host_turn=ctx.extras["host_turn"])
+        return logits
+
+    def _choose_under_rules(self, seqs, logits, extras, at: int, turn: int, host_out):
+        """The tokens of ``seqs`` once more where some have rules, chosen from a step's logits under them: over the tokens that the step itself chose.
+        ``at``: the rows' first place among the sampled tokens.  Returns the pinned row that receives the log-probabilities, or None."""
+        if not any(s.params.has_rules for s in seqs):
             return None
-        return self.sampler.sample(logits, ctx.extras["temperature"], ctx.extras["request"],
-                                   ctx.extras["out_position"], out=tokens_out, seed=seed,
-                                   host_out=self._pinned_tokens if host_out is None else host_out,
-                                   host_turn=ctx.extras["host_turn"])
+        k = len(seqs)
+        lp = None
+        if any(s.params.logprobs for s in seqs):
+            if self._logprobs is None:
+                self._logprobs = torch.zeros(self._sampled.numel(), dtype=torch.float32, device=self.device)
+                self._pinned_logprobs = torch.zeros(2, self._sampled.numel(), dtype=torch.float32, pin_memory=True)
+            lp = self._logprobs[at:at + k]
+        tokens = self._sampled[at:at + k]
+        if not self.sampler.sample_ruled(logits[:k], extras, tokens, seqs, self.rules, host_out=host_out, logprob=lp):
+            host_out[turn, :k].copy_(tokens, non_blocking=True)
+        if lp is None:
+            return None
+        row = self._pinned_logprobs[turn, at:at + k]
+        row.copy_(lp, non_blocking=True)
+        return row
 
     @torch.inference_mode()
     def _capture_cuda_graphs(self):
@@ -211,9 +260,10 @@ class LLMEngine:
                 g = torch.cuda.CUDAGraph()
                 before = ops.launches
                 with torch.cuda.graph(g, pool=pool):
-                    self._forward_and_sample(ctx, tokens)
+                    logits = self._forward_and_sample(ctx, tokens)
                 pool = g.pool()
-                self.graphs[bs, bound] = _DecodeGraph(g, layout, static, tokens, ops.launches - before)
+                self.graphs[bs, bound] = _DecodeGraph(g, layout, static, tokens, ops.launches - before, ctx, logits)
+                del logits                                          # (its memory goes to the graphs behind)
         torch.cuda.synchronize()
         self._graph_pool = pool
         self.graph_sizes = sizes
@@ -227,6 +277,53 @@ class LLMEngine:
         included) is ``context``."""
         bs = next(s for s in self.graph_sizes if s >= rows)
         return self.graphs[bs, next(c for c in self.graph_bounds if c >= context)]
+
+    # ------------------------------------------------------------------ CUDA graphs of decode steps over shared prefixes
+    SHARED_GROUPS = 8        # prefixes that the rows of a step may share between them; with more, every row reads its own pages
+
+    def _shared_step(self, dseqs):
+        """The groups of decoding rows that share a prefix, if the step is to read those once a group; else None."""
+        if self.dtype != torch.bfloat16:
+            return None
+        groups = shared_groups(dseqs, self.cfg.block_size)
+        if not groups or len(groups) > self.SHARED_GROUPS or not sharing_pays(groups, self._bytes_per_key):
+            return None
+        return groups
+
+    def _decode_shared(self, drows, extras, groups, context: int):
+        """Runs a decode step whose rows share prefixes: from its bucket's graph, which is captured the second time the bucket occurs (the first time
+        builds kernels and sizes buffers).  Returns (extras on the device, logits)."""
+        b = self.runner.builder
+        bs = next(s for s in self.graph_sizes if s >= len(drows))
+        bound = next(c for c in self.graph_bounds if c >= context)
+        buf, layout = b.pack(drows, pad_rows=bs, table_width=self.max_blocks_per_seq, extras=extras, shared=groups, most_groups=self.SHARED_GROUPS)
+        layout["max_ctx_len"] = bound
+        self.h2d_bytes += buf.nbytes
+        tokens = self._sampled[:bs]
+        seen, g = (bs, bound) in self._shared_graphs, self._shared_graphs.get((bs, bound))
+        if not seen:
+            ctx = b.to_device(buf, layout)
+            ctx.token_feedback = self._sampled
+            logits = self._forward_and_sample(ctx, tokens)
+            self._shared_graphs[bs, bound] = None
+            return ctx.extras, logits
+        if g is None:
+            static = torch.zeros(layout["size"], dtype=torch.int32, device=self.device)
+            ctx = b.to_device(buf, layout, into=static)
+            ctx.token_feedback = self._sampled
+            graph = torch.cuda.CUDAGraph()
+            before = ops.launches
+            with self._capturing(graph):
+                logits = self._forward_and_sample(ctx, tokens)
+            if self._graph_pool is None:
+                self._graph_pool = graph.pool()
+            g = self._shared_graphs[bs, bound] = _DecodeGraph(graph, layout, static, tokens, ops.launches - before, ctx, logits)
+            del logits
+        assert layout["size"] == g.layout["size"]
+        b.to_device(buf, g.layout, into=g.buffer)
+        g.graph.replay()
+        self.num_graph_steps += 1
+        return g.ctx.extras, g.logits
 
     # ------------------------------------------------------------------ CUDA graphs of prompt portions
     PORTION_GRAPH_MIN_TOKENS = 2
@@ -308,40 +405,145 @@ class LLMEngine:
         graph = torch.cuda.CUDAGraph()
         before = ops.launches
         with self._capturing(graph):
-            self._forward_and_sample(ctx, tokens, host_out=self._pinned_portion)
+            logits = self._forward_and_sample(ctx, tokens, host_out=self._pinned_portion)
         if self._graph_pool is None:
             self._graph_pool = graph.pool()
-        g = _DecodeGraph(graph, layout, static, tokens, ops.launches - before)
+        g = _DecodeGraph(graph, layout, static, tokens, ops.launches - before, ctx, logits)
+        del logits
         while len(self._portion_graphs) >= max(1, self.cfg.graph_prompt_portions):
             self._portion_graphs.pop(next(iter(self._portion_graphs)))
         self._portion_graphs[key] = g
         return g
 
     # ------------------------------------------------------------------ requests
-    def add_request(self, prompt, params: SamplingParams | None = None) -> Sequence:
+    def _prompt_ids(self, prompt) -> list:
         if isinstance(prompt, str):
             if self.tokenizer is None:
                 raise ValueError("a text prompt needs a tokenizer in the model folder; pass token ids instead")
             ids = self.tokenizer.encode(prompt)
         else:
             ids = [int(t) for t in prompt]
-        params = params or SamplingParams()
         if not ids:
             raise ValueError("empty prompt")
         bad = [t for t in ids if not 0 <= t < self.vocab_size]
         if bad:
             raise ValueError(f"token id {bad[0]} is outside the vocabulary [0, {self.vocab_size})")
+        return ids
+
+    @torch.inference_mode()
+    def add_prefix(self, prompt) -> Prefix:
+        """Computes the keys and values of ``prompt`` (as many of its tokens as fill whole pages) once, for requests that begin with it
+        (``add_request(..., prefix=)``): they share the pages, and steps in which many rows share them read them once.  The pages are held until
+        ``release_prefix``.  Refused with ValueError where a layer keeps a window, a block of positions or a state, and where the
+        pages would leave a request that waits or runs too few ever to end."""
+        ids = self._prompt_ids(prompt)
+        pages = len(ids) // self.cfg.block_size
+        if not self.can_share:
+            raise ValueError("requests of this model cannot share pages: a layer keeps a window, a block of positions or a state per request")
+        if not pages:
+            raise ValueError(f"a prefix of {len(ids)} tokens fills no page of {self.cfg.block_size}")
+        if len(ids) > self.cfg.max_model_len:
+            raise ValueError(f"prefix of {len(ids)} tokens exceeds max_model_len {self.cfg.max_model_len}")
+        p = Prefix(ids[:pages * self.cfg.block_size])
+        live = list(self.scheduler.running) + list(self.scheduler.waiting)
+        for s in live:
+            most = min(s.prompt_len + s.params.max_tokens, self.cfg.max_model_len)
+            if not self.scheduler.can_ever_fit(most, s.prefix_pages, pinned=pages):
+                raise ValueError(f"a prefix of {pages} pages would leave request {s.seq_id} too few")
+        if not self.cache.can_reserve(p.cache, len(p.token_ids), watermark=self.scheduler.watermark):
+            raise ValueError(f"a prefix of {pages} pages, {min(q.num_free for q in self.cache.pools)} free")
+        try:
+            arr = np.asarray(p.token_ids, dtype=np.int32)
+            for a in range(0, arr.size, self.cfg.max_num_batched_tokens):
+                part = arr[a:a + self.cfg.max_num_batched_tokens]
+                self.cache.reserve(p.cache, part.size)
+                ctx = self.runner.builder.build([self.runner.make_row(p.cache, part, ())])
+                ctx.token_feedback = self._sampled
+                self.model.step(ctx)
+                self.cache.advance(p.cache, part.size)
+        except BaseException:
+            self.cache.free(p.cache)
+            raise
+        self.cache.pin(p.cache)
+        self.prefixes.append(p)
+        return p
+
+    def release_prefix(self, prefix: Prefix) -> None:
+        """No further request begins with ``prefix``; its pages go back when the last that does has ended."""
+        if prefix not in self.prefixes:
+            raise ValueError("not a prefix of this engine, or released already")
+        prefix.closed = True
+        self.prefixes.remove(prefix)
+        if not prefix.users:
+            self._free_prefix(prefix)
+
+    def _free_prefix(self, prefix: Prefix) -> None:
+        self.cache.pin(prefix.cache, False)
+        self.cache.free(prefix.cache)
+
+    def _ended(self, seq) -> None:
+        """What a request that has ended holds beside its pages goes back."""
+        self.rules.release(seq)
+        if seq.prefix is not None:
+            prefix, seq.prefix = seq.prefix, None
+            prefix.users -= 1
+            if prefix.closed and not prefix.users:
+                self._free_prefix(prefix)
+
+    def add_request(self, prompt, params: SamplingParams | None = None, prefix: Prefix | None = None) -> Sequence:
+        """``prefix``: what the prompt begins with, from ``add_prefix``; the request shares its pages (all of them that lie in front of the prompt's
+        last token)."""
+        ids = self._prompt_ids(prompt)
+        params = params or SamplingParams()
+        if params.logit_bias and max(params.logit_bias) >= self.vocab_size:
+            raise ValueError(f"logit_bias names token {max(params.logit_bias)}, outside the vocabulary [0, {self.vocab_size})")
+        shared = 0
+        if prefix is not None:
+            if prefix not in self.prefixes:
+                raise ValueError("not a prefix of this engine, or released already")
+            shared = min(len(prefix.token_ids), len(ids) - 1) // self.cfg.block_size
+            if ids[:len(prefix.token_ids)] != prefix.token_ids[:len(ids)]:
+                raise ValueError("the prompt does not begin with the prefix")
         if len(ids) > self.cfg.max_model_len:
             raise ValueError(f"prompt of {len(ids)} tokens exceeds max_model_len {self.cfg.max_model_len}")
         if len(ids) + params.max_tokens > self.cfg.max_model_len:     # inference_engine/engine.py:126-127
             params = SamplingParams(**{**params.__dict__, "max_tokens": max(1, self.cfg.max_model_len - len(ids))})
         most = min(len(ids) + params.max_tokens, self.cfg.max_model_len)
-        if not self.scheduler.can_ever_fit(most):
+        if not self.scheduler.can_ever_fit(most, shared):
             raise ValueError(f"a request of {most} positions can never fit the cache "
-                             f"({self.cache.pools[0].num_usable} usable pages of {self.cfg.block_size})")
+                             f"({self.cache.pools[0].num_usable} usable pages of {self.cfg.block_size}, {self.cache.pinned[0]} held by prefixes)")
         seq = Sequence(ids, params)
+        if shared:
+            seq.prefix, seq.prefix_pages = prefix, shared
+            prefix.users += 1
         self.scheduler.add(seq)
         return seq
+
+    # ------------------------------------------------------------------ grammars
+    def _ask_grammars(self) -> list:
+        """Before a step: what every live request's grammar allows next.  A grammar reads the tokens so far, so the step in flight is read first.  Returns
+        the requests that end here (their grammar allows nothing), beside those that ended with the step that was read."""
+        if not any(s.params.grammar is not None for s in (*self.scheduler.running, *self.scheduler.waiting)):
+            return []
+        finished = self.drain()
+        for s in (*self.scheduler.running, *self.scheduler.waiting):
+            if s.params.grammar is None or s.mask_at == len(s.token_ids):
+                continue
+            try:
+                s.mask = mask_words(s.params.grammar.allowed(list(s.output_ids)), self.vocab_size)
+            except BaseException:            # the request goes, the others and the engine stay as they are
+                self._end_now(s)
+                raise
+            s.mask_at = len(s.token_ids)
+            if s.mask is not None and not s.mask.any():
+                self._end_now(s)
+                finished.append(s)
+        return finished
+
+    def _end_now(self, seq) -> None:
+        seq.finish_time = time.perf_counter()
+        self.scheduler.finish(seq)
+        self._ended(seq)
 
     # ------------------------------------------------------------------ one engine step
     def has_work(self) -> bool:
@@ -357,8 +559,10 @@ class LLMEngine:
         -(k+1) in the batch means "entry k of the previous step's samples"), so nothing but the stop
         rules waits for the host: a request that ends by count is known beforehand, one that ends by
         EOS runs one step too many, whose token is dropped."""
+        finished = self._ask_grammars()
         launched = self._launch()
-        finished = self._complete(self._in_flight) if self._in_flight is not None else []
+        if self._in_flight is not None:
+            finished += self._complete(self._in_flight)
         self._in_flight = launched
         # nothing to run ahead of: read the step's tokens now (also keeps the reference's loop
         # `while engine.scheduler.has_work(): engine.step()` complete)
@@ -377,6 +581,8 @@ class LLMEngine:
         if not batch:
             return None
         with _nvtx_range("prepare"):
+            if any(s.prefix is not None for s, _ in batch):    # rows of one prefix side by side (a stable sort: the rest keep their order)
+                batch.sort(key=lambda e: (0, e[0].prefix.serial, e[0].cache.shared) if e[0].prefix is not None else (1, 0, 0))
             rows, sample_seqs, decoding, others = [], [], [], []
             make_row = self.runner.make_row
             for i, (seq, n) in enumerate(batch):
@@ -409,22 +615,30 @@ class LLMEngine:
 
         with _nvtx_range("forward"):
             b = self.runner.builder
-            sources = []
+            sources, logprob_sources = [], []
             if use_graph or (portion_graph and decoding):      # ---- the requests that decode, from their bucket's graph
                 drows = [rows[i] for i in decoding]
                 dseqs = [batch[i][0] for i in decoding]
                 bs = next(s for s in self.graph_sizes if s >= len(drows))
-                g = self.decode_graph(bs, max(seq.cache.num_computed + 1 for seq in dseqs))
-                buf, layout = b.pack(drows, pad_rows=bs, table_width=self.max_blocks_per_seq, extras=extras_for(dseqs, bs))
-                assert layout["size"] == g.layout["size"]
-                b.to_device(buf, g.layout, into=g.buffer)
-                g.graph.replay()
-                self.h2d_bytes += buf.nbytes
+                context = max(seq.cache.num_computed + 1 for seq in dseqs)
+                groups = self._shared_step(dseqs)
+                if groups:
+                    extras, logits = self._decode_shared(drows, extras_for(dseqs, bs), groups, context)
+                else:
+                    g = self.decode_graph(bs, context)
+                    buf, layout = b.pack(drows, pad_rows=bs, table_width=self.max_blocks_per_seq, extras=extras_for(dseqs, bs))
+                    assert layout["size"] == g.layout["size"]
+                    b.to_device(buf, g.layout, into=g.buffer)
+                    g.graph.replay()
+                    self.h2d_bytes += buf.nbytes
+                    extras, logits = g.ctx.extras, g.logits
+                    if use_graph:
+                        self.num_graph_steps += 1
+                lp = self._choose_under_rules(dseqs, logits, extras, 0, turn, self._pinned_tokens)
                 sources.append((self._pinned_tokens[turn], len(dseqs)))
+                logprob_sources.append((lp, len(dseqs)))
                 for k, seq in enumerate(dseqs):
                     seq.pending_index = k
-                if use_graph:
-                    self.num_graph_steps += 1
             if use_graph:
                 pass
             elif portion_graph:                                # ---- the one prompt portion, from a graph of its padded length
@@ -441,27 +655,35 @@ class LLMEngine:
                     b.to_device(buf, pg.layout, into=pg.buffer)
                     pg.graph.replay()
                     self.num_portion_graph_steps += 1
+                    ctx, logits = pg.ctx, pg.logits
                 else:                                          # the first time a shape occurs: launched kernel by kernel
                     buf, layout = b.pack([row], extras=extras)
                     ctx = b.to_device(buf, layout)
                     ctx.token_feedback = self._sampled
-                    self._forward_and_sample(ctx, tokens, host_out=self._pinned_portion)
+                    logits = self._forward_and_sample(ctx, tokens, host_out=self._pinned_portion)
                 self.h2d_bytes += buf.nbytes
                 if pseqs:
+                    lp = self._choose_under_rules(pseqs, logits, ctx.extras, self._portion_slot, turn, self._pinned_portion)
                     sources.append((self._pinned_portion[turn], 1))
+                    logprob_sources.append((lp, 1))
                     pseq.pending_index = self._portion_slot
             else:                                              # ---- any other mix: one batch, launched kernel by kernel
                 k = len(sample_seqs)
                 extras = extras_for(sample_seqs, 0)
-                buf, layout = b.pack(rows, extras=extras)
+                groups = self._shared_step([seq for seq, _ in batch]) if not others else None
+                buf, layout = b.pack(rows, extras=extras, shared=groups)
                 ctx = b.to_device(buf, layout)
                 ctx.token_feedback = self._sampled
                 self.h2d_bytes += buf.nbytes
                 logits = self.model.step(ctx)
-                if sample_seqs and not self.sampler.sample_step(logits, ctx.extras, self._sampled[:k], row_seeds, seeds,
-                                                                host_out=self._pinned_tokens):
+                lp = None
+                if any(s.params.has_rules for s in sample_seqs):
+                    lp = self._choose_under_rules(sample_seqs, logits, ctx.extras, 0, turn, self._pinned_tokens)
+                elif sample_seqs and not self.sampler.sample_step(logits, ctx.extras, self._sampled[:k], row_seeds, seeds,
+                                                                  host_out=self._pinned_tokens):
                     self._pinned_tokens[turn, :k].copy_(self._sampled[:k], non_blocking=True)   # this rare way copies
                 sources.append((self._pinned_tokens[turn], k))
+                logprob_sources.append((lp, k))
                 for k2, seq in enumerate(sample_seqs):
                     seq.pending_index = k2
             self._turn = turn
@@ -481,23 +703,26 @@ class LLMEngine:
             total = len(seq.token_ids)
             if total - seq.prompt_len >= seq.params.max_tokens or total >= max_len:
                 self.scheduler.finish(seq)                 # its pages may go to the next step: that one runs after this one
+                self._ended(seq)
                 ending.append(seq)
-        return _InFlight(sample_seqs, [s.num_tokens - 1 for s in sample_seqs], ending, sources, done_event)
+        return _InFlight(sample_seqs, [s.num_tokens - 1 for s in sample_seqs], ending, sources, logprob_sources, done_event)
 
     def _complete(self, fl) -> list:
         with _nvtx_range("sample"):
             fl.event.synchronize()
-            new_tokens = fl.tokens()
+            new_tokens, new_logprobs = fl.tokens(), fl.logprobs()
         ops.check_range_errors()           # an integer out of range that a kernel refused to follow
         ops.check_tc_errors()
         gemm_tc.check_error()              # a bounded wait that ran out in a tensor-core product is an error, not a result
         now = time.perf_counter()
         finished = []
-        for seq, place, tok in zip(fl.seqs, fl.places, new_tokens):
+        for seq, place, tok, lp in zip(fl.seqs, fl.places, new_tokens, new_logprobs):
             if seq.ended_by_eos:
                 del seq.token_ids[place:]                  # it ended by EOS a step ago: this token is one too many
                 continue
             seq.token_ids[place] = tok
+            if seq.params.logprobs:
+                seq.logprobs.append(lp)
             if seq.first_token_time is None:
                 seq.first_token_time = now
             if seq in fl.ending:
@@ -508,16 +733,38 @@ class LLMEngine:
                 seq.ended_by_eos = True
                 seq.finish_time = now
                 self.scheduler.finish(seq)
+                self._ended(seq)
                 finished.append(seq)
         return finished
 
     # ------------------------------------------------------------------ offline API
-    def generate(self, prompts, params=None, decode_text: bool = True) -> list:
+    def generate(self, prompts, params=None, decode_text: bool = True, n: int = 1) -> list:
+        """``n`` answers to every prompt, one behind another in the result; with more than one, the answers to a prompt share its pages where the
+        model allows it (``add_prefix``)."""
         if not isinstance(params, list):
             params = [params or SamplingParams()] * len(prompts)
         if len(params) != len(prompts):
             raise ValueError("one SamplingParams per prompt")
-        seqs = [self.add_request(p, sp) for p, sp in zip(prompts, params)]
+        if n < 1:
+            raise ValueError(f"n must be at least 1, got {n}")
+        seqs, prefixes = [], []
+        try:
+            for p, sp in zip(prompts, params):
+                prefix = None
+                if n > 1 and self.can_share:
+                    ids = self._prompt_ids(p)
+                    whole = (len(ids) - 1) // self.cfg.block_size * self.cfg.block_size
+                    if whole:
+                        try:
+                            prefix = self.add_prefix(ids[:whole])
+                        except ValueError:                     # no room to hold it beside the requests: every answer computes its own
+                            prefix = None
+                        else:
+                            prefixes.append(prefix)
+                seqs += [self.add_request(p, sp, prefix=prefix) for _ in range(n)]
+        finally:
+            for prefix in prefixes:                            # (held by the requests that begin with it)
+                self.release_prefix(prefix)
         while self.has_work():
             self.step()
         outs = []
@@ -525,6 +772,7 @@ class LLMEngine:
             text = None
             if decode_text and self.tokenizer is not None:
                 text = self.tokenizer.decode(s.output_ids, skip_special_tokens=True)
-            outs.append(RequestOutput(s.seq_id, s.prompt_len, s.output_ids, text,
-                                      s.first_token_time - s.arrival_time, s.finish_time - s.arrival_time))
+            first = None if s.first_token_time is None else s.first_token_time - s.arrival_time      # (a grammar may allow no token at all)
+            outs.append(RequestOutput(s.seq_id, s.prompt_len, s.output_ids, text, first, s.finish_time - s.arrival_time,
+                                      s.logprobs if s.params.logprobs else None))
         return outs

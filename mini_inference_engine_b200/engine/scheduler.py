@@ -67,9 +67,12 @@ class Scheduler:
         self.watermark = max(1, min(p.num_pages for p in cache.pools) // 100)
 
     # ------------------------------------------------------------------ the queue
-    def can_ever_fit(self, num_positions: int) -> bool:
+    def can_ever_fit(self, num_positions: int, shared: int = 0, pinned: int = 0) -> bool:
+        """Whether a request of that many positions, the first ``shared`` pages of them a prefix's, fits the pages that prefixes leave
+        (``pinned``: pages that one more prefix would hold)."""
         need = self.cache.max_pages_for(num_positions)
-        return all(n + self.watermark <= pool.num_usable for n, pool in zip(need, self.cache.pools))
+        return all(n - shared + self.watermark <= pool.num_usable - held - pinned
+                   for n, pool, held in zip(need, self.cache.pools, self.cache.pinned))
 
     def add(self, seq: Sequence) -> None:
         self.waiting.append(seq)
@@ -132,6 +135,8 @@ class Scheduler:
     def _admit(self, draft: _Draft, whole_prompts_only: bool) -> None:
         while self.waiting and draft.budget > 0 and len(self.running) < self.cfg.max_num_seqs:
             seq = self.waiting[0]
+            if seq.prefix is not None and not seq.cache.shared:
+                self.cache.adopt(seq.cache, seq.prefix.cache, seq.prefix_pages)
             n = min(seq.num_new_tokens, draft.budget)
             if whole_prompts_only and n < seq.num_new_tokens:
                 return

@@ -38,6 +38,11 @@ class Sequence:
         self.finish_time: float | None = None
         self.pending_index = 0           # where the step in flight will leave this request's next token
         self.ended_by_eos = False        # ended by EOS while a further step was already in flight
+        self.prefix = None               # the Prefix whose first ``prefix_pages`` pages this request begins with
+        self.prefix_pages = 0
+        self.mask = None                 # what the request's grammar allows next (words of bits; None: everything), and for how many tokens ...
+        self.mask_at = -1                # ... it was asked
+        self.logprobs: list = []         # log-probabilities of the answer's tokens (``SamplingParams.logprobs``)
 
     @property
     def num_computed(self) -> int:

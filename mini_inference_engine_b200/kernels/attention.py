@@ -57,7 +57,19 @@ def rotates_in_decode(dtype, head_dim: int, ctx) -> bool:
     """Whether ``attention(..., rope=...)`` can rotate q and the new key itself and write the cache: a step of
     decoding rows only, on the tensor-core decode kernel, with a head size it rotates."""
     return (_backend == "auto" and dtype == torch.bfloat16 and head_dim <= 128 and head_dim % 32 == 0
-            and decode_only(ctx))
+            and decode_only(ctx) and ctx.prefix is None)
+
+
+# Shared prefixes against ordinary decode attention, which reads a prefix once a row, by the bytes of keys and values that sharing saves a layer (SHARE_MIN_BYTES).
+# Us, ordinary : shared -- 32 heads of 64 on 4, 2 rows behind 208 keys 4.2 : 11.9, 8 behind 2,048 (15 MB) 10.0 : 15.8; 32 of 128 on 8, 64 behind 8,000 (2.1 GB) 376 : 62, 256 behind
+# 16,384 1,983 : 143; 32 of 128 on 32, 33 rows in five groups (0.9 GB) 159 : 76.
+SHARE_MIN_BYTES = 48 << 20
+
+
+def sharing_pays(groups, bytes_per_key: int) -> bool:
+    """Whether a step of single tokens whose rows share prefixes -- ``groups`` as (rows, ..., positions) -- is attended over with them shared; ``bytes_per_key``
+    of keys and values in a layer."""
+    return sum((g[0] - 1) * g[-1] for g in groups) * bytes_per_key >= SHARE_MIN_BYTES
 
 
 # float32: tiles of (token, head) pairs (csrc/attention_f32.cu) against a warp a pair.  A tile takes as long with one pair as with 64, a walk of keys shared out over up to eight
@@ -125,7 +137,10 @@ def attention(qkv, ctx, cache, out, num_heads, num_kv_heads, head_dim, scale, wi
     keys of the query's own block of -w positions.  ``keep``: beside a window or block, the first ``keep`` keys of the
     sequence stay in sight.  ``q_stride``: elements between the token rows of ``qkv`` (by
     default rows of a fused q|k|v projection).  ``mods`` (``ops.ScoreMods``): a cap on the scores, a bias or a slope by distance, a sink in
-    the softmax; every kernel applies them (the tcgen05 kernel for portions in an instance of its own)."""
+    the softmax; every kernel applies them (the tcgen05 kernel for portions in an instance of its own).
+
+    A step whose rows share prefixes (``ctx.prefix``) reads those once for all rows where the layer is plain bfloat16 attention over all keys; other
+    layers read them row by row through the rows' own block tables."""
     if q_stride is None:
         q_stride = (num_heads + 2 * num_kv_heads) * head_dim
     args = (qkv, q_stride, cache.k, cache.v, ctx.block_tables[cache.group], ctx.row_q_start, ctx.row_q_len,
@@ -143,6 +158,9 @@ def attention(qkv, ctx, cache, out, num_heads, num_kv_heads, head_dim, scale, wi
                              "in steps of 32 up to 128)")
         return ops.decode_attention(*args, out, num_heads, num_kv_heads, head_dim, cache.page_size, scale, window,
                                     max_ctx=ctx.max_ctx_len, rope=rope)
+    if ctx.prefix is not None and fast and window == 0 and mods is None and decode_only(ctx):
+        return ops.shared_prefix_attention(*args, ctx.prefix.start, ctx.prefix.length, out, num_heads, num_kv_heads, head_dim, cache.page_size, scale,
+                                           max_prefix=ctx.prefix.max_prefix, max_own=ctx.prefix.max_own)
     if not fast and _backend == "auto" and ops.attention_f32_takes(qkv, cache.k, cache.v, out, head_dim):
         return _attention_f32(args, ctx, out, num_heads, num_kv_heads, head_dim, cache.page_size, scale, window, mods, keep)
     if not fast:

@@ -124,6 +124,17 @@ class StepContext:
     host: dict = field(default_factory=dict)
     extras: dict = field(default_factory=dict)   # small per-step device arrays that rode along (sampling inputs)
     token_feedback: torch.Tensor | None = None   # int32: tokens the previous step sampled; a token id -(k+1) means entry k
+    prefix: object = None                        # PrefixGroups, where the step's rows are to be attended over with shared prefixes
+
+
+@dataclass
+class PrefixGroups:
+    """Rows of a step of single tokens that share their first keys (kernels.ops.shared_prefix_attention): ``start`` int32 [groups + 1], ``length``
+    int32 [groups], and bounds for planning on the longest prefix and on a row's keys behind it."""
+    start: torch.Tensor
+    length: torch.Tensor
+    max_prefix: int
+    max_own: int
 
 
 @dataclass

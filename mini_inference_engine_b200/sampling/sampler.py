@@ -55,6 +55,24 @@ class Sampler:
                         extras["out_position"][i:i + 1], out=out[i:i + 1], seed=sd)
         return False
 
+    def sample_ruled(self, logits: torch.Tensor, extras: dict, out: torch.Tensor, requests, book, host_out: torch.Tensor | None = None,
+                     logprob: torch.Tensor | None = None) -> bool:
+        """As ``sample_step`` for rows of which some have rules (``book`` holds their texts): one row of ``logits`` a request.  ``logprob``
+        (float32, an entry a row) receives every token's log-probability."""
+        seeds, noisy = self.seeds_of(requests)
+        names = ("temperature", "request", "out_position")
+        if len(noisy) <= 1:
+            rows = len(requests)
+            rules = book.step_rules(requests)
+            ops.sample(logits, *(extras[n][:rows] for n in names), next(iter(noisy)) if noisy else self.seed, out, host_out, extras["host_turn"],
+                       rules=rules, logprob=logprob, append=rules.history is not None)
+            return True
+        for i, (seed, request) in enumerate(zip(seeds, requests)):
+            rules = book.step_rules([request])
+            ops.sample(logits[i:i + 1], *(extras[n][i:i + 1] for n in names), seed, out[i:i + 1], rules=rules,
+                       logprob=None if logprob is None else logprob[i:i + 1], append=rules.history is not None)
+        return False
+
     def sample(self, logits: torch.Tensor, temperature: torch.Tensor, request: torch.Tensor,
                position: torch.Tensor, out: torch.Tensor | None = None, seed: int | None = None,
                host_out: torch.Tensor | None = None, host_turn: torch.Tensor | None = None) -> torch.Tensor:
