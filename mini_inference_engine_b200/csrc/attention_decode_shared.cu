@@ -1,21 +1,17 @@
-// The second half of attention over shared prefixes: every row's own keys (those behind its group's prefix), by the kernel of attention_decode.cu, whose
-// merge takes in what attention_prefix.cu left for the prefix.  A row of no group, or of one without a prefix, is ordinary decode attention.
+// The second half of attention over shared prefixes where the first is attention_prefix.cu's kernel for any head size: every row's own keys (those behind its
+// group's prefix), by the kernel of attention_decode.cu, whose merge takes in what was left for the prefix.  A row of no group, or of one without a prefix, is
+// ordinary decode attention.
 #include "attention_decode.cuh"
+#include "prefix_args.cuh"
 
-// Parameters as mie_decode_attention (attention_decode.cu), without a window, modifiers and the rotation inside the kernel; the splits merge through scratch
-// memory.  The groups, the layout, the partial results and `pre_chunk` are those of mie_prefix_attention (attention_prefix.cu) on the same stream before.
-extern "C" int mie_decode_attention_shared(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const int* block_tables,
-                                           int table_stride, const int* row_q_start, const int* row_q_len, const int* row_ctx_len, int num_rows,
-                                           const int* group_start, const int* group_prefix, int groups, const int* layout, const float* pre_o,
-                                           const float* pre_lse, const int* pre_chunk, long long most_slots, void* out, int num_heads, int num_kv_heads, int head_dim,
-                                           int page_size, float scale, int splits, float* part_o, float* part_lse, int* counters, int stages,
-                                           int64_t num_pages, int64_t check_pages, int min_part_tiles, int out_f32, cudaStream_t stream) {
-    const int64_t covered = (int64_t)table_stride * page_size;
-    const PrefixGroups g{group_start, group_prefix, groups, num_rows, (int)(covered < 0x7fffff00ll ? covered : 0x7fffff00ll), num_kv_heads * layout[1], layout[2], layout[3]};
-    return decode_attention_launch<false, true>(q, q_stride, k_cache, v_cache, block_tables, table_stride, row_q_start, row_q_len, row_ctx_len, num_rows, out,
-                                                num_heads, num_kv_heads, head_dim, page_size, scale, 0, splits, part_o, part_lse, counters, stream, stages,
-                                                num_pages, check_pages, g_range_report, min_part_tiles, nullptr, nullptr, 0, out_f32 != 0, nullptr, 0, &g,
-                                                pre_o, pre_lse, pre_chunk, most_slots);
+// `a`: as for mie_prefix_attention (attention_prefix.cu) before, on the same stream; groups 0: nothing came before.  The splits merge through scratch memory.
+extern "C" int mie_decode_attention_shared(const SharedArgs* a, cudaStream_t stream) {
+    const PrefixGroups g = shared_groups_of(*a);
+    return decode_attention_launch<false, true>(a->q, a->q_stride, a->k_cache, a->v_cache, a->block_tables, a->table_stride, a->row_q_start, a->row_q_len,
+                                                a->row_ctx_len, a->num_rows, a->out, a->num_heads, a->num_kv_heads, a->head_dim, a->page_size, a->scale, 0,
+                                                a->splits, a->part_o, a->part_lse, a->counters, stream, a->stages, a->tma ? a->num_pages : 0, a->num_pages,
+                                                g_range_report, a->min_part_tiles, nullptr, nullptr, 0, a->out_f32 != 0, nullptr, 0, &g, a->pre_o, a->pre_lse,
+                                                a->pre_chunk, a->most_slots);
 }
 
 // Non-zero when a block of any launch so far gave up a bounded wait (TMA copies that did not arrive).

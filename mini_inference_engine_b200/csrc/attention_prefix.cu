@@ -1,10 +1,11 @@
 // Attention of decoding rows over keys that they share: every (row, query head) pair of a group against the group's prefix, computed once for
-// all rows, in bfloat16 with float32 scores, softmax statistics and sums.  Leaves, for a pair and a range of the prefix,
+// all rows, in bfloat16 with float32 scores, softmax statistics and sums.  Leaves, for a pair and a range of keys,
 //     o = sum_j 2^(s_j - m) v_j / l   and   m + log2 l,     l = sum_j 2^(s_j - m),  s_j = scale log2(e) q . k_j
-// which the kernel for the rows' own keys (attention_decode_shared.cu) joins with its own.  prefix_plan.cuh says how the work is cut.
+// which a kernel behind joins with the pair's other ranges.  prefix_plan.cuh says how the work is cut.
 //
-// Two kernels.  Heads of 64 and 128 on pages of 8 positions or more: tcgen05, below.  Any head size in steps of 16: a block takes 64 pairs, 16 a warp
-// (mma.sync m16n8k16), and walks its range of keys in tiles of 64 that arrive by cp.async, two in flight; a tile serves all 64 pairs.
+// Two ways.  Heads of 64 and 128 on pages of 8 positions or more: tcgen05, prefix and own keys in one walk, below.  Any head size in steps of 16: a
+// block takes 64 pairs, 16 a warp (mma.sync m16n8k16), and walks its range of the prefix in tiles of 64 keys that arrive by cp.async, two in flight; a tile
+// serves all 64 pairs, and the kernel for the rows' own keys (attention_decode_shared.cu) joins its results with its own.
 #include "mma_common.cuh"
 #include "tcgen05_common.cuh"
 #include "prefix_plan.cuh"
@@ -205,38 +206,162 @@ static int launch_prefix(const PrefixParams& p, long long items, cudaStream_t st
     return launch_kernel(prefix_attention_kernel<D>, dim3((unsigned)items), dim3(PFX_WARPS * 32), smem, stream, p);
 }
 
-// --------------------------------------------------------------------------- heads of 64 and 128: tcgen05
+// --------------------------------------------------------------------------- heads of 64 and 128: tcgen05, one walk
 //
-// A block holds up to 256 pairs as two tiles of 128 (one pair a tensor-memory lane) and walks its keys in tiles of 128 that TMA brings a page a copy; a
-// tile of keys and values serves both tiles of pairs.  Two groups of four softmax warps, one a tile of pairs, and a thread that issues for each: while a
-// group takes its scores through the softmax the tensor pipe works on the other's products.
-//   S_u = Q_u K^T into tensor memory; the group's threads move their rows of S into registers, write P = 2^(s - m), rounded to bfloat16, back, and
-//   O_u += P_u V with P as the left operand out of tensor memory and V as it lies.
-// Tensor memory: heads of 64 S 2 x 128 columns, P 2 x 64, O 2 x 64; S of the next tile is issued as soon as the rows are in registers.  Heads of 128: O takes
-// 2 x 128, and P lies over the S that it came from, so that S of the next tile is issued behind this tile's product with the values.
-// Queries are fetched by the threads whose rows they are (any rows, any stride) and written to shared memory as the products want them; the first keys are on
-// their way before the wait for the kernel in front (the prefix is older than the step).
-#define PT_THREADS 352
+// Rows of a group (or rows that belong to none) are taken `tile_rows` at a time: up to 256 (row, head) pairs of a unit, two tiles of 128, one pair a
+// tensor-memory lane.  Their walk goes in steps of 128 keys: first the group's prefix, which all pairs see, then the rows' own keys, laid end to end a page (or
+// 128 keys of one) a slot, where a pair sees its own row's keys only; a step holds own keys of one tile, and the tiles take turns.  An item is a range of steps
+// of such a walk; it leaves o and m + log2 l of its keys for every pair (-inf where a pair saw none), and a second kernel joins the ranges of a row.  Own keys
+// that way cost their bytes and little else: attended over by the decode kernel behind a kernel for the prefixes, 64 rows of up to 512 own keys behind 8,000
+// took 62 us, 256 rows of up to 96 behind 16,384 143 us, of which 40 and 54 were the decode kernel's.
+//
+// Two chains of work run side by side, each with four softmax warps, a thread that issues its products, and its own S, P and O in tensor memory:
+//   S = Q K^T; the chain's threads move their rows of S into registers, write P = 2^(s - m), rounded to bfloat16, back, and
+//   O += P V with P as the left operand out of tensor memory and V as it lies.
+// Such a chain takes 4,400 cycles a step, four times what its products take; two fill one another's gaps.  With two tiles of pairs a chain owns a tile, and a
+// step of the prefix serves both; with one the chains take the steps in turns over the same queries and leave a result each.
+// Keys and values come by TMA, a slot a copy, keys and values each with barriers of their own: keys of a later step arrive as soon as S is formed.
+// Tensor memory: heads of 64 S 2 x 128 columns, P 2 x 64, O 2 x 64; S of the next step is issued as soon as the rows are in registers.  Heads of 128: O takes
+// 2 x 128, and P lies over the S that it came from, so that S of the next step is issued behind this step's product with the values.
+//
+// Values of one row must not reach another's output: slots' keys that are nobody's (in front of a row's own keys, behind its context) are made zero in
+// shared memory, and so are own values that are not finite, since 0 times those is not 0; the row is marked, and the joining kernel adds them to its output.
+#define PT_THREADS 384
 #define PT_ROWS 128
 #define PT_KEYS 128
+#define PT_MOST_TILES 512          // tiles of rows that a launch can plan for ...
+#define PT_MOST_SEGMENTS 63        // ... and groups with the rows between them
+
+struct WalkParams {
+    PrefixParams b;
+    const int* row_ctx_len; int2* row_info; int* marks;    // row_info: a row's first slot and its ranges; marks: 0, or the query heads of a (row, key head) with values that are not finite
+};
 
 template <int D> constexpr int PT_STAGES = D == 64 ? 4 : 2;
 template <int D> constexpr size_t PT_SMEM = (size_t)PT_ROWS * D * 2 * 2 + (size_t)PT_STAGES<D> * 2 * PT_KEYS * D * 2 + 1024;
 
+// What a block needs to know of the step's plan, and the scratch it is worked out in.
+struct WalkPlan {
+    int first[PT_MOST_SEGMENTS], rows[PT_MOST_SEGMENTS], keys[PT_MOST_SEGMENTS], tile0[PT_MOST_SEGMENTS];      // segments: rows, shared keys, first tile of rows
+    int segments, tiles;
+    int slots[2 * PT_MOST_TILES];                          // own slots of a tile of pairs
+    int steps[PT_MOST_TILES], seg[PT_MOST_TILES];          // steps of a tile of rows' walk; its segment
+    unsigned long long best;
+    int found, splits, item0, slot0;                       // the item's tile of rows (-1: none), its ranges, first item and slot
+    int own_first[2 * PT_ROWS + 1], ctx[2 * PT_ROWS];      // of the tile's rows: first own slot; context (0: not a row of one new token)
+};
+
+// Keys of an own slot as a shift, and a row's own slots: slots are whole pages, or 128 keys of a longer page.
+#define PT_KEYS_SHIFT 7
+__device__ __forceinline__ int slot_shift(int page_shift) { return min(page_shift, PT_KEYS_SHIFT); }
+__device__ __forceinline__ int own_slots(int ctx, int prefix, int ss) { return ctx > prefix ? ((ctx + (1 << ss) - 1) >> ss) - (prefix >> ss) : 0; }
+
+// By the whole block.  Afterwards w.found is the item's tile of rows.
+template <int T>
+__device__ __forceinline__ void walk_plan(WalkPlan& w, const WalkParams& q, int item) {
+    const PrefixGroups& p = q.b.groups;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ss = slot_shift(q.b.page_shift), half = p.tile_rows / 2;
+    // segments: the rows in front of the first group, the groups, the rows behind the last
+    if (tid < p.groups + 2) {
+        auto at = [&](int k) { return max(0, min(p.start[k], p.num_rows)); };
+        const int a = tid == 0 ? 0 : at(tid - 1), b = tid == p.groups + 1 ? p.num_rows : at(tid);
+        w.first[tid] = a;
+        w.rows[tid] = max(0, b - a);
+        w.keys[tid] = tid >= 1 && tid <= p.groups ? max(0, min(p.prefix[tid - 1], p.most_keys)) : 0;
+    }
+    if (tid == 0) { w.segments = p.groups + 2; w.best = ~0ull; w.found = -1; }
+    // this thread's first row (the others are asked for where there are more rows than threads)
+    const int r_len = tid < p.num_rows ? q.b.row_q_len[tid] : 0, r_ctx = tid < p.num_rows ? q.row_ctx_len[tid] : 0;
+    __syncthreads();
+    if (warp == 0) {                                       // first tiles of the segments
+        int at = 0;
+        for (int g0 = 0; g0 < w.segments; g0 += 32) {
+            const int g = g0 + lane, n = g < w.segments ? (w.rows[g] + p.tile_rows - 1) / p.tile_rows : 0;
+            int sum = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += up; }
+            if (g < w.segments) {
+                w.tile0[g] = at + sum - n;
+                for (int i = 0; i < n && at + sum - n + i < PT_MOST_TILES; ++i) w.seg[at + sum - n + i] = g;
+            }
+            at += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) w.tiles = min(at, PT_MOST_TILES);
+        const int tiles = min(at, PT_MOST_TILES);
+        for (int t = lane; t < 2 * tiles; t += 32) w.slots[t] = 0;
+    }
+    __syncthreads();
+    const int tiles = w.tiles;
+    for (int r = tid; r < p.num_rows; r += T) {            // own slots of the tiles of pairs
+        int g = 0;
+        while (g + 1 < w.segments && !(r >= w.first[g] && r < w.first[g] + w.rows[g])) ++g;
+        const int in_seg = r - w.first[g], t = w.tile0[g] + in_seg / p.tile_rows;
+        const int len = r == tid ? r_len : q.b.row_q_len[r], ctx = r == tid ? r_ctx : q.row_ctx_len[r];
+        if (in_seg >= 0 && t < tiles && len == 1) atomicAdd(&w.slots[2 * t + (in_seg % p.tile_rows) / half], own_slots(min(ctx, p.most_keys), w.keys[g], ss));
+    }
+    __syncthreads();
+    const int ws = PT_KEYS_SHIFT - ss, W = 1 << ws;        // own slots a step
+    for (int t = tid; t < tiles; t += T)
+        w.steps[t] = (w.keys[w.seg[t]] + PREFIX_STEP - 1) / PREFIX_STEP + ((w.slots[2 * t] + W - 1) >> ws) + ((w.slots[2 * t + 1] + W - 1) >> ws);
+    __syncthreads();
+    // How many ranges the longest walk is cut into: a candidate a lane (prefix_plan.cuh says what is weighed).
+    if (warp < PREFIX_MAX_SPLITS / 32) {
+        int most = 1;
+        for (int t = lane; t < tiles; t += 32) most = max(most, w.steps[t]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const int s = warp * 32 + lane + 1;
+        if (s <= most) {
+            const int c = (most + s - 1) / s;
+            unsigned items = 0;
+            for (int t = 0; t < tiles; ++t) items += p.units * prefix_splits(w.steps[t], c);
+            if (s == 1 || items <= 2u * p.places) {
+                const unsigned long long cost = (unsigned long long)((items + p.places - 1) / p.places) * (c + PREFIX_COST_START);
+                atomicMin(&w.best, cost << 32 | (0xffffffffu - (unsigned)c));
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const int c = max(1, (int)(0xffffffffu - (unsigned)w.best));
+        int items = 0, slots = 0;
+        for (int t0 = 0; t0 < tiles; t0 += 32) {
+            const int t = t0 + lane, splits = t < tiles ? prefix_splits(w.steps[t], c) : 0;
+            int rows = 0;
+            if (t < tiles) rows = min(p.tile_rows, w.rows[w.seg[t]] - (t - w.tile0[w.seg[t]]) * p.tile_rows);
+            const int n = p.units * splits, k = rows * splits * (rows > half ? 1 : 2);      // (a tile of pairs alone: a result a chain)
+            int ni = n, ki = k;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int a = __shfl_up_sync(0xffffffffu, ni, o), b = __shfl_up_sync(0xffffffffu, ki, o);
+                if (lane >= o) { ni += a; ki += b; }
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, item >= items + ni - n && item < items + ni);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) { w.found = t; w.splits = splits; w.item0 = items + ni - n; w.slot0 = slots + ki - k; }
+                break;
+            }
+            items += __shfl_sync(0xffffffffu, ni, 31);
+            slots += __shfl_sync(0xffffffffu, ki, 31);
+        }
+    }
+    __syncthreads();
+}
+
 template <int D>
 __global__ void __launch_bounds__(PT_THREADS, 1)
-prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixParams p) {
+prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const WalkParams wp) {
     constexpr int PARTS = D / 64, STAGES = PT_STAGES<D>;
     constexpr uint32_t SUB = 128 * 64 * 2;                 // one [128 x 64] part of a tile
     constexpr uint32_t TILE = PARTS * SUB;
     constexpr bool OVER = D == 128;                        // P lies over S
     constexpr uint32_t TMEM_S = 0, TMEM_P = OVER ? 0 : 256, TMEM_O = OVER ? 256 : 384, S_STEP = 128, P_STEP = OVER ? 128 : 64, O_STEP = D;
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(8) uint64_t q_full[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], s_free[2], p_full[2], pv_done[2], o_full[2], exp_done[2];
+    __shared__ __align__(8) uint64_t q_full[2], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], s_free[2], p_full[2], pv_done[2], o_full[2], exp_done[2];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
-    __shared__ PrefixPart s_part;
-    __shared__ int s_chunk;
+    __shared__ WalkPlan plan;
+    const PrefixParams& p = wp.b;
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char* tiles = smem_dyn + (base - smem_u32(smem_dyn));
     auto q_off = [&](int u) { return (uint32_t)u * TILE; };
@@ -244,201 +369,339 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     auto v_off = [&](int st) { return 2 * TILE + (uint32_t)st * 2 * TILE + TILE; };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) {
-        const int chunk = prefix_chunk(p.groups);
-        const PrefixPart t = prefix_find(p.groups, chunk, (int)blockIdx.x, false);
-        if (lane == 0) { s_part = t; s_chunk = chunk; }
-    }
-    __syncthreads();
-    const PrefixPart t = s_part;
-    if (t.rows == 0 || t.splits == 0) {
+    walk_plan<PT_THREADS>(plan, wp, (int)blockIdx.x);
+    if (plan.found < 0) {
         pdl_wait();                                        // a block without work waits too: see common.cuh
-        if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = s_chunk;
         return;
     }
-    int index = (int)blockIdx.x - t.item0;
-    const int split = index % t.splits;
-    index /= t.splits;
-    const int tile = index % t.tiles, unit = index / t.tiles;
+    const int t = plan.found, splits = plan.splits, seg = plan.seg[t], in_seg = t - plan.tile0[seg];
+    const int index = (int)blockIdx.x - plan.item0, split = index % splits, unit = index / splits;
     const int G = p.num_heads / p.num_kv_heads, kvh = unit / p.chunks, h0 = (unit - kvh * p.chunks) * p.chunk_heads;
     const int heads = min(p.chunk_heads, G - h0);          // of this unit
     const int half = p.groups.tile_rows / 2;               // rows of a tile of pairs
-    const int row0 = t.first_row + tile * p.groups.tile_rows, rows = min(p.groups.tile_rows, t.first_row + t.rows - row0);
-    const int nsub = rows > half ? 2 : 1;
-    int step0, steps;
-    prefix_range(t.steps, t.splits, split, step0, steps);
-    const int key_lo = step0 * PREFIX_STEP, key_hi = min(t.keys, (step0 + steps) * PREFIX_STEP);
-    const int J = (key_hi - key_lo + PT_KEYS - 1) / PT_KEYS;
-
-    if (threadIdx.x == 0) {
+    const int leader = plan.first[seg], row0 = leader + in_seg * p.groups.tile_rows, rows = min(p.groups.tile_rows, leader + plan.rows[seg] - row0);
+    const bool both = rows > half;                         // two tiles of pairs, a chain each; else one, both chains over it
+    const int prefix = plan.keys[seg], ss = slot_shift(p.page_shift), sk = 1 << ss, ws = PT_KEYS_SHIFT - ss, W = 1 << ws;
+    const int pre_steps = (prefix + PREFIX_STEP - 1) / PREFIX_STEP;
+    int x0, J;                                             // this item's steps: x0 .. x0 + J - 1 of the walk
+    prefix_range(plan.steps[t], splits, split, x0, J);
+    // the rows' own slots, one behind another
+    if (warp == 0) {
+        int at = 0;
+        for (int i0 = 0; i0 < rows; i0 += 32) {
+            const int i = i0 + lane, r = row0 + i;
+            const bool on = i < rows && p.row_q_len[r] == 1;
+            const int all = on ? wp.row_ctx_len[r] : 0, ctx = min(all, p.groups.most_keys);
+            if (on && unit == 0 && split == 0 && (all < prefix || all > p.groups.most_keys))         // a context that ends inside its prefix, or beyond its block table
+                range_report(p.report, MIE_RANGE_POSITION, MIE_K_ATTENTION_PREFIX, r, all);
+            const int n = own_slots(ctx, prefix, ss);
+            int sum = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += up; }
+            if (i < rows) { plan.own_first[i] = at + sum - n; plan.ctx[i] = on ? max(1, ctx) : 0; }
+            at += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) plan.own_first[rows] = at;
+    }
+    if (threadIdx.x == 32) {
         abort_flag = 0;
         for (int u = 0; u < 2; ++u) {
             mbar_init(&q_full[u], 4); mbar_init(&s_full[u], 1); mbar_init(&s_free[u], 4); mbar_init(&p_full[u], 4);
             mbar_init(&pv_done[u], 1); mbar_init(&o_full[u], 1); mbar_init(&exp_done[u], 4);
         }
-        for (int st = 0; st < STAGES; ++st) { mbar_init(&kv_full[st], 1); mbar_init(&kv_empty[st], nsub); }      // every issuing thread gives a stage back
+        for (int st = 0; st < STAGES; ++st) {              // (both issuing threads give a stage back, whether or not their chain used it)
+            mbar_init(&k_full[st], 1); mbar_init(&v_full[st], 1); mbar_init(&k_empty[st], 2); mbar_init(&v_empty[st], 2);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
     volatile int* abort_p = &abort_flag;
-    // ---- the keys and values (warp 0): lane c copies page c of a tile
-    const int* table = p.block_tables + (int64_t)t.first_row * p.table_stride;           // the prefix lies where the group's first row says
-    const int rows_per_copy = min(p.page_size, PT_KEYS);
-    auto copies_of = [&](int j) { return (min(key_lo + (j + 1) * PT_KEYS, key_hi) - (key_lo + j * PT_KEYS) + rows_per_copy - 1) / rows_per_copy; };
-    auto page_of = [&](int j) {
-        if (j >= J || lane >= copies_of(j)) return 0;
-        const int entry = (key_lo + j * PT_KEYS + lane * rows_per_copy) >> p.page_shift;
-        return checked_page(table[entry], p.num_pages, p.report, MIE_K_ATTENTION_PREFIX, entry);
+    const int npre = max(0, min(J, pre_steps - x0));       // the first npre of this item's steps are the prefix's
+    // own slots go by lists, one a tile of pairs: list l's begin at list0[l], and take list_steps[l] steps, turn by turn while both have some
+    const int list0[2] = {0, both ? plan.own_first[half] : 0}, list_end[2] = {both ? plan.own_first[half] : plan.own_first[rows], plan.own_first[rows]};
+    const int steps0 = (list_end[0] + W - 1) >> ws, steps1 = both ? (list_end[1] - list0[1] + W - 1) >> ws : 0, turns = min(steps0, steps1);
+    struct OwnStep { int list, k; };                       // the k-th step of a list
+    auto own_step = [&](int j) {
+        const int x = x0 + j - pre_steps;
+        if (x < 2 * turns) return OwnStep{x & 1, x >> 1};
+        return OwnStep{steps1 > steps0 ? 1 : 0, x - turns};
     };
-    auto load_tile = [&](int j, int st, int page) {
+    // does chain c take part in step j?
+    auto active = [&](int c, int j) {
+        if (!both) return (j & 1) == c;
+        return j < npre || own_step(j).list == c;
+    };
+    // the row of the tile of rows that an own slot belongs to
+    auto owner = [&](int slot) {
+        int lo = 0, hi = rows - 1;                         // the last row whose first slot is not behind it
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (plan.own_first[mid] <= slot) lo = mid; else hi = mid - 1;
+        }
+        return lo;
+    };
+    const int own_begin = prefix >> ss << ss;                // where every row's first own slot begins
+
+    // ---- the keys and values: lane c copies slot c of a step
+    const int* table = p.block_tables + (int64_t)leader * p.table_stride;                // the prefix lies where the group's first row says
+    auto copies_of = [&](int j) {
+        if (j < npre) return (min((x0 + j + 1) * PT_KEYS, prefix) - (x0 + j) * PT_KEYS + sk - 1) >> ss;
+        const OwnStep o = own_step(j);
+        return min(W, (o.list ? list_end[1] : list_end[0]) - (o.list ? list0[1] : 0) - o.k * W);
+    };
+    // Where this lane's copy of step j begins: the entry of a block table, fetched long before it is asked for, and the key's place in that page.
+    struct Place { int entry, page, offset; };
+    auto place_of = [&](int j) {
+        Place at = {0, 0, -1};
+        if (j >= J || lane >= copies_of(j)) return at;
+        int key;
+        const int* from = table;
+        if (j < npre) key = (x0 + j) * PT_KEYS + lane * sk;
+        else {
+            const OwnStep o = own_step(j);
+            const int slot = (o.list ? list0[1] : 0) + o.k * W + lane, i = owner(slot);
+            key = own_begin + (slot - plan.own_first[i]) * sk;
+            from = p.block_tables + (int64_t)(row0 + i) * p.table_stride;
+        }
+        at.entry = key >> p.page_shift;
+        at.page = from[at.entry];
+        at.offset = key & (p.page_size - 1);
+        return at;
+    };
+    auto row_of = [&](const Place& at) {                   // the cache's key row
+        if (at.offset < 0) return 0;
+        return (checked_page(at.page, p.num_pages, p.report, MIE_K_ATTENTION_PREFIX, at.entry) * p.num_kv_heads + kvh) * p.page_size + at.offset;
+    };
+    auto load = [&](int j, uint64_t* full, const CUtensorMap* map, uint32_t to, int src_row) {
         const int copies = copies_of(j);
-        if (lane == 0) mbar_expect_tx(&kv_full[st], (uint32_t)copies * rows_per_copy * 128u * PARTS * 2u);
+        if (lane == 0) mbar_expect_tx(full, (uint32_t)copies * sk * 128u * PARTS);
         __syncwarp();
         if (lane < copies) {
-            const int key = key_lo + j * PT_KEYS + lane * rows_per_copy;
-            const int src_row = (page * p.num_kv_heads + kvh) * p.page_size + (key & (p.page_size - 1));
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                const uint32_t off = part * SUB + (uint32_t)lane * rows_per_copy * 128u;
-                tma_load_2d(tiles + k_off(st) + off, &map_k, &kv_full[st], part * 64, src_row);
-                tma_load_2d(tiles + v_off(st) + off, &map_v, &kv_full[st], part * 64, src_row);
-            }
+            for (int part = 0; part < PARTS; ++part) tma_load_2d(tiles + to + part * SUB + (uint32_t)lane * sk * 128u, map, full, part * 64, src_row);
         }
     };
-    const int ahead = min(STAGES, J);
-    if (warp == 0) {
-        int pages[STAGES];
+    // Warp 0 fetches keys, warp 11 values: neither waits for places of the other's.
+    const bool fetches = warp == 0 || warp == 11;
+    uint64_t* full = warp == 0 ? k_full : v_full;
+    uint64_t* empty = warp == 0 ? k_empty : v_empty;
+    const CUtensorMap* map = warp == 0 ? &map_k : &map_v;
+    auto to = [&](int st) { return warp == 0 ? k_off(st) : v_off(st); };
+    const int ahead = min(STAGES, J), early = min(ahead, npre);      // the prefix is older than the step: its first keys are on their way before the wait
+    Place later;                                           // of the step behind those that shared memory has places for
+    if (fetches) {
+        Place at[STAGES];
 #pragma unroll
-        for (int j = 0; j < STAGES; ++j) pages[j] = page_of(j);
+        for (int j = 0; j < STAGES; ++j) at[j] = place_of(j);
 #pragma unroll
-        for (int j = 0; j < STAGES; ++j) if (j < ahead) load_tile(j, j, pages[j]);
+        for (int j = 0; j < STAGES; ++j) if (j < early) load(j, &full[j], map, to(j), row_of(at[j]));
+        pdl_wait();
+#pragma unroll
+        for (int j = 0; j < STAGES; ++j) if (j >= early && j < ahead) load(j, &full[j], map, to(j), row_of(at[j]));
+        later = place_of(STAGES);
     }
     // Tensor memory is taken behind the wait, and the next kernel let in behind that: a block that held it before the kernels in front are done could keep
     // it from a block of theirs, and one that came later from this one.
     pdl_wait();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = s_chunk;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    const int per_row = splits * (both ? 1 : 2);           // results of a row
+    if (unit == 0 && split == 0)                           // where the joining kernel finds them
+        for (int i = threadIdx.x; i < rows; i += PT_THREADS) wp.row_info[row0 + i] = make_int2(plan.slot0 + i * per_row, plan.ctx[i] ? per_row : 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem_base = tmem_base_slot;
 
-    if (warp == 0) {
-        // the rest of the tiles, their pages looked up a tile ahead
-        int page_next = page_of(ahead);
-        for (int j = ahead; j < J; ++j) {
-            const int st = j % STAGES, round = j / STAGES, page = page_next;
-            page_next = page_of(j + 1);
+    if (fetches) {
+        // the rest of the steps
+        // (asking L2 for later steps as well gained nothing: 53 -> 57 us for 64 rows behind 8,000 keys.  A copy's instruction takes 100 cycles for every lane that
+        // issues one, and sixteen a step are two thirds of what a step may take already.)
+        for (int j = STAGES; j < J; ++j) {
+            const int st = j % STAGES, src_row = row_of(later);
+            later = place_of(j + 1);
             int ok = 1;
-            if (lane == 0) ok = mbar_wait(&kv_empty[st], (round & 1) ^ 1, abort_p) ? 1 : 0;
+            if (lane == 0) ok = mbar_wait(&empty[st], ((j / STAGES) & 1) ^ 1, abort_p) ? 1 : 0;
             ok = __shfl_sync(0xffffffffu, ok, 0);
             if (!ok) break;
-            load_tile(j, st, page);
+            load(j, &full[st], map, to(st), src_row);
         }
     } else if (warp == 1 || warp == 10) {
         const int mu = warp == 1 ? 0 : 1;
-        if (lane == 0 && mu < nsub) {
-            // ---- the thread that issues for group mu
+        {
+            // ---- the warp that issues for chain mu: it walks its loop as a whole, so that what feeds the instructions stays uniform, and one lane issues
+            const bool issuer = elect_one();               // (one lane alone in the loop: 740 cycles for the eight products of P V instead of 300)
+            auto wait_for = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_p)) != 0; };
             const uint32_t idesc_s = umma_idesc_bf16(PT_ROWS, PT_KEYS), idesc_o = umma_idesc_bf16(PT_ROWS, D) | (1u << 16);
             constexpr int KS = D / 16, KV = PT_KEYS / 16;
+            const int qt = both ? mu : 0;
             uint64_t dq[KS];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) dq[ks] = umma_desc_sw128(base + q_off(mu) + (ks / 4) * SUB + (ks % 4) * 32);
+            for (int ks = 0; ks < KS; ++ks) dq[ks] = umma_desc_sw128(base + q_off(qt) + (ks / 4) * SUB + (ks % 4) * 32);
             const uint64_t dk0 = umma_desc_sw128(base + k_off(0)), dv0 = umma_desc_sw128_mn(base + v_off(0), SUB);
             constexpr uint64_t STAGE_STEP = (2 * TILE) >> 4;       // descriptors of another stage differ in the address field only
             const uint32_t s_at = tmem_base + TMEM_S + S_STEP * mu, p_at = tmem_base + TMEM_P + P_STEP * mu, o_at = tmem_base + TMEM_O + O_STEP * mu;
-            auto issue_s = [&](int st) {
+            int last = J - 1;                              // the chain's last step (-1: it has none)
+            while (last >= 0 && !active(mu, last)) --last;
+            bool ok = wait_for(&q_full[qt], 0);
+            auto scores = [&](int j) {                     // S of step j, once its keys are here
+                const int st = j % STAGES;
+                ok = wait_for(&k_full[st], (j / STAGES) & 1);
+                if (!ok) return;
+                tc_fence_after();
+                if (issuer) {
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
                     umma_bf16(s_at, dq[ks], dk0 + STAGE_STEP * st + (uint64_t)(((ks / 4) * SUB + (ks % 4) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
                 umma_commit(&s_full[mu]);
+                umma_commit(&k_empty[st]);
+                }
+                __syncwarp();
             };
-            bool ok = mbar_wait(&q_full[mu], 0, abort_p);
-            if (ok) ok = mbar_wait(&kv_full[0], 0, abort_p);
-            if (ok) { tc_fence_after(); issue_s(0); }
-            int st = 0, round = 0;
+            if (ok && active(mu, 0)) scores(0);
+            int used = 0;                                  // steps that the chain has taken part in
             for (int j = 0; j < J && ok; ++j) {
-                const int st_next = st + 1 == STAGES ? 0 : st + 1, round_next = st + 1 == STAGES ? round + 1 : round;
-                if (!OVER && j + 1 < J) {                  // the next scores, as soon as the rows of these are in registers
-                    ok = mbar_wait(&s_free[mu], j & 1, abort_p) && mbar_wait(&kv_full[st_next], round_next & 1, abort_p);
+                const int st = j % STAGES;
+                const uint32_t parity = (j / STAGES) & 1;
+                const bool now = active(mu, j), next = j + 1 < J && active(mu, j + 1), soon = !OVER && now && next;
+                if (soon) {                                // the next scores, as soon as the rows of these are in registers
+                    ok = wait_for(&s_free[mu], used & 1);
+                    if (ok) scores(j + 1);
+                    if (!ok) break;
+                }
+                if (now) {
+                    ok = wait_for(&p_full[mu], used & 1) && wait_for(&v_full[st], parity);      // P(j) is written, O rescaled
                     if (!ok) break;
                     tc_fence_after();
-                    issue_s(st_next);
-                }
-                ok = mbar_wait(&p_full[mu], j & 1, abort_p);       // P(j) is written, O rescaled
-                if (!ok) break;
-                tc_fence_after();
+                    if (issuer) {
 #pragma unroll
-                for (int kk = 0; kk < KV; ++kk)
-                    umma_bf16_ts(o_at, p_at + kk * 8, dv0 + STAGE_STEP * st + (uint64_t)((kk * 2048) >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-                umma_commit(&pv_done[mu]);                 // P may be overwritten, O rescaled
-                if (j + 1 == J) umma_commit(&o_full[mu]);
-                umma_commit(&kv_empty[st]);
-                if (OVER && j + 1 < J) {                   // (products run in the order they were issued: P has been read when S overwrites it)
-                    ok = mbar_wait(&kv_full[st_next], round_next & 1, abort_p);
+                    for (int kk = 0; kk < KV; ++kk)
+                        umma_bf16_ts(o_at, p_at + kk * 8, dv0 + STAGE_STEP * st + (uint64_t)((kk * 2048) >> 4), idesc_o, (used > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit(&pv_done[mu]);             // P may be overwritten, O rescaled
+                    if (j == last) umma_commit(&o_full[mu]);
+                    umma_commit(&v_empty[st]);
+                    }
+                    __syncwarp();
+                    ++used;
+                } else {                                   // a stage is given back only once it has been filled: an arrival ahead would count for another round
+                    ok = wait_for(&k_full[st], parity);
                     if (!ok) break;
-                    tc_fence_after();
-                    issue_s(st_next);
+                    if (issuer) mbar_arrive(&k_empty[st]);
+                    ok = wait_for(&v_full[st], parity);
+                    if (!ok) break;
+                    if (issuer) mbar_arrive(&v_empty[st]);
                 }
-                st = st_next; round = round_next;
+                // (products run in the order they were issued: where P lies over S, it has been read when the next S overwrites it)
+                if (next && !soon) scores(j + 1);
             }
         }
         __syncwarp();
     } else {
-        // ---- softmax group u = 0 (warps 2..5) or 1 (warps 6..9): a thread a pair
+        // ---- softmax of chain u = 0 (warps 2..5) or 1 (warps 6..9): a thread a pair
         const int u = warp >= 6 ? 1 : 0, q = warp & 3, r = q * 32 + lane;      // (the lanes of tensor memory that a warp reaches go by its number)
         const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16);
         const uint32_t S_AT = lane_addr + TMEM_S + S_STEP * u, P_AT = lane_addr + TMEM_P + P_STEP * u, O_AT = lane_addr + TMEM_O + O_STEP * u;
         bool ok = true;
-        if (u < nsub) {
-            const int in_tile = r / heads, my_row = row0 + u * half + in_tile, head = kvh * G + h0 + r - in_tile * heads;
-            const bool pair = in_tile < half && u * half + in_tile < rows;
-            {
-                const bf16* src = pair && p.row_q_len[my_row] == 1 ? p.q + (int64_t)p.row_q_start[my_row] * p.q_stride + (int64_t)head * D : nullptr;
-                uint4 v[D / 8];
+        const int in_tile = (both ? u * half : 0) + r / heads, my_row = row0 + in_tile, head = kvh * G + h0 + r % heads;
+        const bool pair = r / heads < half && in_tile < rows && plan.ctx[min(in_tile, rows - 1)] > 0;
+        if (both || u == 0) {                              // queries
+            const bf16* src = pair ? p.q + (int64_t)p.row_q_start[my_row] * p.q_stride + (int64_t)head * D : nullptr;
+            uint4 v[D / 8];
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) v[i] = src ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < D / 8; ++i) v[i] = src ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    *reinterpret_cast<uint4*>(tiles + q_off(u) + (i >> 3) * SUB + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = v[i];
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[u]);
-            }
-            float m_run = -INFINITY, l_run = 0.f;
-            for (int j = 0; j < J && ok; ++j) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], j & 1, abort_p));
+            for (int i = 0; i < D / 8; ++i)
+                *reinterpret_cast<uint4*>(tiles + q_off(u) + (i >> 3) * SUB + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = v[i];
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[u]);
+        }
+        // own keys that this pair sees, counted from its list's first: [seen_lo, seen_hi)
+        int seen_lo = 0, seen_hi = 0;
+        if (pair && plan.own_first[in_tile + 1] > plan.own_first[in_tile]) {
+            const int at = (plan.own_first[in_tile] - (both && u ? list0[1] : 0)) << ss;
+            seen_lo = at + (prefix - own_begin);
+            seen_hi = at + (plan.ctx[in_tile] - own_begin);
+        }
+        float m_run = -INFINITY, l_run = 0.f;
+        int used = 0;
+        for (int j = 0; j < J && ok; ++j) {
+            if (!active(u, j)) continue;
+            const int st = j % STAGES;
+            // the keys of the step that this pair sees: [lo, hi)
+            int lo = 0, hi = min(PT_KEYS, prefix - (x0 + j) * PT_KEYS);
+            unsigned char* v_row = tiles + v_off(st) + r * 128;            // the values of key r of the step (its 16-byte pieces in the swizzle's order)
+            if (j >= npre) {                               // (under the product that forms the scores)
+                const OwnStep o = own_step(j);
+                lo = max(0, min(PT_KEYS, seen_lo - o.k * PT_KEYS));
+                hi = max(lo, min(PT_KEYS, seen_hi - o.k * PT_KEYS));
+                // key r: whose is it, and is it one of its keys?
+                const int slot = (o.list ? list0[1] : 0) + o.k * W + (r >> ss);
+                bool valid = false;
+                int i = 0;
+                if (slot < (o.list ? list_end[1] : list_end[0])) {
+                    i = owner(slot);
+                    const int key = own_begin + ((slot - plan.own_first[i]) << ss) + (r & (sk - 1));
+                    valid = key >= prefix && key < plan.ctx[i];
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / STAGES) & 1, abort_p));
                 if (!ok) break;
-                tc_fence_after();
-                const int left = key_hi - (key_lo + j * PT_KEYS);      // keys of the tile that there are
+                if (!valid) {
+#pragma unroll
+                    for (int c = 0; c < 8 * PARTS; ++c) *reinterpret_cast<uint4*>(v_row + (c >> 3) * SUB + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                } else {
+                    uint32_t bad = 0;                      // an exponent of all ones carries into its number's highest bit
+#pragma unroll
+                    for (int c = 0; c < 8 * PARTS; ++c) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(v_row + (c >> 3) * SUB + (c & 7) * 16);
+                        bad |= ((v.x & 0x7f807f80u) + 0x00800080u) | ((v.y & 0x7f807f80u) + 0x00800080u) | ((v.z & 0x7f807f80u) + 0x00800080u) | ((v.w & 0x7f807f80u) + 0x00800080u);
+                    }
+                    if (bad & 0x80008000u) {
+                        for (int c = 0; c < 8 * PARTS * 4; ++c) {
+                            uint32_t* at = reinterpret_cast<uint32_t*>(v_row + (c >> 5) * SUB + (c & 31) * 4);
+                            uint32_t x = *at;
+                            if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+                            if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
+                            *at = x;
+                        }
+                        wp.marks[(int64_t)(row0 + i) * p.num_kv_heads + kvh] = G;
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                }
+            }
+            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], used & 1, abort_p));
+            if (!ok) break;
+            tc_fence_after();
+            float alpha = 1.f;
+            if (__any_sync(0xffffffffu, hi > lo)) {
                 uint32_t sv[128];
                 tmem_ld32_async(S_AT, sv);
                 tmem_ld32_async(S_AT + 32, sv + 32);
                 tmem_ld32_async(S_AT + 64, sv + 64);
                 tmem_ld32_async(S_AT + 96, sv + 96);
-                if (left < PT_KEYS && r >= left) {         // values of keys that there are not (their weights are 0, and 0 * NaN is NaN): both groups write the same zeros
+                if (j < npre && r >= hi) {                 // behind the prefix's end: zeros for its values (both chains write the same; the keys' arrival is long past)
+                    ok = mbar_wait(&v_full[st], (j / STAGES) & 1, abort_p);
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<uint4*>(tiles + v_off(j % STAGES) + part * SUB + r * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                    for (int c = 0; c < 8 * PARTS; ++c) *reinterpret_cast<uint4*>(v_row + (c >> 3) * SUB + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 tmem_ld_wait(sv); tmem_ld_wait(sv + 32); tmem_ld_wait(sv + 64); tmem_ld_wait(sv + 96);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
                 tc_fence_before();
                 __syncwarp();
                 if (!OVER && lane == 0) mbar_arrive(&s_free[u]);
-                if (left < PT_KEYS) {
+                if (__any_sync(0xffffffffu, lo > 0 || hi < PT_KEYS)) {
+                    const unsigned n = hi - lo;
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) if (i >= left) sv[i] = __float_as_uint(-INFINITY);
+                    for (int i = 0; i < 128; ++i) if ((unsigned)(i - lo) >= n) sv[i] = __float_as_uint(-INFINITY);
                 }
                 // the reference point of the exponent moves only when a score would exceed 2^8 against the one in use
-                float alpha = 1.f, sum;
                 {
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -449,68 +712,90 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                         m_run = mx;
                     }
                 }
-                if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (j - 1) & 1, abort_p))) { ok = false; break; }
-                if (nsub == 2) {                           // the groups take turns at the exponentials
+                if (used > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (used - 1) & 1, abort_p))) { ok = false; break; }
+                if (both && j < npre) {                    // the chains take turns at the exponentials of the steps that both take part in
                     const int turn = u == 0 ? j - 1 : j;
                     if (turn >= 0 && !__all_sync(0xffffffffu, mbar_wait(&exp_done[u ^ 1], turn & 1, abort_p))) { ok = false; break; }
                 }
-                {
-                    const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-                    float sm[4] = {0.f, 0.f, 0.f, 0.f};
+                const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+                float sm[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int ch = 0; ch < 4; ++ch) {
-                        uint32_t packed[16];
+                for (int ch = 0; ch < 4; ++ch) {
+                    uint32_t packed[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float p0 = ex2_approx(fmaf(__uint_as_float(sv[ch * 32 + i]), p.scale_log2e, neg_m));
-                            const float p1 = ex2_approx(fmaf(__uint_as_float(sv[ch * 32 + i + 1]), p.scale_log2e, neg_m));
-                            sm[(i >> 1) & 3] += p0 + p1;
-                            packed[i >> 1] = pack2_bf16(p0, p1);
-                        }
-                        tmem_st16(P_AT + ch * 16, packed);
+                    for (int i = 0; i < 32; i += 2) {
+                        const float p0 = ex2_approx(fmaf(__uint_as_float(sv[ch * 32 + i]), p.scale_log2e, neg_m));
+                        const float p1 = ex2_approx(fmaf(__uint_as_float(sv[ch * 32 + i + 1]), p.scale_log2e, neg_m));
+                        sm[(i >> 1) & 3] += p0 + p1;
+                        packed[i >> 1] = pack2_bf16(p0, p1);
                     }
-                    sum = (sm[0] + sm[1]) + (sm[2] + sm[3]);
+                    tmem_st16(P_AT + ch * 16, packed);
                 }
+                l_run = l_run * alpha + ((sm[0] + sm[1]) + (sm[2] + sm[3]));
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&exp_done[u]);
-                l_run = l_run * alpha + sum;
-                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {
-                        float v[16];
-                        tmem_ld16(O_AT + c, v);
-                        uint32_t w[16];
+                if (both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
+            } else {                                       // own keys of other warps' rows (never a step of the prefix): weights of zero
+                if (!OVER && lane == 0) mbar_arrive(&s_free[u]);
+                if (used > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (used - 1) & 1, abort_p))) { ok = false; break; }
+                uint32_t none[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i] * alpha);
-                        tmem_st8(O_AT + c, w);
-                        tmem_st8(O_AT + c + 8, w + 8);
-                    }
-                }
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[u]);
+                for (int i = 0; i < 16; ++i) none[i] = 0;
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) tmem_st16(P_AT + ch * 16, none);
             }
-            if (ok) ok = mbar_wait(&o_full[u], 0, abort_p);
-            tc_fence_after();
-            __syncwarp();
-            if (__all_sync(0xffffffffu, ok)) {
-                const float inv = l_run > 0.f ? 1.0f / l_run : l_run == 0.f ? 0.f : NAN;      // a sum that is no number stays none
-                const int64_t slot = t.slot0 + (int64_t)(my_row - t.first_row) * t.splits + split;
-                const bool writes = pair && slot < p.most_slots;       // (the host sizes the scratch memory for every plan)
-                float* op = p.part_o + (slot * p.num_heads + head) * D;
+            if (used > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
                 for (int c = 0; c < D; c += 16) {
                     float v[16];
                     tmem_ld16(O_AT + c, v);
-                    if (!writes) continue;
+                    uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<float4*>(op + c + i) = make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+                    for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i] * alpha);
+                    tmem_st8(O_AT + c, w);
+                    tmem_st8(O_AT + c + 8, w + 8);
                 }
-                if (writes) p.part_lse[slot * p.num_heads + head] = l_run != 0.f ? m_run + __log2f(l_run) : -INFINITY;
-                tc_fence_before();
             }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[u]);
+            ++used;
+        }
+        if (ok && used > 0) ok = mbar_wait(&o_full[u], 0, abort_p);
+        tc_fence_after();
+        __syncwarp();
+        if (__all_sync(0xffffffffu, ok)) {
+            const float inv = l_run > 0.f ? 1.0f / l_run : l_run == 0.f ? 0.f : NAN;      // a sum that is no number stays none
+            const int64_t slot = plan.slot0 + (int64_t)in_tile * per_row + (both ? split : 2 * split + u);
+            const bool writes = pair && slot < p.most_slots;       // (the host sizes the scratch memory for every plan)
+            if (writes) p.part_lse[slot * p.num_heads + head] = l_run != 0.f ? m_run + __log2f(l_run) : -INFINITY;
+            // O goes through shared memory a quarter of its columns at a time, so that a pair's entries leave side by side (written out of the registers, 128 bytes
+            // apart a lane, they took 10,000 cycles a block).  The queries' place is free: this chain's, or the half of the unused one.
+            constexpr int COLS = D / 4, PIECES = COLS / 4;         // entries and 16-byte pieces of a pass
+            float* stage = reinterpret_cast<float*>(tiles + (both ? q_off(u) : q_off(1) + u * (TILE / 2))) + q * 32 * COLS;
+            auto piece = [&](int row, int c) { return row * PIECES + (PIECES == 8 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)); };
+            const int to = writes && l_run != 0.f ? (int)(slot * p.num_heads + head) : -1;
+            if (__any_sync(0xffffffffu, to >= 0)) {
+#pragma unroll 1
+                for (int pass = 0; pass < 4; ++pass) {
+#pragma unroll
+                    for (int c = 0; c < COLS; c += 16) {
+                        float v[16];
+                        tmem_ld16(O_AT + pass * COLS + c, v);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            *reinterpret_cast<float4*>(stage + piece(lane, (c + i) / 4) * 4) = make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < PIECES; ++k) {
+                        const int row = k * (32 / PIECES) + lane / PIECES, c = lane % PIECES, dst = __shfl_sync(0xffffffffu, to, row);
+                        if (dst >= 0) *reinterpret_cast<float4*>(p.part_o + (int64_t)dst * D + pass * COLS + c * 4) = *reinterpret_cast<const float4*>(stage + piece(row, c) * 4);
+                    }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
         }
     }
 
@@ -526,6 +811,102 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     }
 }
 
+// Joins the ranges of a row's walk: out = sum_s 2^(L_s - max L) o_s / sum_s 2^(L_s - max L).  A warp a head, a lane D / 32 entries of it.
+#define JOIN_WARPS 8
+template <int D>
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+prefix_join_kernel(const WalkParams wp, bf16* __restrict__ out, float* __restrict__ out32) {
+    constexpr int E = D / 32;
+    pdl_enter();
+    const PrefixParams& p = wp.b;
+    const int row = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
+    const int2 info = __ldcg(wp.row_info + row);
+    const int S = min(info.y, 2 * PREFIX_MAX_SPLITS);
+    if (p.row_q_len[row] != 1 || wp.row_ctx_len[row] <= 0 || head >= p.num_heads) return;      // (a row of more than one new token is left alone)
+    if (S <= 0 || (int64_t)info.x + S > p.most_slots) return;
+    const int kvh = head / (p.num_heads / p.num_kv_heads);
+    int* mark = wp.marks + (int64_t)row * p.num_kv_heads + kvh;
+    const int marked = __ldcg(mark);
+    const float* lse = p.part_lse + (int64_t)info.x * p.num_heads + head;
+    const float* from = p.part_o + ((int64_t)info.x * p.num_heads + head) * D + lane * E;
+    const int64_t step = (int64_t)p.num_heads * D;
+    constexpr int WORDS = 2 * PREFIX_MAX_SPLITS / 32;
+    float w[WORDS], mm = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < WORDS; ++h) {
+        w[h] = h * 32 + lane < S ? __ldcg(lse + (int64_t)(h * 32 + lane) * p.num_heads) : -INFINITY;
+        mm = fmaxf(mm, w[h]);
+    }
+    mm = warp_max(mm);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (int h = 0; h < WORDS; ++h) { w[h] = exp2_fast(w[h] - ref); sum += w[h]; }
+    sum = warp_sum(sum);
+    const float inv = sum > 0.f ? __frcp_rn(sum) : sum == 0.f ? 0.f : sum;
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    // results of ranges in which the pair saw no key hold nothing: they are passed over; eight of the others are asked for at a time
+#pragma unroll
+    for (int h = 0; h < WORDS; ++h) {
+        if (h * 32 >= S) break;
+        unsigned left = __ballot_sync(0xffffffffu, w[h] != 0.f);
+        while (left) {
+            float v[8][E], wk[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int l = left ? __ffs(left) - 1 : 0;
+                wk[k] = left ? __shfl_sync(0xffffffffu, w[h], l) * inv : 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[k][e] = 0.f;
+                if (left) {
+                    left &= left - 1;
+                    const float* src = from + (int64_t)(h * 32 + l) * step;
+                    if constexpr (E == 4) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+                        v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
+                    } else {
+                        const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+                        v[k][0] = x.x; v[k][1] = x.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = fmaf(wk[k], v[k][e], acc[e]);
+        }
+    }
+    if (marked) {                                          // own values that are not finite: each reaches the output as it is (its weight is positive)
+        int prefix = 0;
+        for (int g = 0; g < p.groups.groups; ++g) {
+            const PrefixPart t = prefix_group(p.groups, g);
+            if (row >= t.first_row && row < t.first_row + t.rows) { prefix = t.keys; break; }
+        }
+        const int ctx = min(wp.row_ctx_len[row], p.groups.most_keys);
+        for (int key = prefix; key < ctx; ++key) {
+            const int entry = key >> p.page_shift;
+            const int page = checked_page(p.block_tables[(int64_t)row * p.table_stride + entry], p.num_pages, p.report, MIE_K_ATTENTION_PREFIX, entry);
+            const bf16* v = p.v_cache + (((int64_t)page * p.num_kv_heads + kvh) * p.page_size + (key & (p.page_size - 1))) * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = __bfloat162float(v[e]);
+                if (!isfinite(x)) acc[e] += x;
+            }
+        }
+        __syncwarp();
+        if (lane == 0) atomicSub(mark, 1);                 // the last of the key head's query heads leaves it 0
+    }
+    const int64_t at = ((int64_t)p.row_q_start[row] * p.num_heads + head) * D + lane * E;
+    if (out32) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) out32[at + e] = acc[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(out + at + e) = __floats2bfloat162_rn(acc[e], acc[e + 1]);
+    }
+}
+
 static int prefix_map(CUtensorMap* map, const void* ptr, uint64_t rows, int head_dim, int box_rows) {
     cuuint64_t gdim[2] = {(cuuint64_t)head_dim, rows};
     cuuint64_t gstride[1] = {(cuuint64_t)head_dim * 2};
@@ -536,55 +917,65 @@ static int prefix_map(CUtensorMap* map, const void* ptr, uint64_t rows, int head
 }
 
 template <int D>
-static int launch_prefix_tc(PrefixParams p, long long items, cudaStream_t stream) {
+static int launch_walk(WalkParams p, void* out, bool out_f32, long long items, cudaStream_t stream) {
     int rc = tc_setup();
     if (rc) return rc;
-    p.error = g_error_dev;
+    p.b.error = g_error_dev;
     CUtensorMap mk, mv;
-    const uint64_t rows = (uint64_t)p.num_pages * p.num_kv_heads * p.page_size;
-    const int box = p.page_size < PT_KEYS ? p.page_size : PT_KEYS;
-    if ((rc = prefix_map(&mk, p.k_cache, rows, D, box)) || (rc = prefix_map(&mv, p.v_cache, rows, D, box))) return rc;
-    const cudaError_t e = cudaFuncSetAttribute(prefix_attention_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PT_SMEM<D>);
+    const uint64_t rows = (uint64_t)p.b.num_pages * p.b.num_kv_heads * p.b.page_size;
+    const int box = p.b.page_size < PT_KEYS ? p.b.page_size : PT_KEYS;
+    if ((rc = prefix_map(&mk, p.b.k_cache, rows, D, box)) || (rc = prefix_map(&mv, p.b.v_cache, rows, D, box))) return rc;
+    const cudaError_t e = cudaFuncSetAttribute(prefix_walk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PT_SMEM<D>);
     if (e != cudaSuccess) return (int)e;
-    return launch_kernel(prefix_attention_tc_kernel<D>, dim3((unsigned)items), dim3(PT_THREADS), PT_SMEM<D>, stream, mk, mv, p);
+    if ((rc = launch_kernel(prefix_walk_kernel<D>, dim3((unsigned)items), dim3(PT_THREADS), PT_SMEM<D>, stream, mk, mv, p))) return rc;
+    return launch_kernel(prefix_join_kernel<D>, dim3(p.b.groups.num_rows, (p.b.num_heads + JOIN_WARPS - 1) / JOIN_WARPS), dim3(JOIN_WARPS * 32), 0, stream, p,
+                         out_f32 ? nullptr : (bf16*)out, out_f32 ? (float*)out : nullptr);
 }
 
-// How a launch on `sms` SMs cuts (row, head) pairs: out[0] query heads a unit, out[1] units a key head, out[2] rows an item, out[3] items side by side,
-// out[4] 1: the tcgen05 kernel (heads of 64 and 128, pages of 8 positions or more), 0: the other.  Also the most slots (rows of num_heads x head_dim
-// float32, and num_heads float32) that it writes, as the return value; -1: a size it does not take.
-extern "C" long long mie_prefix_layout(int num_rows, int num_heads, int num_kv_heads, int head_dim, int page_size, int sms, int* out) {
-    if (num_rows < 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || head_dim < 16 || head_dim > 128 || head_dim % 16 || sms <= 0) return -1;
-    const int G = num_heads / num_kv_heads, tc = (head_dim == 64 || head_dim == 128) && page_size >= 8, pairs = tc ? PT_ROWS : PFX_PAIRS;
-    out[1] = (G + pairs - 1) / pairs;
-    out[0] = (G + out[1] - 1) / out[1];
-    out[2] = pairs / out[0] * (tc ? 2 : 1);
-    out[3] = tc ? sms : 2 * sms;
-    out[4] = tc;
-    return prefix_most_slots(num_rows, num_kv_heads * out[1], out[2], out[3]);
+// The arguments of attention over shared prefixes as the caller keeps them (kernels/ops.py).  How pairs are cut (mie_prefix_layout): chunk_heads query heads
+// a unit, `chunks` units a key head, tile_rows rows an item, `places` items side by side, walk 1: the walk above, 0: the kernel for any head size, and
+// attention_decode_shared.cu behind it.
+#include "prefix_args.cuh"
+
+// Fills in the layout, and most_slots: the most slots of partial results (num_heads x head_dim float32, and num_heads float32) that a launch writes.
+// Non-zero: a size that is not taken.
+extern "C" int mie_prefix_layout(SharedArgs* a, int sms) {
+    if (a->num_rows < 0 || a->num_kv_heads <= 0 || a->num_heads <= 0 || a->num_heads % a->num_kv_heads || a->head_dim < 16 || a->head_dim > 128 || a->head_dim % 16
+        || sms <= 0 || a->page_size < 1 || (a->page_size & (a->page_size - 1))) return MIE_ERR_BAD_ARG;
+    const int G = a->num_heads / a->num_kv_heads;
+    for (a->walk = 1; a->walk >= 0; --a->walk) {
+        const int pairs = a->walk ? PT_ROWS : PFX_PAIRS;
+        a->chunks = (G + pairs - 1) / pairs;
+        a->chunk_heads = (G + a->chunks - 1) / a->chunks;
+        a->tile_rows = pairs / a->chunk_heads * (a->walk ? 2 : 1);
+        a->places = a->walk ? sms : 2 * sms;
+        if ((a->head_dim == 64 || a->head_dim == 128) && a->page_size >= 8 && a->groups + 2 <= PT_MOST_SEGMENTS
+            && (a->num_rows + a->tile_rows - 1) / a->tile_rows + a->groups + 2 <= PT_MOST_TILES) break;
+        if (!a->walk) break;
+    }
+    a->most_slots = prefix_most_slots(a->num_rows, a->num_kv_heads * a->chunks, a->tile_rows, a->places);
+    return 0;
 }
 
-extern "C" int mie_prefix_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const int* block_tables, int table_stride,
-                                    const int* row_q_start, const int* row_q_len, int num_rows, const int* group_start, const int* group_prefix, int groups,
-                                    int num_heads, int num_kv_heads, int head_dim, int page_size, float scale, const int* layout, float* part_o,
-                                    float* part_lse, int* chunk, long long most_slots, long long num_pages, cudaStream_t stream) {
-    if (num_rows <= 0 || groups <= 0) return 0;
-    if (num_kv_heads <= 0 || num_heads % num_kv_heads) return MIE_ERR_BAD_ARG;
-    if (page_size < 1 || (page_size & (page_size - 1))) return MIE_ERR_BAD_ARG;
-    PrefixParams p = {};
-    p.q = (const bf16*)q; p.q_stride = q_stride; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache;
-    p.block_tables = block_tables; p.table_stride = table_stride; p.row_q_start = row_q_start; p.row_q_len = row_q_len;
-    p.part_o = part_o; p.part_lse = part_lse; p.most_slots = most_slots; p.chunk = chunk;
-    p.num_heads = num_heads; p.num_kv_heads = num_kv_heads; p.page_size = page_size;
-    while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    p.chunk_heads = layout[0]; p.chunks = layout[1];
-    p.scale_log2e = scale * 1.4426950408889634f;
-    p.num_pages = num_pages; p.report = g_range_report;
-    const int64_t covered = (int64_t)table_stride * page_size;
-    p.groups = PrefixGroups{group_start, group_prefix, groups, num_rows, (int)(covered < 0x7fffff00ll ? covered : 0x7fffff00ll), num_kv_heads * layout[1], layout[2], layout[3]};
-    const long long items = prefix_most_items(num_rows, groups, p.groups.units, p.groups.tile_rows, p.groups.places);
+extern "C" int mie_prefix_attention(const SharedArgs* a, cudaStream_t stream) {
+    if (a->num_rows <= 0 || (!a->walk && a->groups <= 0)) return 0;
+    if (a->num_rows > 65535) return MIE_ERR_TOO_LARGE;
+    WalkParams w = {};
+    PrefixParams& p = w.b;
+    p.q = (const bf16*)a->q; p.q_stride = a->q_stride; p.k_cache = (const bf16*)a->k_cache; p.v_cache = (const bf16*)a->v_cache;
+    p.block_tables = a->block_tables; p.table_stride = a->table_stride; p.row_q_start = a->row_q_start; p.row_q_len = a->row_q_len;
+    p.part_o = a->pre_o; p.part_lse = a->pre_lse; p.most_slots = a->most_slots; p.chunk = a->pre_chunk;
+    p.num_heads = a->num_heads; p.num_kv_heads = a->num_kv_heads; p.page_size = a->page_size;
+    while ((1 << p.page_shift) < a->page_size) ++p.page_shift;
+    p.chunk_heads = a->chunk_heads; p.chunks = a->chunks;
+    p.scale_log2e = a->scale * 1.4426950408889634f;
+    p.num_pages = a->num_pages; p.report = g_range_report;
+    p.groups = shared_groups_of(*a);
+    w.row_ctx_len = a->row_ctx_len; w.row_info = (int2*)a->row_info; w.marks = a->marks;
+    const long long items = prefix_most_items(a->num_rows, a->walk ? a->groups + 2 : a->groups, p.groups.units, p.groups.tile_rows, p.groups.places);
     if (items > 0x7fffffffll) return MIE_ERR_TOO_LARGE;
-    if (layout[4]) return head_dim == 64 ? launch_prefix_tc<64>(p, items, stream) : launch_prefix_tc<128>(p, items, stream);
-    switch (head_dim) {
+    if (a->walk) return a->head_dim == 64 ? launch_walk<64>(w, a->out, a->out_f32 != 0, items, stream) : launch_walk<128>(w, a->out, a->out_f32 != 0, items, stream);
+    switch (a->head_dim) {
         case 16: return launch_prefix<16>(p, items, stream);
         case 32: return launch_prefix<32>(p, items, stream);
         case 48: return launch_prefix<48>(p, items, stream);

@@ -419,43 +419,44 @@ static int launch_rules(RuleParams& p, bool choose, cudaStream_t stream) {
     }
 }
 
-static void set_rules(RuleParams& p, const int* history, int64_t history_stride, int slots, int width, const int* slot, const int* prompt_len,
-                      const int* total_len, const float* repetition, const float* presence, const float* frequency, const int* bias_tokens,
-                      const float* bias_values, int bias_width, const int* bias_len, const int* mask, int64_t mask_stride, int masks, const int* mask_row) {
-    p.history = history; p.history_stride = history_stride; p.slots = slots; p.width = width;
-    p.slot = slot; p.prompt_len = prompt_len; p.total_len = total_len;
-    p.repetition = repetition; p.presence = presence; p.frequency = frequency;
-    p.bias_tokens = bias_tokens; p.bias_values = bias_values; p.bias_width = bias_width; p.bias_len = bias_len;
-    p.mask = mask; p.mask_stride = mask_stride; p.masks = masks; p.mask_row = mask_row;
+// The rules' arguments as the caller lays them out once for many calls (kernels/ops.py: LogitRules).
+struct RuleArgs {
+    const int* history; const int* slot; const int* prompt_len; const int* total_len;
+    const float* repetition; const float* presence; const float* frequency;
+    const int* bias_tokens; const float* bias_values; const int* bias_len;
+    const int* mask; const int* mask_row;
+    long long history_stride, mask_stride;
+    int slots, width, bias_width, masks;
+};
+static void set_rules(RuleParams& p, const RuleArgs& a) {
+    p.history = a.history; p.history_stride = a.history_stride; p.slots = a.slots; p.width = a.width;
+    p.slot = a.slot; p.prompt_len = a.prompt_len; p.total_len = a.total_len;
+    p.repetition = a.repetition; p.presence = a.presence; p.frequency = a.frequency;
+    p.bias_tokens = a.bias_tokens; p.bias_values = a.bias_values; p.bias_width = a.bias_width; p.bias_len = a.bias_len;
+    p.mask = a.mask; p.mask_stride = a.mask_stride; p.masks = a.masks; p.mask_row = a.mask_row;
     p.report = g_range_report;
 }
 
-#define RULE_ARGS const int* history, int64_t history_stride, int slots, int width, const int* slot, const int* prompt_len, const int* total_len,             \
-                  const float* repetition, const float* presence, const float* frequency, const int* bias_tokens, const float* bias_values, int bias_width,   \
-                  const int* bias_len, const int* mask, int64_t mask_stride, int masks, const int* mask_row
-#define RULE_NAMES history, history_stride, slots, width, slot, prompt_len, total_len, repetition, presence, frequency, bias_tokens, bias_values, bias_width, \
-                   bias_len, mask, mask_stride, masks, mask_row
-
 // out[r] = the logits of row r under its rules (out may be the logits).
-extern "C" int mie_apply_logit_rules(RULE_ARGS, const float* logits, int64_t logits_stride, float* out, int64_t out_stride, int rows, int vocab,
+extern "C" int mie_apply_logit_rules(const RuleArgs* rules, const float* logits, long long logits_stride, float* out, long long out_stride, int rows, int vocab,
                                      cudaStream_t stream) {
     RuleParams p = {};
-    set_rules(p, RULE_NAMES);
+    set_rules(p, *rules);
     p.logits = logits; p.logits_stride = logits_stride; p.out = out; p.out_stride = out_stride; p.rows = rows; p.vocab = vocab;
     if (rows > 0 && !out) return MIE_ERR_BAD_ARG;
     return launch_rules(p, false, stream);
 }
 
 // The token of every row under its rules; see mie_sample (sampling.cu) for the noise and the host's copy.  `logprob` (or null): log softmax of the
-// ruled logits at the token, -inf where the rules leave nothing (the token is 0 there).  `append` (or null, else the history): the token
-// joins the row's text.
-extern "C" int mie_sample_rules(RULE_ARGS, const float* logits, int64_t logits_stride, const float* temperature, const int64_t* request, const int* position,
-                                uint64_t seed, int* token, float* logprob, int* append, int rows, int vocab, int* host_out, const int* host_turn,
-                                int host_stride, cudaStream_t stream) {
+// ruled logits at the token, -inf where the rules leave nothing (the token is 0 there).  `append`: the token joins the row's text.
+extern "C" int mie_sample_rules(const RuleArgs* rules, const float* logits, long long logits_stride, const float* temperature, const int64_t* request,
+                                const int* position, uint64_t seed, int* token, float* logprob, int append, int rows, int vocab, int* host_out,
+                                const int* host_turn, int host_stride, cudaStream_t stream) {
     RuleParams p = {};
-    set_rules(p, RULE_NAMES);
+    set_rules(p, *rules);
     p.logits = logits; p.logits_stride = logits_stride; p.rows = rows; p.vocab = vocab;
     p.temperature = temperature; p.request = request; p.position = position; p.seed = seed;
-    p.token = token; p.logprob = logprob; p.append = append; p.host_out = host_out; p.host_turn = host_turn; p.host_stride = host_stride;
+    p.token = token; p.logprob = logprob; p.append = append ? const_cast<int*>(p.history) : nullptr;
+    p.host_out = host_out; p.host_turn = host_turn; p.host_stride = host_stride;
     return launch_rules(p, true, stream);
 }

@@ -1,0 +1,23 @@
+// Arguments of attention over shared prefixes, laid out alike in kernels/ops.py (_SharedArgs).
+#pragma once
+#include "prefix_plan.cuh"
+
+struct SharedArgs {
+    const void* q; const void* k_cache; const void* v_cache;
+    const int* block_tables; const int* row_q_start; const int* row_q_len; const int* row_ctx_len;
+    const int* group_start; const int* group_prefix;
+    void* out;
+    float* pre_o; float* pre_lse; int* pre_chunk; int* row_info; int* marks;      // scratch: partial results of ranges, how prefixes are cut, a row's results, rows marked
+    float* part_o; float* part_lse; int* counters;                                // scratch of the decode kernel (splits > 1); counters and marks are left zero
+    long long q_stride, num_pages, most_slots;
+    int table_stride, num_rows, groups, num_heads, num_kv_heads, head_dim, page_size, out_f32;
+    int splits, stages, tma, min_part_tiles;                                      // the decode kernel's plan for the rows' own keys
+    int chunk_heads, chunks, tile_rows, places, walk;                             // mie_prefix_layout
+    float scale;
+};
+
+static inline PrefixGroups shared_groups_of(const SharedArgs& a) {
+    const long long covered = (long long)a.table_stride * a.page_size;
+    return PrefixGroups{a.group_start, a.group_prefix, a.groups, a.num_rows, (int)(covered < 0x7fffff00ll ? covered : 0x7fffff00ll), a.num_kv_heads * a.chunks, a.tile_rows,
+                        a.places};
+}

@@ -67,7 +67,7 @@ __host__ __device__ __forceinline__ long long prefix_most_items(int rows, int gr
     return whole > 2ll * places ? whole : 2ll * places;
 }
 __host__ __device__ __forceinline__ long long prefix_most_slots(int rows, int units, int tile_rows, int places) {
-    return rows + 2ll * places * tile_rows / units + tile_rows;
+    return 2ll * rows + 2ll * places * tile_rows / units + tile_rows;      // (a walk's results come in twos where its pairs fill one tile only)
 }
 
 #ifdef __CUDACC__

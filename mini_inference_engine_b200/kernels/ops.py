@@ -39,6 +39,15 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr())
 
 
+def _at(t):
+    """A tensor's address for a launcher whose argument types are declared (None: null)."""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise KernelError("kernels of this package run on CUDA tensors only; got a tensor on " + str(t.device))
+    return t.data_ptr()
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -732,15 +741,49 @@ def decode_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, block_tab
     return out
 
 
+class _SharedArgs(ctypes.Structure):          # csrc/prefix_args.cuh
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k_cache", "v_cache", "block_tables", "row_q_start", "row_q_len", "row_ctx_len", "group_start", "group_prefix",
+                                                "out", "pre_o", "pre_lse", "pre_chunk", "row_info", "marks", "part_o", "part_lse", "counters")]
+                + [(n, ctypes.c_longlong) for n in ("q_stride", "num_pages", "most_slots")]
+                + [(n, ctypes.c_int) for n in ("table_stride", "num_rows", "groups", "num_heads", "num_kv_heads", "head_dim", "page_size", "out_f32", "splits",
+                                               "stages", "tma", "min_part_tiles", "chunk_heads", "chunks", "tile_rows", "places", "walk")]
+                + [("scale", ctypes.c_float)])
+
+
 @functools.lru_cache(maxsize=None)
-def _prefix_layout(rows: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, sms: int):
-    """How the prefix kernel cuts (row, head) pairs, as its library says, and the most slots of partial results that it writes."""
-    layout = (ctypes.c_int * 5)()
-    fn = load("attention_prefix").mie_prefix_layout
-    fn.restype = ctypes.c_longlong
-    slots = fn(rows, num_heads, num_kv_heads, head_dim, page_size, sms, layout)
-    _need(slots >= 0, f"{num_heads} heads of {head_dim} on {num_kv_heads}: the prefix kernel takes head sizes in steps of 16 up to 128")
-    return layout, slots
+def _shared_libs():
+    first, second = load("attention_prefix"), load("attention_decode_shared")
+    for fn in (first.mie_prefix_attention, second.mie_decode_attention_shared):
+        fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    return first, second
+
+
+@functools.lru_cache(maxsize=256)
+def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_own: int,
+                 pages: int):
+    """What a launch of these sizes keeps from call to call: its plan and its scratch memory, as the bytes of a _SharedArgs (and the tensors)."""
+    a = _SharedArgs(num_rows=rows, groups=groups, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size,
+                    num_pages=pages)
+    where = torch.device("cuda", device)
+    _need(_shared_libs()[0].mie_prefix_layout(ctypes.byref(a), num_sms(where)) == 0, f"{num_heads} heads of {head_dim} on {num_kv_heads}: not taken")
+    kept = [_workspace(where, "prefix_o", a.most_slots * num_heads * head_dim, torch.float32), _workspace(where, "prefix_lse", a.most_slots * num_heads, torch.float32),
+            _workspace(where, "prefix_chunk", 1, torch.int32), _workspace(where, "prefix_rows", 2 * rows, torch.int32),
+            _workspace(where, "prefix_marks", rows * num_kv_heads, torch.int32)]
+    for name, t in zip(("pre_o", "pre_lse", "pre_chunk", "row_info", "marks"), kept):
+        setattr(a, name, t.data_ptr())
+    if not a.walk:                                            # the rows' own keys by the decode kernel behind
+        units = num_kv_heads * -(-(num_heads // num_kv_heads) // 16)
+        tma_ok = head_dim in (64, 128) and page_size >= 8
+        a.splits, a.min_part_tiles = own_keys_plan(rows, units, max_own, tma_ok, head_dim)
+        blocks = rows * units * a.splits
+        a.tma = tma_ok and decode_uses_tma(blocks, head_dim)
+        a.stages = decode_stages(blocks, max_own, a.splits, bool(a.tma), head_dim, clustered=False)
+        if a.splits > 1:
+            more = [_workspace(where, "decode_part_o", rows * num_heads * a.splits * head_dim, torch.float32),
+                    _workspace(where, "decode_part_lse", rows * num_heads * a.splits, torch.float32), _workspace(where, "decode_counters", rows * units, torch.int32)]
+            a.part_o, a.part_lse, a.counters = (t.data_ptr() for t in more)
+            kept += more
+    return bytes(a), bool(a.walk), kept
 
 
 def own_keys_plan(rows: int, kv_units: int, max_own: int, tma_ok: bool, head_dim: int) -> tuple[int, int]:
@@ -768,60 +811,51 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     overlap; rows of no group share nothing.  A row's context (``row_ctx_len``) includes its prefix.  ``max_prefix`` and ``max_own``: bounds on the
     prefixes and on the keys behind them, for planning (a captured step's may be shorter); without them the block table's width bounds both.
 
-    Two launches: the groups' (row, head) pairs against the prefixes in tiles, then the rows' own keys, joined with those.  Rows with more than
-    one new token are skipped.  Slots of a row's last page behind its context must hold finite values (see ``decode_uses_tma``)."""
+    Two launches: the keys (prefixes in tiles of (row, head) pairs, and the rows' own), then what joins a row's partial results.  Rows with more than
+    one new token are skipped.  With other head sizes than 64 and 128, or pages below 8, slots of a row's last page behind its context must hold
+    finite values (see ``decode_uses_tma``)."""
     _need(q.dtype == torch.bfloat16 == k_cache.dtype == v_cache.dtype and out.dtype in (torch.bfloat16, torch.float32),
           "attention over shared prefixes is bfloat16 (its output bfloat16 or float32)")
-    for t, n in ((block_tables, "block_tables"), (row_q_start, "row_q_start"), (row_q_len, "row_q_len"), (row_ctx_len, "row_ctx_len"),
-                 (group_start, "group_start"), (group_prefix, "group_prefix")):
-        _i32(t, n)
+    i32 = torch.int32
+    _need(block_tables.dtype == row_q_start.dtype == row_q_len.dtype == row_ctx_len.dtype == group_start.dtype == group_prefix.dtype == i32
+          and block_tables.is_contiguous() and row_q_start.is_contiguous() and row_q_len.is_contiguous() and row_ctx_len.is_contiguous()
+          and group_start.is_contiguous() and group_prefix.is_contiguous(), "block tables, rows and groups must be contiguous int32 tensors")
     rows, groups = row_q_len.numel(), group_prefix.numel()
     _need(num_kv_heads > 0 and num_heads % num_kv_heads == 0, "query heads must be a multiple of kv heads")
     _need(head_dim % 16 == 0 and 16 <= head_dim <= 128, f"head_dim {head_dim}: attention over shared prefixes takes multiples of 16 from 16 to 128")
     _need(page_size >= 1 and page_size & (page_size - 1) == 0, "the page size must be a power of two")
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and tuple(k_cache.shape[1:]) == (num_kv_heads, page_size, head_dim)
-          and k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous [pages, kv heads, page size, head_dim]")
+    shape = k_cache.shape
+    _need(len(shape) == 4 and shape == v_cache.shape and shape[1:] == (num_kv_heads, page_size, head_dim) and k_cache.is_contiguous() and v_cache.is_contiguous(),
+          "caches must be contiguous [pages, kv heads, page size, head_dim]")
     _need(block_tables.dim() == 2 and block_tables.shape[0] >= rows and row_q_start.numel() >= rows and row_ctx_len.numel() >= rows,
           "block_tables, row_q_start and row_ctx_len need an entry for every row")
     _need(group_start.numel() == groups + 1, "group_start has one entry more than group_prefix")
-    _need(q_stride % 8 == 0 and q.data_ptr() % 16 == 0 and k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0, "rows of q and the caches must begin on 16 bytes")
-    _need(out.is_contiguous() and out.data_ptr() % 16 == 0, "the output must be contiguous [tokens, heads, head_dim], 16-byte aligned")
-    _need(k_cache.shape[0] * num_kv_heads * page_size < 1 << 31, "caches of 2^31 key rows and more are not taken")
+    at_q, at_k, at_v, at_out = _at(q), _at(k_cache), _at(v_cache), _at(out)
+    _need(q_stride % 8 == 0 and (at_q | at_k | at_v) % 16 == 0, "rows of q and the caches must begin on 16 bytes")
+    _need(out.is_contiguous() and at_out % 16 == 0, "the output must be contiguous [tokens, heads, head_dim], 16-byte aligned")
+    _need(shape[0] * num_kv_heads * page_size < 1 << 31, "caches of 2^31 key rows and more are not taken")
     _need(scale > 0, "the scale of the scores must be positive")
-    _need(q.device.index == torch.cuda.current_device() if q.is_cuda else True, "the tensors must be on the current device")
+    device = q.device.index
+    _need(device == torch.cuda.current_device(), "the tensors must be on the current device")
     if rows == 0:
         return out
-    covered = block_tables.shape[1] * page_size
-    max_own = covered if max_own is None else max(1, min(max_own, covered))
-    chunks = -(-(num_heads // num_kv_heads) // 16)
-    units = num_kv_heads * chunks
-    tma_ok = head_dim in (64, 128) and page_size >= 8
-    splits, part_tiles = own_keys_plan(rows, units, max_own, tma_ok, head_dim)
-    blocks = rows * units * splits
-    tma = tma_ok and decode_uses_tma(blocks, head_dim)
-    stages = decode_stages(blocks, max_own, splits, tma, head_dim, clustered=False)
-    part_o = part_lse = counters = None
-    if splits > 1:
-        part_o = _workspace(q.device, "decode_part_o", rows * num_heads * splits * head_dim, torch.float32)
-        part_lse = _workspace(q.device, "decode_part_lse", rows * num_heads * splits, torch.float32)
-        counters = _workspace(q.device, "decode_counters", rows * units, torch.int32)
-    shared = groups > 0 and max_prefix != 0
-    layout, slots = _prefix_layout(rows, num_heads, num_kv_heads, head_dim, page_size, num_sms(q.device))
-    pre_o = pre_lse = pre_chunk = None
-    if shared:
-        pre_o = _workspace(q.device, "prefix_o", slots * num_heads * head_dim, torch.float32)
-        pre_lse = _workspace(q.device, "prefix_lse", slots * num_heads, torch.float32)
-        pre_chunk = _workspace(q.device, "prefix_chunk", 1, torch.int32)
-        _check(load("attention_prefix").mie_prefix_attention(
-            _ptr(q), ctypes.c_int64(q_stride), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(row_q_start), _ptr(row_q_len),
-            rows, _ptr(group_start), _ptr(group_prefix), groups, num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale), layout, _ptr(pre_o),
-            _ptr(pre_lse), _ptr(pre_chunk), ctypes.c_longlong(slots), ctypes.c_longlong(k_cache.shape[0]), _stream()), "shared_prefix_attention (prefixes)")
-    _check(load("attention_decode_shared").mie_decode_attention_shared(
-        _ptr(q), ctypes.c_int64(q_stride), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(row_q_start), _ptr(row_q_len),
-        _ptr(row_ctx_len), rows, _ptr(group_start), _ptr(group_prefix), groups if shared else 0, layout, _ptr(pre_o), _ptr(pre_lse),
-        _ptr(pre_chunk), ctypes.c_longlong(slots), _ptr(out), num_heads, num_kv_heads, head_dim, page_size, ctypes.c_float(scale), int(splits), _ptr(part_o),
-        _ptr(part_lse), _ptr(counters), int(stages), ctypes.c_int64(k_cache.shape[0] if tma else 0), ctypes.c_int64(k_cache.shape[0]), int(part_tiles),
-        int(out.dtype == torch.float32), _stream()), "shared_prefix_attention (own keys)")
+    width = block_tables.shape[1]
+    max_own = width * page_size if max_own is None else max(1, min(max_own, width * page_size))
+    if groups == 0 or max_prefix == 0:                        # nothing is shared
+        return decode_attention(q, q_stride, k_cache, v_cache, block_tables, row_q_start, row_q_len, row_ctx_len, out, num_heads, num_kv_heads, head_dim,
+                                page_size, scale, max_ctx=max_own)
+    # (own keys are planned for in powers of two: a plan serves many steps)
+    plan, walk, _ = _shared_plan(device, rows, groups, num_heads, num_kv_heads, head_dim, page_size, 1 << (max_own - 1).bit_length(), shape[0])
+    a = _SharedArgs.from_buffer_copy(plan)
+    a.q, a.k_cache, a.v_cache, a.out = at_q, at_k, at_v, at_out
+    a.block_tables, a.row_q_start, a.row_q_len, a.row_ctx_len = _at(block_tables), _at(row_q_start), _at(row_q_len), _at(row_ctx_len)
+    a.group_start, a.group_prefix = _at(group_start), _at(group_prefix)
+    a.q_stride, a.table_stride, a.scale, a.out_f32 = q_stride, width, scale, out.dtype == torch.float32
+    first, second = _shared_libs()
+    at = ctypes.addressof(a)
+    _check(first.mie_prefix_attention(at, _stream()), "shared_prefix_attention (walk)" if walk else "shared_prefix_attention (prefixes)")
+    if not walk:
+        _check(second.mie_decode_attention_shared(at, _stream()), "shared_prefix_attention (own keys)")
     return out
 
 
@@ -854,6 +888,21 @@ def gemm_simt(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: torch.T
 
 
 # --------------------------------------------------------------------------- sampling
+
+class _RuleArgs(ctypes.Structure):          # csrc/logit_rules.cu: RuleArgs
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("history", "slot", "prompt_len", "total_len", "repetition", "presence", "frequency", "bias_tokens", "bias_values",
+                                                "bias_len", "mask", "mask_row")]
+                + [(n, ctypes.c_longlong) for n in ("history_stride", "mask_stride")] + [(n, ctypes.c_int) for n in ("slots", "width", "bias_width", "masks")])
+
+
+@functools.lru_cache(maxsize=None)
+def _rules_lib():
+    lib = load("logit_rules")
+    P, L, I = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+    lib.mie_apply_logit_rules.argtypes = [P, P, L, P, L, I, I, P]
+    lib.mie_sample_rules.argtypes = [P, P, L, P, P, P, ctypes.c_uint64, P, P, I, I, I, P, P, I, P]
+    return lib
+
 
 class LogitRules:
     """What holds for the logits of a step's rows beside the model: penalties for tokens that a row's text holds already, biases on single tokens,
@@ -902,9 +951,11 @@ class LogitRules:
         width = history.shape[1] if history is not None else 0
         self.history, self.words = history, mask.shape[1] if mask is not None else None
         self._kept = (slot, prompt_len, total_len, repetition, presence, frequency, bias_tokens, bias_values, bias_len, mask, mask_row)
-        self._args = (_ptr(history), ctypes.c_int64(width), slots, width, _ptr(slot), _ptr(prompt_len), _ptr(total_len), _ptr(repetition), _ptr(presence),
-                      _ptr(frequency), _ptr(bias_tokens), _ptr(bias_values), bias_tokens.shape[1] if bias_tokens is not None else 0, _ptr(bias_len),
-                      _ptr(mask), ctypes.c_int64(self.words or 0), mask.shape[0] if mask is not None else 0, _ptr(mask_row))
+        given = dict(history=history, slot=slot, prompt_len=prompt_len, total_len=total_len, repetition=repetition, presence=presence, frequency=frequency,
+                     bias_tokens=bias_tokens, bias_values=bias_values, bias_len=bias_len, mask=mask, mask_row=mask_row)
+        self._args = _RuleArgs(**{n: _ptr(t) for n, t in given.items()}, history_stride=width, mask_stride=self.words or 0, slots=slots, width=width,
+                               bias_width=bias_tokens.shape[1] if bias_tokens is not None else 0, masks=mask.shape[0] if mask is not None else 0)
+        self._address = ctypes.addressof(self._args)
 
     def args(self, logits: torch.Tensor):
         """The kernel arguments of these rules for ``logits`` [rows, vocab] (entries of a row side by side, rows any distance apart)."""
@@ -912,7 +963,7 @@ class LogitRules:
         _need(logits.shape[0] == self.rows, f"rules of {self.rows} rows, logits of {logits.shape[0]}")
         _need(logits.device == self.device and self.device.index == torch.cuda.current_device(), "logits and rules must be on the current device")
         _need(self.words is None or self.words * 32 >= logits.shape[1], "a mask has a bit for every entry of the vocabulary")
-        return self._args
+        return self._address
 
 
 def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor) -> torch.Tensor:
@@ -924,8 +975,8 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     _need(rows <= 1 or out.stride(0) >= vocab, "the output's rows must not overlap")
     if rows == 0 or vocab == 0:
         return out
-    _check(load("logit_rules").mie_apply_logit_rules(*args, _ptr(logits), ctypes.c_int64(logits.stride(0)), _ptr(out), ctypes.c_int64(out.stride(0)),
-                                                     rows, vocab, _stream()), "apply_logit_rules")
+    _check(_rules_lib().mie_apply_logit_rules(args, logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, _stream()),
+           "apply_logit_rules")
     return out
 
 
@@ -971,13 +1022,13 @@ def sample(logits: torch.Tensor, temperature, request, position, seed: int, out:
     _need(logprob is None or logprob.dtype == torch.float32, "logprob must be float32")
     _need(not append or (rules is not None and rules.history is not None), "append goes with rules that have a history")
     _ptr(logits)                                               # (refuses what is not on a CUDA device)
-    _check(load("logit_rules").mie_sample_rules(*args, _ptr(logits), ctypes.c_int64(logits.stride(0)), _ptr(temperature), _ptr(request), _ptr(position),
-                                                ctypes.c_uint64(seed & ((1 << 64) - 1)), _ptr(out), _ptr(logprob), _ptr(rules.history) if append else ctypes.c_void_p(0),
-                                                rows, vocab, host_ptr, turn_ptr, stride, _stream()), "sample with rules")
+    _check(_rules_lib().mie_sample_rules(args, logits.data_ptr(), logits.stride(0), _at(temperature), _at(request), _at(position), seed & ((1 << 64) - 1), _at(out),
+                                         _at(logprob), int(append), rows, vocab, host_ptr, turn_ptr, stride, _stream()), "sample with rules")
     return out
 
 
-_NO_RULES = (None, ctypes.c_int64(0), 0, 0, None, None, None, None, None, None, None, None, 0, None, None, ctypes.c_int64(0), 0, None)
+_no_rules = _RuleArgs()
+_NO_RULES = ctypes.addressof(_no_rules)
 
 
 # --------------------------------------------------------------------------- post-norm stream, grouped statistics
