@@ -229,6 +229,8 @@ static int launch_prefix(const PrefixParams& p, long long items, cudaStream_t st
 #define PT_THREADS 384
 #define PT_ROWS 128
 #define PT_KEYS 128
+#define PT_COST_START 7            // what starting and ending an item costs, in steps (3: 131 us for 256 rows behind 16,384 keys instead of 124)
+#define PT_WALK_PAIRS 128          // pairs on a key head up to which the kernel for any head size takes over: see mie_prefix_layout
 #define PT_MOST_TILES 512          // tiles of rows that a launch can plan for ...
 #define PT_MOST_SEGMENTS 63        // ... and groups with the rows between them
 
@@ -316,7 +318,7 @@ __device__ __forceinline__ void walk_plan(WalkPlan& w, const WalkParams& q, int 
             unsigned items = 0;
             for (int t = 0; t < tiles; ++t) items += p.units * prefix_splits(w.steps[t], c);
             if (s == 1 || items <= 2u * p.places) {
-                const unsigned long long cost = (unsigned long long)((items + p.places - 1) / p.places) * (c + PREFIX_COST_START);
+                const unsigned long long cost = (unsigned long long)((items + p.places - 1) / p.places) * (c + PT_COST_START);
                 atomicMin(&w.best, cost << 32 | (0xffffffffu - (unsigned)c));
             }
         }
@@ -943,7 +945,9 @@ extern "C" int mie_prefix_layout(SharedArgs* a, int sms) {
     if (a->num_rows < 0 || a->num_kv_heads <= 0 || a->num_heads <= 0 || a->num_heads % a->num_kv_heads || a->head_dim < 16 || a->head_dim > 128 || a->head_dim % 16
         || sms <= 0 || a->page_size < 1 || (a->page_size & (a->page_size - 1))) return MIE_ERR_BAD_ARG;
     const int G = a->num_heads / a->num_kv_heads;
-    for (a->walk = 1; a->walk >= 0; --a->walk) {
+    // Few pairs leave the walk's tiles of 128 empty, and it takes longer to begin.  Us, walk : the other two kernels -- 32 heads of 64 on 4, 2 rows behind 208 keys 11.2 : 9.8, 8
+    // behind 2,048 14.8 : 13.0, 16 16.0 : 14.0, 32 19.6 : 30.1; 32 of 128 on 8, 16 rows behind 4,000 25.3 : 21.4, 64 behind 8,000 53 : 84; 32 of 128 on 32, 33 rows in five groups 91 : 74.
+    for (a->walk = a->num_rows * (long long)G > PT_WALK_PAIRS; a->walk >= 0; --a->walk) {
         const int pairs = a->walk ? PT_ROWS : PFX_PAIRS;
         a->chunks = (G + pairs - 1) / pairs;
         a->chunk_heads = (G + a->chunks - 1) / a->chunks;
