@@ -338,3 +338,18 @@ def test_no_rows(ops):
     rules = ops.LogitRules(mask=torch.zeros(1, 2, dtype=torch.int32, device=DEV), mask_row=torch.empty(0, dtype=torch.int32, device=DEV))
     x = torch.empty(0, 40, device=DEV)
     assert ops.apply_logit_rules(x, rules, torch.empty_like(x)).shape == (0, 40)
+
+
+@pytest.mark.parametrize("rows,vocab,width", [(3, 1000, 6000), (9, 50001, 9000), (2, 70001, 17000)])
+def test_the_same_call_gives_the_same_bits(ops, rows, vocab, width):
+    """Texts that name the same tokens again and again: whichever thread comes to one first, the sums are the same."""
+    s = Step(ops, rows, vocab, width=width, seed=vocab)
+    s.total = [width - r for r in range(rows)]
+    s.rep, s.pres = [1.3] * rows, [0.7] * rows
+    s.build()
+    logits, first = s.logits.to(DEV), None
+    for _ in range(30):
+        tokens, lp = s.choose(logits, temperature=0.8)
+        now = (tokens.tolist(), lp.view(torch.int32).tolist())
+        first = first or now
+        assert now == first

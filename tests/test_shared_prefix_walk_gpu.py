@@ -1,0 +1,219 @@
+"""Decode attention of rows that share a prefix, where prefix and own keys are one walk on the tensor cores (heads of 64 and 128, more than 128 pairs of a
+row and a query head on a key head), against attention of every row over its whole sequence in 64 bits."""
+import pytest
+import torch
+
+from test_shared_prefix_gpu import DEV, Case, ops  # noqa: F401  (the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def walks(ops, c, **hints):
+    """The case, run by the walk: its plan says so."""
+    return ops._shared_plan(torch.cuda.current_device(), c.rows, c.group_prefix.numel(), c.H, c.G, c.D, c.page, hints.get("max_own", 1), c.cache.shape[1])[1]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [8, 16, 32, 128, 256])
+def test_pages(ops, D, page):
+    c = Case([(5, 200), (1, 70), (4, 131)], 90, 32, 2, D, page, seed=D + page)
+    assert walks(ops, c, **c.hints)
+    out = c.run(ops, **c.hints)
+    c.check(out)
+    assert torch.equal(out, c.run(ops, **c.hints))            # run to run: the same bits
+
+
+@pytest.mark.parametrize("H,G,rows", [(16, 16, 129), (17, 1, 8), (96, 2, 3), (136, 1, 2), (300, 1, 5), (40, 8, 27), (12, 4, 44)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_head_shapes(ops, H, G, rows, D):
+    c = Case([(rows - 1, 150), (1, 20)], 40, H, G, D, 16, seed=H + D)
+    assert walks(ops, c, **c.hints)
+    c.check(c.run(ops, **c.hints))
+
+
+@pytest.mark.parametrize("groups,own", [
+    ([(9, 1)], 1), ([(9, 127)], 1), ([(9, 128)], 1), ([(9, 129)], 3), ([(9, 255)], 128), ([(9, 256)], 129), ([(10, 0)], 200),
+    ([(2, 0), (9, 100), (2, 0)], 40), ([(0, 90), (9, 90), (0, 0), (1, 33), (0, 4)], 10),
+    ([(1, 100)] * 12, 60),                                    # groups of one row
+    ([(40, 777)], 20), ([(20, 300), (1, 5), (30, 129)], 150), # more pairs than a tile holds
+    ([(9, 5000)], [1, 700, 64, 1, 129, 128, 127, 2, 333]),    # a long prefix, unequal rests
+    ([(3, 3000), (2, 10), (2, 900), (2, 1), (2, 2000)], 500)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_groups(ops, groups, own, D):
+    c = Case(groups, own, 32, 2, D, 16, seed=len(groups) + D)
+    assert walks(ops, c, **c.hints)
+    out = c.run(ops, **c.hints)
+    c.check(out)
+    c.check(c.run(ops))                                       # without the hints: planned for the table's width
+    assert torch.equal(out, c.run(ops, **c.hints))
+
+
+@pytest.mark.parametrize("count", [30, 61, 64, 80])
+def test_many_groups(ops, count):
+    """More groups than the walk plans for: the kernel for any head size takes over, with the same results."""
+    c = Case([(1 + i % 2, 10 + 7 * (i % 5)) for i in range(count)], 20, 32, 2, 64, 16, seed=count)
+    c.check(c.run(ops, **c.hints))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_of_no_group_and_rows_without_own_keys(ops, D):
+    c = Case([(6, 150), (4, 96)], [0, 4, 0, 0, 1, 9, 0, 0, 0, 128, 60, 1, 300], 32, 2, D, 16, uncovered=3, seed=D)
+    assert walks(ops, c, **c.hints)
+    c.check(c.run(ops, **c.hints))
+
+
+@pytest.mark.parametrize("loud", [0, 77, 1023, 1024, 1030])
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_key_that_every_row_hears(ops, loud, D):
+    c = Case([(9, 1024)], [7, 8, 9, 10, 20, 30, 40, 100, 300], 32, 2, D, 16, loud=loud)
+    assert walks(ops, c, **c.hints)
+    out = c.run(ops, **c.hints)
+    c.check(out)
+    assert (out.float() - 5.0).abs().max() < 0.05
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_float32_output(ops, D):
+    c = Case([(8, 700), (2, 0)], 100, 32, 2, D, 16)
+    assert walks(ops, c, **c.hints)
+    c.check(c.run(ops, dtype=torch.float32, **c.hints))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_with_more_tokens_are_left_alone(ops, D):
+    """A row of several tokens, or of none, inside a group and outside: its output stays, and its neighbours do not see it."""
+    c = Case([(8, 300), (3, 40)], 50, 32, 2, D, 16, uncovered=2)
+    assert walks(ops, c, **c.hints)
+    for row, n in ((1, 3), (5, 0), (8, 2), (11, 0)):
+        c.q_len[row] = n
+    out = c.run(ops, **c.hints)
+    c.check(out, [0, 2, 3, 4, 6, 7, 9, 10, 12])
+    for row in (1, 5, 8, 11):
+        assert (out[row] == 77.0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_bad_page_is_reported(ops, D):
+    """In a prefix: the other group is as it should be.  In own keys: the other rows are."""
+    for row, entry, sound in ((0, 2, range(6, 10)), (3, 8, [0, 1, 2, 4, 5, 6, 7, 8, 9])):
+        c = Case([(6, 100), (4, 20)], [40] * 10, 32, 2, D, 16)
+        assert walks(ops, c, **c.hints)
+        c.tables[row, entry] = 10 ** 6
+        out = c.run(ops, **c.hints)
+        torch.cuda.synchronize()
+        got = ops.range_report().tolist()
+        assert got[0] == 4 and got[3] == 10 ** 6
+        with pytest.raises(ops.KernelError, match="page"):
+            ops.check_range_errors()
+        c.check(out, sound)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_context_inside_its_prefix_is_reported(ops, D):
+    c = Case([(6, 100), (4, 20)], 30, 32, 2, D, 16)
+    assert walks(ops, c, **c.hints)
+    c.ctx_len[1] = 60
+    out = c.run(ops, **c.hints)
+    torch.cuda.synchronize()
+    assert ops.range_report().tolist()[:1] == [2]
+    with pytest.raises(ops.KernelError, match="position"):
+        ops.check_range_errors()
+    c.check(out, [0, 2, 3, 4, 5, 6, 7, 8, 9])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+def test_what_is_no_number_stays_in_its_row(ops, D, what):
+    """A value, a key and a query of one row's own, and a value of one group's prefix."""
+    H, G = 32, 2
+
+    def spoiled(row, prefix, cache, at):
+        c = Case([(7, 130), (3, 90)], [30] * 10, H, G, D, 16, seed=D)
+        assert walks(ops, c, **c.hints)
+        key = 53 if prefix else c.ctx[row] - 9
+        pg = int(c.tables[0 if prefix and row < 7 else row, key // 16])
+        c.cache[cache, pg, 1, key % 16, at] = what
+        return c, c.run(ops, **c.hints)
+
+    c, out = spoiled(2, False, 1, 7)                          # an own value: one number of every head on that key head
+    assert not torch.isfinite(out[2, H // G:, 7]).any()
+    out[2, H // G:, 7] = 0
+    assert torch.isfinite(out).all()
+    c.check(out, [0, 1, 3, 4, 5, 6, 7, 8, 9])
+    c, out = spoiled(4, True, 1, 7)                           # a prefix's value
+    assert not torch.isfinite(out[:7, H // G:, 7]).any()
+    out[:7, H // G:, 7] = 0
+    assert torch.isfinite(out).all()
+    c.check(out, [7, 8, 9])
+    c, out = spoiled(5, False, 0, 3)                          # an own key
+    assert torch.isfinite(out[:, :H // G]).all()
+    c.check(out, [0, 1, 2, 3, 4, 6, 7, 8, 9])
+    c = Case([(7, 130), (3, 90)], [30] * 10, H, G, D, 16, seed=D)
+    c.qkv[6, 5] = what                                        # a query: one head
+    out = c.run(ops, **c.hints)
+    c.check(out, [0, 1, 2, 3, 4, 5, 7, 8, 9])
+    assert torch.isfinite(out[6, 1:]).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_captured_step_follows_its_groups(ops, D):
+    """One captured call, replayed for other groups, prefixes and lengths; between the replays another call uses the same workspaces."""
+    cases = [Case([(9, 400), (3, 0)], 30, 32, 2, D, 16, seed=1), Case([(2, 90), (10, 250)], 60, 32, 2, D, 16, seed=2), Case([(1, 1), (11, 512)], [1] * 12, 32, 2, D, 16, seed=3)]
+    pages, width = max(c.cache.shape[1] for c in cases), max(c.tables.shape[1] for c in cases)
+    s = Case([(9, 400), (3, 0)], 30, 32, 2, D, 16, seed=1)
+    s.cache, s.tables = torch.zeros(2, pages, 2, 16, D, dtype=torch.bfloat16, device=DEV), torch.zeros(12, width, dtype=torch.int32, device=DEV)
+
+    def fill(c):
+        s.cache.zero_()
+        s.cache[:, :c.cache.shape[1]].copy_(c.cache)
+        s.tables.zero_()
+        s.tables[:, :c.tables.shape[1]].copy_(c.tables)
+        for name in ("qkv", "q_start", "q_len", "ctx_len", "group_start", "group_prefix"):
+            getattr(s, name).copy_(getattr(c, name))
+
+    out = torch.empty(12, 32, D, dtype=torch.bfloat16, device=DEV)
+    hints = dict(max_prefix=512, max_own=128)
+    assert walks(ops, s, **hints)
+    fill(cases[0])
+    s.run(ops, out=out, **hints)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        s.run(ops, out=out, **hints)
+    other = Case([(30, 700)], 100, 32, 2, D, 16, seed=9)
+    for c in (cases[1], cases[0], cases[2], cases[1]):
+        fill(c)
+        out.zero_()
+        graph.replay()
+        other_out = other.run(ops, **other.hints)
+        torch.cuda.synchronize()
+        c.check(out)
+        other.check(other_out)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_cache_whose_offsets_pass_32_bits(ops, D):
+    c = Case([(9, 100)], 40, 32, 2, D, 16, extra_pages=2)
+    assert walks(ops, c, **c.hints)
+    pages = (1 << 31) // (2 * 16 * D) + 64                    # elements before the last pages: more than 2^31
+    big = torch.empty(2, pages, 2, 16, D, dtype=torch.bfloat16, device=DEV)
+    n = c.cache.shape[1]
+    big[:, pages - n:] = c.cache
+    big[:, 0] = 0
+    c.cache, c.tables = big, c.tables + (pages - n)
+    c.check(c.run(ops, **c.hints))
+
+
+def test_rows_spread_over_the_packed_tokens(ops):
+    """The rows' tokens lie anywhere, in any order, with others between them: what is no row's token keeps its output."""
+    c = Case([(9, 200), (1, 30)], 50, 32, 2, 64, 16, seed=7)
+    at = [17, 3, 8, 0, 21, 5, 11, 14, 2, 9]
+    qkv = torch.full((24, c.qkv.shape[1]), float("nan"), dtype=torch.bfloat16, device=DEV)
+    qkv[at] = c.qkv
+    c.qkv, c.q_start = qkv, torch.tensor(at, dtype=torch.int32, device=DEV)
+    out = torch.full((24, c.H, c.D), 77.0, dtype=torch.bfloat16, device=DEV)
+    c.run(ops, out=out, **c.hints)
+    c.check(out[at])
+    out[at] = 77.0
+    assert (out == 77.0).all()
