@@ -111,7 +111,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     const int kvh = blockIdx.y / p.chunks, chunk = blockIdx.y - kvh * p.chunks;
     const int g0 = chunk * 16, gn = min(16, G - g0);               // query heads of this block within the group
     const int split = blockIdx.x;
-    const int ctx = p.row_ctx_len[row];
+    const int ctx = SHARED ? max(0, min(p.row_ctx_len[row], p.groups.most_keys)) : p.row_ctx_len[row];
     const int token = p.row_q_start[row];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int quad = lane >> 2, tq = lane & 3;
@@ -123,9 +123,9 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
             const PrefixPart t = prefix_group(p.groups, g);
             if (row >= t.first_row && row < t.first_row + t.rows) { prefix = t.keys; break; }
         }
-        if (prefix > ctx) {                                        // a context that ends inside its prefix
-            if (threadIdx.x == 0 && split == 0 && blockIdx.y == 0) range_report(p.report, MIE_RANGE_POSITION, MIE_K_ATTENTION_DECODE, row, prefix);
-            prefix = ctx;
+        if (prefix > ctx || ctx != p.row_ctx_len[row]) {           // a context that ends inside its prefix, or beyond its block table
+            if (threadIdx.x == 0 && split == 0 && blockIdx.y == 0) range_report(p.report, MIE_RANGE_POSITION, MIE_K_ATTENTION_DECODE, row, p.row_ctx_len[row]);
+            prefix = min(prefix, ctx);
         }
     }
     // this block's part of the context: the range [lo, ctx) cut into `splits` parts of whole tiles

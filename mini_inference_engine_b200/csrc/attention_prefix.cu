@@ -20,7 +20,7 @@ struct PrefixParams {
     const bf16* q; int64_t q_stride;
     const bf16* k_cache; const bf16* v_cache;
     const int* block_tables; int table_stride;
-    const int* row_q_start; const int* row_q_len;
+    const int* row_q_start; const int* row_q_len; const int* row_ctx_len;
     PrefixGroups groups;
     float* part_o; float* part_lse; int64_t most_slots; int* chunk;       // chunk: how the prefixes are cut, for the kernel behind
     int num_heads, num_kv_heads, page_size, page_shift, chunks, chunk_heads;       // a unit: up to chunk_heads query heads of a key head, `chunks` units each
@@ -34,6 +34,16 @@ __device__ __forceinline__ float exp2_fast(float x) {      // two units in the l
     return y;
 }
 
+// Does a row's step write a key of its prefix (its newest key is the prefix's last, say)?
+__device__ __forceinline__ bool writes_prefix(int len, int ctx, int keys) { return len > 0 && ctx - len < keys; }
+__device__ __forceinline__ bool writes_prefix(const PrefixParams& p, int row, int keys) { return writes_prefix(p.row_q_len[row], p.row_ctx_len[row], keys); }
+// Reports a group whose rows are none of the step's, or go back, and a prefix that is negative or longer than a block table.
+__device__ __forceinline__ void check_group(const PrefixGroups& p, int g, int* report) {
+    const int a = p.start[g], b = p.start[g + 1], keys = p.prefix[g];
+    if (a < 0 || a > b || b > p.num_rows) range_report(report, MIE_RANGE_ROW, MIE_K_ATTENTION_PREFIX, g, a < 0 || a > b ? a : b);
+    else if (b > a && (keys < 0 || keys > p.most_keys)) range_report(report, MIE_RANGE_POSITION, MIE_K_ATTENTION_PREFIX, a, keys);
+}
+
 template <int D>
 __global__ void __launch_bounds__(PFX_WARPS * 32)
 prefix_attention_kernel(const PrefixParams p) {
@@ -45,6 +55,8 @@ prefix_attention_kernel(const PrefixParams p) {
     __shared__ int s_chunk;
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, tq = lane & 3;
+    if (blockIdx.x == 0 && warp == 1)
+        for (int g = lane; g < p.groups.groups; g += 32) check_group(p.groups, g, p.report);
     if (warp == 0) {
         const int chunk = prefix_chunk(p.groups);
         const PrefixPart t = prefix_find(p.groups, chunk, (int)blockIdx.x, false);
@@ -88,7 +100,12 @@ prefix_attention_kernel(const PrefixParams p) {
             }
         }
     };
-    load_tile(0, 0);                                       // the prefix is older than the step: before the wait
+    // The prefix is older than the step, so that its first tile is asked for before the wait -- unless a row of the group writes a key of it in this step.
+    bool young = false;
+    for (int r = t.first_row + threadIdx.x; r < t.first_row + t.rows; r += PFX_WARPS * 32) young |= writes_prefix(p, r, t.keys);
+    young = __syncthreads_or(young);
+    if (young) pdl_wait();
+    load_tile(0, 0);
     cp_async_commit();
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = s_chunk;
@@ -236,7 +253,7 @@ static int launch_prefix(const PrefixParams& p, long long items, cudaStream_t st
 
 struct WalkParams {
     PrefixParams b;
-    const int* row_ctx_len; int2* row_info; int* marks;    // row_info: a row's first slot and its ranges; marks: 0, or the query heads of a (row, key head) with values that are not finite
+    int2* row_info; int* marks;                            // row_info: a row's first slot and its ranges; marks: 0, or the query heads of a (row, key head) with values that are not finite
 };
 
 template <int D> constexpr int PT_STAGES = D == 64 ? 4 : 2;
@@ -249,6 +266,7 @@ struct WalkPlan {
     int slots[2 * PT_MOST_TILES];                          // own slots of a tile of pairs
     int steps[PT_MOST_TILES], seg[PT_MOST_TILES];          // steps of a tile of rows' walk; its segment
     unsigned long long best;
+    int young;                                             // some row's step writes a key of its prefix
     int found, splits, item0, slot0;                       // the item's tile of rows (-1: none), its ranges, first item and slot
     int own_first[2 * PT_ROWS + 1], ctx[2 * PT_ROWS];      // of the tile's rows: first own slot; context (0: not a row of one new token)
 };
@@ -271,9 +289,10 @@ __device__ __forceinline__ void walk_plan(WalkPlan& w, const WalkParams& q, int 
         w.rows[tid] = max(0, b - a);
         w.keys[tid] = tid >= 1 && tid <= p.groups ? max(0, min(p.prefix[tid - 1], p.most_keys)) : 0;
     }
-    if (tid == 0) { w.segments = p.groups + 2; w.best = ~0ull; w.found = -1; }
+    if (item == 0 && tid < p.groups) check_group(p, tid, q.b.report);
+    if (tid == 0) { w.segments = p.groups + 2; w.best = ~0ull; w.found = -1; w.young = 0; }
     // this thread's first row (the others are asked for where there are more rows than threads)
-    const int r_len = tid < p.num_rows ? q.b.row_q_len[tid] : 0, r_ctx = tid < p.num_rows ? q.row_ctx_len[tid] : 0;
+    const int r_len = tid < p.num_rows ? q.b.row_q_len[tid] : 0, r_ctx = tid < p.num_rows ? q.b.row_ctx_len[tid] : 0;
     __syncthreads();
     if (warp == 0) {                                       // first tiles of the segments
         int at = 0;
@@ -298,7 +317,8 @@ __device__ __forceinline__ void walk_plan(WalkPlan& w, const WalkParams& q, int 
         int g = 0;
         while (g + 1 < w.segments && !(r >= w.first[g] && r < w.first[g] + w.rows[g])) ++g;
         const int in_seg = r - w.first[g], t = w.tile0[g] + in_seg / p.tile_rows;
-        const int len = r == tid ? r_len : q.b.row_q_len[r], ctx = r == tid ? r_ctx : q.row_ctx_len[r];
+        const int len = r == tid ? r_len : q.b.row_q_len[r], ctx = r == tid ? r_ctx : q.b.row_ctx_len[r];
+        if (in_seg >= 0 && writes_prefix(len, ctx, w.keys[g])) w.young = 1;
         if (in_seg >= 0 && t < tiles && len == 1) atomicAdd(&w.slots[2 * t + (in_seg % p.tile_rows) / half], own_slots(min(ctx, p.most_keys), w.keys[g], ss));
     }
     __syncthreads();
@@ -393,7 +413,7 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int i0 = 0; i0 < rows; i0 += 32) {
             const int i = i0 + lane, r = row0 + i;
             const bool on = i < rows && p.row_q_len[r] == 1;
-            const int all = on ? wp.row_ctx_len[r] : 0, ctx = min(all, p.groups.most_keys);
+            const int all = on ? p.row_ctx_len[r] : 0, ctx = min(all, p.groups.most_keys);
             if (on && unit == 0 && split == 0 && (all < prefix || all > p.groups.most_keys))         // a context that ends inside its prefix, or beyond its block table
                 range_report(p.report, MIE_RANGE_POSITION, MIE_K_ATTENTION_PREFIX, r, all);
             const int n = own_slots(ctx, prefix, ss);
@@ -490,7 +510,7 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     uint64_t* empty = warp == 0 ? k_empty : v_empty;
     const CUtensorMap* map = warp == 0 ? &map_k : &map_v;
     auto to = [&](int st) { return warp == 0 ? k_off(st) : v_off(st); };
-    const int ahead = min(STAGES, J), early = min(ahead, npre);      // the prefix is older than the step: its first keys are on their way before the wait
+    const int ahead = min(STAGES, J), early = plan.young ? 0 : min(ahead, npre);      // a prefix older than the step: its first keys are on their way before the wait
     Place later;                                           // of the step behind those that shared memory has places for
     if (fetches) {
         Place at[STAGES];
@@ -824,7 +844,7 @@ prefix_join_kernel(const WalkParams wp, bf16* __restrict__ out, float* __restric
     const int row = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
     const int2 info = __ldcg(wp.row_info + row);
     const int S = min(info.y, 2 * PREFIX_MAX_SPLITS);
-    if (p.row_q_len[row] != 1 || wp.row_ctx_len[row] <= 0 || head >= p.num_heads) return;      // (a row of more than one new token is left alone)
+    if (p.row_q_len[row] != 1 || p.row_ctx_len[row] <= 0 || head >= p.num_heads) return;      // (a row of more than one new token is left alone)
     if (S <= 0 || (int64_t)info.x + S > p.most_slots) return;
     const int kvh = head / (p.num_heads / p.num_kv_heads);
     int* mark = wp.marks + (int64_t)row * p.num_kv_heads + kvh;
@@ -885,7 +905,7 @@ prefix_join_kernel(const WalkParams wp, bf16* __restrict__ out, float* __restric
             const PrefixPart t = prefix_group(p.groups, g);
             if (row >= t.first_row && row < t.first_row + t.rows) { prefix = t.keys; break; }
         }
-        const int ctx = min(wp.row_ctx_len[row], p.groups.most_keys);
+        const int ctx = min(p.row_ctx_len[row], p.groups.most_keys);
         for (int key = prefix; key < ctx; ++key) {
             const int entry = key >> p.page_shift;
             const int page = checked_page(p.block_tables[(int64_t)row * p.table_stride + entry], p.num_pages, p.report, MIE_K_ATTENTION_PREFIX, entry);
@@ -975,7 +995,8 @@ extern "C" int mie_prefix_attention(const SharedArgs* a, cudaStream_t stream) {
     p.scale_log2e = a->scale * 1.4426950408889634f;
     p.num_pages = a->num_pages; p.report = g_range_report;
     p.groups = shared_groups_of(*a);
-    w.row_ctx_len = a->row_ctx_len; w.row_info = (int2*)a->row_info; w.marks = a->marks;
+    p.row_ctx_len = a->row_ctx_len;
+    w.row_info = (int2*)a->row_info; w.marks = a->marks;
     const long long items = prefix_most_items(a->num_rows, a->walk ? a->groups + 2 : a->groups, p.groups.units, p.groups.tile_rows, p.groups.places);
     if (items > 0x7fffffffll) return MIE_ERR_TOO_LARGE;
     if (a->walk) return a->head_dim == 64 ? launch_walk<64>(w, a->out, a->out_f32 != 0, items, stream) : launch_walk<128>(w, a->out, a->out_f32 != 0, items, stream);

@@ -217,3 +217,41 @@ def test_rows_spread_over_the_packed_tokens(ops):
     c.check(out[at])
     out[at] = 77.0
     assert (out == 77.0).all()
+
+
+@pytest.mark.parametrize("H,G,D,rows", [(32, 2, 64, 9), (32, 2, 128, 9), (8, 2, 64, 3), (8, 2, 96, 3)])
+def test_a_prefix_whose_last_key_the_step_writes(ops, H, G, D, rows):
+    """The launch in front writes the prefix's last key and value: the very next launch sees them, time after time."""
+    c = Case([(rows, 128)], [0] * (rows - 1) + [5], H, G, D, 16, seed=D)
+    page, cos, sin = int(c.tables[0, 7]), torch.ones(256, D // 2, device=DEV), torch.zeros(256, D // 2, device=DEV)
+    positions, slots = torch.tensor([127], dtype=torch.int32, device=DEV), torch.tensor([page * 16 + 15], dtype=torch.int32, device=DEV)
+    busy = torch.randn(2048, 2048, device=DEV)
+    g = torch.Generator().manual_seed(D)
+    for turn in range(8):
+        k, v = torch.randn(2, G, D, generator=g).to(torch.bfloat16)
+        k *= 4
+        for r in range(rows):
+            c.keys[r][127], c.values[r][127] = k, v
+        c.qkv[0, H * D:(H + 2 * G) * D] = torch.cat([k.reshape(-1), v.reshape(-1)]).to(DEV)
+        torch.cuda.synchronize()
+        busy @ busy
+        ops.rope_cache_write(c.qkv[:1], positions, slots, cos, sin, c.cache[0], c.cache[1], H, G, D, D, 16)
+        c.check(c.run(ops, **c.hints))
+
+
+@pytest.mark.parametrize("H,G,D", [(32, 2, 64), (32, 2, 128), (4, 2, 64), (4, 2, 80)])
+def test_groups_and_lengths_out_of_range_are_reported(ops, H, G, D):
+    """Groups that go back or reach beyond the rows, a prefix and a context longer than a block table: reported, and nothing outside is touched."""
+    for name, at, value in (("group_start", 1, 99), ("group_start", 2, 3), ("group_start", 0, -1), ("group_prefix", 0, -5), ("group_prefix", 1, 10 ** 6),
+                            ("ctx_len", 2, 10 ** 6), ("ctx_len", 7, 2 ** 31 - 1), ("ctx_len", 8, -4)):
+        c = Case([(6, 100), (4, 20)], 30, H, G, D, 16, seed=D)
+        c.tables = torch.where(c.tables == c.tables.max(), 0, c.tables)      # (entries nobody should follow: page 0)
+        getattr(c, name)[at] = value
+        c.run(ops, **c.hints)
+        torch.cuda.synchronize()
+        assert ops.range_report()[0].item() in (2, 5), (name, at)      # a position, or a row (whichever block comes first)
+        with pytest.raises(ops.KernelError):
+            ops.check_range_errors()
+        ops.range_report().zero_()
+        sound = Case([(6, 100), (4, 20)], 30, H, G, D, 16, seed=D)
+        sound.check(sound.run(ops, **sound.hints))            # the call after it is as it should be
