@@ -247,6 +247,9 @@ static int launch_prefix(const PrefixParams& p, long long items, cudaStream_t st
 #define PT_ROWS 128
 #define PT_KEYS 128
 #define PT_COST_START 7            // what starting and ending an item costs, in steps (3: 131 us for 256 rows behind 16,384 keys instead of 124)
+#ifndef TURNS
+#define TURNS 1
+#endif
 #define PT_WALK_PAIRS 128          // pairs on a key head up to which the kernel for any head size takes over: see mie_prefix_layout
 #define PT_MOST_TILES 512          // tiles of rows that a launch can plan for ...
 #define PT_MOST_SEGMENTS 63        // ... and groups with the rows between them
@@ -376,10 +379,11 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     constexpr int PARTS = D / 64, STAGES = PT_STAGES<D>;
     constexpr uint32_t SUB = 128 * 64 * 2;                 // one [128 x 64] part of a tile
     constexpr uint32_t TILE = PARTS * SUB;
-    constexpr bool OVER = D == 128;                        // P lies over S
-    constexpr uint32_t TMEM_S = 0, TMEM_P = OVER ? 0 : 256, TMEM_O = OVER ? 256 : 384, S_STEP = 128, P_STEP = OVER ? 128 : 64, O_STEP = D;
+    constexpr bool OVER = D == 128;                        // P lies over S, and a step goes in halves of 64 keys
+    constexpr int HALVES = OVER ? 2 : 1, HK = PT_KEYS / HALVES;
+    constexpr uint32_t TMEM_S = 0, TMEM_P = OVER ? 0 : 256, TMEM_O = OVER ? 256 : 384, S_STEP = 128, P_STEP = OVER ? 128 : 64, O_STEP = D, HALF = 64;
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(8) uint64_t q_full[2], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], s_free[2], p_full[2], pv_done[2], o_full[2], exp_done[2];
+    __shared__ __align__(8) uint64_t q_full[2], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2][HALVES], s_free[2], p_full[2][HALVES], pv_done[2], o_full[2], exp_done[2];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
     __shared__ WalkPlan plan;
@@ -428,10 +432,11 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     if (threadIdx.x == 32) {
         abort_flag = 0;
         for (int u = 0; u < 2; ++u) {
-            mbar_init(&q_full[u], 4); mbar_init(&s_full[u], 1); mbar_init(&s_free[u], 4); mbar_init(&p_full[u], 4);
+            for (int h = 0; h < HALVES; ++h) { mbar_init(&s_full[u][h], 1); mbar_init(&p_full[u][h], 4); }
+            mbar_init(&q_full[u], 4); mbar_init(&s_free[u], 4);
             mbar_init(&pv_done[u], 1); mbar_init(&o_full[u], 1); mbar_init(&exp_done[u], 4);
         }
-        for (int st = 0; st < STAGES; ++st) {              // (both issuing threads give a stage back, whether or not their chain used it)
+        for (int st = 0; st < STAGES; ++st) {              // (a stage is given back by both chains' products, or twice by those of the one that uses it)
             mbar_init(&k_full[st], 1); mbar_init(&v_full[st], 1); mbar_init(&k_empty[st], 2); mbar_init(&v_empty[st], 2);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -523,6 +528,30 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int j = 0; j < STAGES; ++j) if (j >= early && j < ahead) load(j, &full[j], map, to(j), row_of(at[j]));
         later = place_of(STAGES);
     }
+    // Softmax warps 2..5 (chain 0) and 6..9 (chain 1), a thread a pair: which, and its query, under the copies and the hand-out of tensor memory.  A query's 16-byte
+    // pieces go to neighbouring lanes (a lane its own query, behind the hand-out: 8,000 cycles a block).
+    const int u = warp >= 6 ? 1 : 0, q = warp & 3, r = q * 32 + lane;      // (the lanes of tensor memory that a warp reaches go by its number)
+    const int in_tile = (both ? u * half : 0) + r / heads, my_row = row0 + in_tile, head = kvh * G + h0 + r % heads;
+    const bool softmax = warp >= 2 && warp <= 9, pair = softmax && r / heads < half && in_tile < rows && plan.ctx[min(in_tile, rows - 1)] > 0;
+    if (softmax && (both || u == 0)) {
+        constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;             // lanes a query, queries an instruction
+        const int64_t mine = pair ? (int64_t)p.row_q_start[my_row] * p.q_stride + (int64_t)head * D : -1;
+        pdl_wait();
+        uint4 v[LANES];
+#pragma unroll
+        for (int i = 0; i < LANES; ++i) {
+            const int64_t src = __shfl_sync(0xffffffffu, mine, i * AT_ONCE + lane / LANES);
+            v[i] = src >= 0 ? *reinterpret_cast<const uint4*>(p.q + src + lane % LANES * 8) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < LANES; ++i) {
+            const int to_r = q * 32 + i * AT_ONCE + lane / LANES, c = lane % LANES;
+            *reinterpret_cast<uint4*>(tiles + q_off(u) + (c >> 3) * SUB + to_r * 128 + (((c & 7) ^ (to_r & 7)) << 4)) = v[i];
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[u]);
+    }
     // Tensor memory is taken behind the wait, and the next kernel let in behind that: a block that held it before the kernels in front are done could keep
     // it from a block of theirs, and one that came later from this one.
     pdl_wait();
@@ -558,8 +587,8 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             // ---- the warp that issues for chain mu: it walks its loop as a whole, so that what feeds the instructions stays uniform, and one lane issues
             const bool issuer = elect_one();               // (one lane alone in the loop: 740 cycles for the eight products of P V instead of 300)
             auto wait_for = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_p)) != 0; };
-            const uint32_t idesc_s = umma_idesc_bf16(PT_ROWS, PT_KEYS), idesc_o = umma_idesc_bf16(PT_ROWS, D) | (1u << 16);
-            constexpr int KS = D / 16, KV = PT_KEYS / 16;
+            const uint32_t idesc_s = umma_idesc_bf16(PT_ROWS, HK), idesc_o = umma_idesc_bf16(PT_ROWS, D) | (1u << 16);
+            constexpr int KS = D / 16, KV = HK / 16;
             const int qt = both ? mu : 0;
             uint64_t dq[KS];
 #pragma unroll
@@ -567,81 +596,70 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             const uint64_t dk0 = umma_desc_sw128(base + k_off(0)), dv0 = umma_desc_sw128_mn(base + v_off(0), SUB);
             constexpr uint64_t STAGE_STEP = (2 * TILE) >> 4;       // descriptors of another stage differ in the address field only
             const uint32_t s_at = tmem_base + TMEM_S + S_STEP * mu, p_at = tmem_base + TMEM_P + P_STEP * mu, o_at = tmem_base + TMEM_O + O_STEP * mu;
-            int last = J - 1;                              // the chain's last step (-1: it has none)
-            while (last >= 0 && !active(mu, last)) --last;
             bool ok = wait_for(&q_full[qt], 0);
-            auto scores = [&](int j) {                     // S of step j, once its keys are here
+            auto next_of = [&](int j) {                    // the chain's next step
+                for (++j; j < J && !active(mu, j);) ++j;
+                return j;
+            };
+            auto give_back = [&](uint64_t* empty, int j) {
+                umma_commit(empty);
+                if (!(both && j < npre)) umma_commit(empty);
+            };
+            auto scores = [&](int j, int h) {              // S of half h of step j, once its keys are here
                 const int st = j % STAGES;
-                ok = wait_for(&k_full[st], (j / STAGES) & 1);
+                if (h == 0) ok = wait_for(&k_full[st], (j / STAGES) & 1);
                 if (!ok) return;
                 tc_fence_after();
                 if (issuer) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    umma_bf16(s_at, dq[ks], dk0 + STAGE_STEP * st + (uint64_t)(((ks / 4) * SUB + (ks % 4) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
-                umma_commit(&s_full[mu]);
-                umma_commit(&k_empty[st]);
+                    for (int ks = 0; ks < KS; ++ks)
+                        umma_bf16(s_at + h * HALF, dq[ks], dk0 + STAGE_STEP * st + (uint64_t)(((ks / 4) * SUB + h * HK * 128 + (ks % 4) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
+                    umma_commit(&s_full[mu][h]);
+                    if (h == HALVES - 1) give_back(&k_empty[st], j);
                 }
                 __syncwarp();
             };
-            if (ok && active(mu, 0)) scores(0);
             int used = 0;                                  // steps that the chain has taken part in
-            for (int j = 0; j < J && ok; ++j) {
-                const int st = j % STAGES;
-                const uint32_t parity = (j / STAGES) & 1;
-                const bool now = active(mu, j), next = j + 1 < J && active(mu, j + 1), soon = !OVER && now && next;
-                if (soon) {                                // the next scores, as soon as the rows of these are in registers
+            int j = next_of(-1);
+            if (j < J)
+                for (int h = 0; h < HALVES && ok; ++h) scores(j, h);
+            while (j < J && ok) {
+                const int st = j % STAGES, next = next_of(j);
+                if (!OVER && next < J) {                   // the next scores, as soon as the rows of these are in registers
                     ok = wait_for(&s_free[mu], used & 1);
-                    if (ok) scores(j + 1);
+                    if (ok) scores(next, 0);
                     if (!ok) break;
                 }
-                if (now) {
-                    ok = wait_for(&p_full[mu], used & 1) && wait_for(&v_full[st], parity);      // P(j) is written, O rescaled
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) {
+                    ok = wait_for(&p_full[mu][h], used & 1) && (h > 0 || wait_for(&v_full[st], (j / STAGES) & 1));      // P is written, O rescaled
                     if (!ok) break;
                     tc_fence_after();
                     if (issuer) {
 #pragma unroll
-                    for (int kk = 0; kk < KV; ++kk)
-                        umma_bf16_ts(o_at, p_at + kk * 8, dv0 + STAGE_STEP * st + (uint64_t)((kk * 2048) >> 4), idesc_o, (used > 0 || kk > 0) ? 1u : 0u);
-                    umma_commit(&pv_done[mu]);             // P may be overwritten, O rescaled
-                    if (j == last) umma_commit(&o_full[mu]);
-                    umma_commit(&v_empty[st]);
+                        for (int kk = 0; kk < KV; ++kk)
+                            umma_bf16_ts(o_at, p_at + h * HALF + kk * 8, dv0 + STAGE_STEP * st + (uint64_t)(((h * KV + kk) * 2048) >> 4), idesc_o, (used > 0 || h > 0 || kk > 0) ? 1u : 0u);
+                        umma_commit(&pv_done[mu]);         // P may be overwritten, O rescaled
+                        if (h == HALVES - 1) {
+                            if (next >= J) umma_commit(&o_full[mu]);
+                            give_back(&v_empty[st], j);
+                        }
                     }
                     __syncwarp();
-                    ++used;
-                } else {                                   // a stage is given back only once it has been filled: an arrival ahead would count for another round
-                    ok = wait_for(&k_full[st], parity);
+                    // (products run in the order they were issued: where P lies over S, it has been read when the next S overwrites it)
+                    if (OVER && next < J) scores(next, h);
                     if (!ok) break;
-                    if (issuer) mbar_arrive(&k_empty[st]);
-                    ok = wait_for(&v_full[st], parity);
-                    if (!ok) break;
-                    if (issuer) mbar_arrive(&v_empty[st]);
                 }
-                // (products run in the order they were issued: where P lies over S, it has been read when the next S overwrites it)
-                if (next && !soon) scores(j + 1);
+                ++used;
+                j = next;
             }
         }
         __syncwarp();
     } else {
-        // ---- softmax of chain u = 0 (warps 2..5) or 1 (warps 6..9): a thread a pair
-        const int u = warp >= 6 ? 1 : 0, q = warp & 3, r = q * 32 + lane;      // (the lanes of tensor memory that a warp reaches go by its number)
+        // ---- softmax
         const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16);
         const uint32_t S_AT = lane_addr + TMEM_S + S_STEP * u, P_AT = lane_addr + TMEM_P + P_STEP * u, O_AT = lane_addr + TMEM_O + O_STEP * u;
         bool ok = true;
-        const int in_tile = (both ? u * half : 0) + r / heads, my_row = row0 + in_tile, head = kvh * G + h0 + r % heads;
-        const bool pair = r / heads < half && in_tile < rows && plan.ctx[min(in_tile, rows - 1)] > 0;
-        if (both || u == 0) {                              // queries
-            const bf16* src = pair ? p.q + (int64_t)p.row_q_start[my_row] * p.q_stride + (int64_t)head * D : nullptr;
-            uint4 v[D / 8];
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) v[i] = src ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-                *reinterpret_cast<uint4*>(tiles + q_off(u) + (i >> 3) * SUB + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = v[i];
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[u]);
-        }
         // own keys that this pair sees, counted from its list's first: [seen_lo, seen_hi)
         int seen_lo = 0, seen_hi = 0;
         if (pair && plan.own_first[in_tile + 1] > plan.own_first[in_tile]) {
@@ -657,30 +675,97 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             // the keys of the step that this pair sees: [lo, hi)
             int lo = 0, hi = min(PT_KEYS, prefix - (x0 + j) * PT_KEYS);
             unsigned char* v_row = tiles + v_off(st) + r * 128;            // the values of key r of the step (its 16-byte pieces in the swizzle's order)
-            if (j >= npre) {                               // (under the product that forms the scores)
+            bool valid = j < npre && r < hi;               // key r of the step: is it anybody's?  (key `owned` of the tile's row, of own keys)
+            int owned = 0;
+            if (j >= npre) {
                 const OwnStep o = own_step(j);
                 lo = max(0, min(PT_KEYS, seen_lo - o.k * PT_KEYS));
                 hi = max(lo, min(PT_KEYS, seen_hi - o.k * PT_KEYS));
-                // key r: whose is it, and is it one of its keys?
                 const int slot = (o.list ? list0[1] : 0) + o.k * W + (r >> ss);
-                bool valid = false;
-                int i = 0;
                 if (slot < (o.list ? list_end[1] : list_end[0])) {
-                    i = owner(slot);
-                    const int key = own_begin + ((slot - plan.own_first[i]) << ss) + (r & (sk - 1));
-                    valid = key >= prefix && key < plan.ctx[i];
+                    owned = owner(slot);
+                    const int key = own_begin + ((slot - plan.own_first[owned]) << ss) + (r & (sk - 1));
+                    valid = key >= prefix && key < plan.ctx[owned];
                 }
+            }
+#pragma unroll 1
+            for (int h = 0; h < HALVES; ++h) {
+            const int key0 = h * HK, from = max(0, min(HK, lo - key0)), end = max(from, min(HK, hi - key0)), n = used * HALVES + h;      // (n: halves before this one)
+            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u][h], used & 1, abort_p));
+            if (!ok) break;
+            tc_fence_after();
+            float alpha = 1.f;
+            if (__any_sync(0xffffffffu, end > from)) {
+                uint32_t sv[HK];
+#pragma unroll
+                for (int c = 0; c < HK; c += 32) tmem_ld32_async(S_AT + h * HALF + c, sv + c);
+#pragma unroll
+                for (int c = 0; c < HK; c += 32) tmem_ld_wait(sv + c);
+                tc_fence_before();
+                __syncwarp();
+                if (!OVER && lane == 0) mbar_arrive(&s_free[u]);
+                if (__any_sync(0xffffffffu, from > 0 || end < HK)) {
+                    const unsigned keys = end - from;
+#pragma unroll
+                    for (int i = 0; i < HK; ++i) if ((unsigned)(i - from) >= keys) sv[i] = __float_as_uint(-INFINITY);
+                }
+                // the reference point of the exponent moves only when a score would exceed 2^8 against the one in use
+                {
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < HK; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sv[i]));
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2e;
+                    if (mx > -INFINITY && (m_run == -INFINITY || mx - m_run > 8.0f)) {
+                        alpha = m_run == -INFINITY ? 1.f : ex2_approx(m_run - mx);
+                        m_run = mx;
+                    }
+                }
+                // (where P lies over S, scores that are here say that the product which read the P before them is done)
+                if (!OVER && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (n - 1) & 1, abort_p))) { ok = false; break; }
+                if (TURNS && both && j < npre) {                    // the chains take turns at the exponentials of the steps that both take part in
+                    const int turn = u == 0 ? n - 1 : n;
+                    if (turn >= 0 && !__all_sync(0xffffffffu, mbar_wait(&exp_done[u ^ 1], turn & 1, abort_p))) { ok = false; break; }
+                }
+                const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+                float sm[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ch = 0; ch < HK / 32; ++ch) {
+                    uint32_t packed[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float p0 = ex2_approx(fmaf(__uint_as_float(sv[ch * 32 + i]), p.scale_log2e, neg_m));
+                        const float p1 = ex2_approx(fmaf(__uint_as_float(sv[ch * 32 + i + 1]), p.scale_log2e, neg_m));
+                        sm[(i >> 1) & 3] += p0 + p1;
+                        packed[i >> 1] = pack2_bf16(p0, p1);
+                    }
+                    tmem_st16(P_AT + h * HALF + ch * 16, packed);
+                }
+                l_run = l_run * alpha + ((sm[0] + sm[1]) + (sm[2] + sm[3]));
+                __syncwarp();
+                if (TURNS && both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
+            } else {                                       // own keys of other warps' rows (of a prefix: none behind its end): weights of zero
+                if (!OVER && lane == 0) mbar_arrive(&s_free[u]);
+                if (!OVER && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (n - 1) & 1, abort_p))) { ok = false; break; }
+                if (TURNS && both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
+                uint32_t none[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) none[i] = 0;
+#pragma unroll
+                for (int ch = 0; ch < HK / 32; ++ch) tmem_st16(P_AT + h * HALF + ch * 16, none);
+            }
+            // The values' turn comes behind the weights, under whose making they arrive (before: 5,250 cycles a step of own keys instead of 3,600).
+            if (h == 0 && !__all_sync(0xffffffffu, valid && j < npre)) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / STAGES) & 1, abort_p));
                 if (!ok) break;
-                if (!valid) {
+                if (!valid) {                              // nobody's: zeros (of a prefix's last step both chains write the same)
 #pragma unroll
-                    for (int c = 0; c < 8 * PARTS; ++c) *reinterpret_cast<uint4*>(v_row + (c >> 3) * SUB + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    for (int c = 0; c < 8 * PARTS; ++c) *reinterpret_cast<uint4*>(v_row + (c >> 3) * SUB + ((c ^ r) & 7) * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                } else {
+                } else if (j >= npre) {
                     uint32_t bad = 0;                      // an exponent of all ones carries into its number's highest bit
 #pragma unroll
                     for (int c = 0; c < 8 * PARTS; ++c) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(v_row + (c >> 3) * SUB + (c & 7) * 16);
+                        const uint4 v = *reinterpret_cast<const uint4*>(v_row + (c >> 3) * SUB + ((c ^ r) & 7) * 16);
                         bad |= ((v.x & 0x7f807f80u) + 0x00800080u) | ((v.y & 0x7f807f80u) + 0x00800080u) | ((v.z & 0x7f807f80u) + 0x00800080u) | ((v.w & 0x7f807f80u) + 0x00800080u);
                     }
                     if (bad & 0x80008000u) {
@@ -691,81 +776,14 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                             if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
                             *at = x;
                         }
-                        wp.marks[(int64_t)(row0 + i) * p.num_kv_heads + kvh] = G;
+                        wp.marks[(int64_t)(row0 + owned) * p.num_kv_heads + kvh] = G;
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
                 }
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], used & 1, abort_p));
-            if (!ok) break;
-            tc_fence_after();
-            float alpha = 1.f;
-            if (__any_sync(0xffffffffu, hi > lo)) {
-                uint32_t sv[128];
-                tmem_ld32_async(S_AT, sv);
-                tmem_ld32_async(S_AT + 32, sv + 32);
-                tmem_ld32_async(S_AT + 64, sv + 64);
-                tmem_ld32_async(S_AT + 96, sv + 96);
-                if (j < npre && r >= hi) {                 // behind the prefix's end: zeros for its values (both chains write the same; the keys' arrival is long past)
-                    ok = mbar_wait(&v_full[st], (j / STAGES) & 1, abort_p);
-#pragma unroll
-                    for (int c = 0; c < 8 * PARTS; ++c) *reinterpret_cast<uint4*>(v_row + (c >> 3) * SUB + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                tmem_ld_wait(sv); tmem_ld_wait(sv + 32); tmem_ld_wait(sv + 64); tmem_ld_wait(sv + 96);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_before();
-                __syncwarp();
-                if (!OVER && lane == 0) mbar_arrive(&s_free[u]);
-                if (__any_sync(0xffffffffu, lo > 0 || hi < PT_KEYS)) {
-                    const unsigned n = hi - lo;
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) if ((unsigned)(i - lo) >= n) sv[i] = __float_as_uint(-INFINITY);
-                }
-                // the reference point of the exponent moves only when a score would exceed 2^8 against the one in use
-                {
-                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sv[i]));
-                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2e;
-                    if (mx > -INFINITY && (m_run == -INFINITY || mx - m_run > 8.0f)) {
-                        alpha = m_run == -INFINITY ? 1.f : ex2_approx(m_run - mx);
-                        m_run = mx;
-                    }
-                }
-                if (used > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (used - 1) & 1, abort_p))) { ok = false; break; }
-                if (both && j < npre) {                    // the chains take turns at the exponentials of the steps that both take part in
-                    const int turn = u == 0 ? j - 1 : j;
-                    if (turn >= 0 && !__all_sync(0xffffffffu, mbar_wait(&exp_done[u ^ 1], turn & 1, abort_p))) { ok = false; break; }
-                }
-                const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-                float sm[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
-                    uint32_t packed[16];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float p0 = ex2_approx(fmaf(__uint_as_float(sv[ch * 32 + i]), p.scale_log2e, neg_m));
-                        const float p1 = ex2_approx(fmaf(__uint_as_float(sv[ch * 32 + i + 1]), p.scale_log2e, neg_m));
-                        sm[(i >> 1) & 3] += p0 + p1;
-                        packed[i >> 1] = pack2_bf16(p0, p1);
-                    }
-                    tmem_st16(P_AT + ch * 16, packed);
-                }
-                l_run = l_run * alpha + ((sm[0] + sm[1]) + (sm[2] + sm[3]));
-                __syncwarp();
-                if (both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
-            } else {                                       // own keys of other warps' rows (never a step of the prefix): weights of zero
-                if (!OVER && lane == 0) mbar_arrive(&s_free[u]);
-                if (used > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (used - 1) & 1, abort_p))) { ok = false; break; }
-                uint32_t none[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) none[i] = 0;
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch) tmem_st16(P_AT + ch * 16, none);
-            }
-            if (used > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                if (OVER && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (n - 1) & 1, abort_p))) { ok = false; break; }
+                tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D; c += 16) {
                     float v[16];
@@ -780,7 +798,9 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[u]);
+            if (lane == 0) mbar_arrive(&p_full[u][h]);
+            }
+            if (!ok) break;
             ++used;
         }
         if (ok && used > 0) ok = mbar_wait(&o_full[u], 0, abort_p);

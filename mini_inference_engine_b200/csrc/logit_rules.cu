@@ -293,7 +293,7 @@ logit_rules_kernel(const RuleParams p) {
         if (marked) {
             __syncthreads();                              // (choose) nobody asks for marks any more; (apply) the output holds the marked entries' logits
             if (text_counts) {
-                constexpr int AT_ONCE = 4;                // (8: choose 34.9 -> 35.1 us for 200 rows)
+                constexpr int AT_ONCE = 4;                // (choosing for 200 and 64 rows 34.9 and 19.6 us; 2: 36.6 and 20.4, 8: 34.2 and 20.9, and 9.4 for 8 rows instead of 8.3)
                 for (int r0 = 0, turn = 0; r0 < total; r0 += AT_ONCE * T, turn ^= 1) {
                     const int j0 = r0 + tid;
                     int t[AT_ONCE];
