@@ -454,10 +454,10 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
             f[w] = (mm == -INFINITY || m_s[w][g] == -INFINITY) ? 0.f : fast_exp2(m_s[w][g] - mm);
             ll += f[w] * l_s[w][g];
         }
-        const float inv = ll > 0.f ? __frcp_rn(ll) : 0.f;
+        const float inv = ll > 0.f ? __frcp_rn(ll) : SHARED && ll != 0.f ? ll : 0.f;
 #pragma unroll
         for (int w = 0; w < DEC_WARPS; ++w) f_s[w][g] = f[w] * inv;
-        c_lse[g] = ll > 0.f ? mm + __log2f(ll) : -INFINITY;           // base-2 log-sum-exp of this block's part
+        c_lse[g] = ll > 0.f ? mm + __log2f(ll) : SHARED && ll != 0.f ? ll : -INFINITY;           // base-2 log-sum-exp of this block's part (SHARED: no number stays none)
     }
     // Merging the splits inside a cluster: (head, four dimensions) items go round the blocks, item i to
     // block i % S.  Every block sends its normalised partial of an item straight to the item's owner
@@ -584,22 +584,57 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     __syncthreads();
     if (!s_last) return;
     __threadfence();
+    if constexpr (SHARED) {                                        // the row's prefix's results come first; weights a warp a head, then four dimensions of a head a thread
+        __shared__ float all_ref[16], all_inv[16];
+        for (int g = warp; g < gn; g += DEC_WARPS) {
+            const int head = kvh * G + g0 + g;
+            const float* own = p.part_lse + ((int64_t)row * p.num_heads + head) * p.splits;
+            const float* lse = p.pre_lse + pre_at * p.num_heads + head;
+            const float a = lane < pre_n ? __ldcg(lse + (int64_t)lane * p.num_heads) : -INFINITY;
+            const float b = lane + 32 < pre_n ? __ldcg(lse + (int64_t)(lane + 32) * p.num_heads) : -INFINITY;
+            float mm = fmaxf(a, b);
+            for (int s2 = lane; s2 < eff; s2 += 32) mm = fmaxf(mm, __ldcg(own + s2));
+            mm = warp_max(mm);
+            const float ref = mm == -INFINITY ? 0.f : mm, wa = fast_exp2(a - ref), wb = fast_exp2(b - ref);
+            float sum = wa + wb;
+            for (int s2 = lane; s2 < eff; s2 += 32) sum += fast_exp2(__ldcg(own + s2) - ref);
+            sum = warp_sum(sum);
+            const float inv = sum > 0.f ? __frcp_rn(sum) : sum;
+            if (lane < pre_n) pre_w[g][lane] = wa * inv;
+            if (lane + 32 < pre_n) pre_w[g][lane + 32] = wb * inv;
+            if (lane == 0) { all_ref[g] = ref; all_inv[g] = inv; }
+        }
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < gn * (D / 4); idx += DEC_WARPS * 32) {
+            const int g = idx / (D / 4), d = (idx - g * (D / 4)) * 4, head = kvh * G + g0 + g;
+            const int64_t base = ((int64_t)row * p.num_heads + head) * p.splits;
+            float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto add = [&](float w, const float* from) {
+                const float4 part = __ldcg(reinterpret_cast<const float4*>(from));
+                val.x += w * part.x; val.y += w * part.y; val.z += w * part.z; val.w += w * part.w;
+            };
+#pragma unroll 6
+            for (int s2 = 0; s2 < pre_n; ++s2) add(pre_w[g][s2], p.pre_o + ((pre_at + s2) * p.num_heads + head) * D + d);
+#pragma unroll 4
+            for (int s2 = 0; s2 < eff; ++s2) add(fast_exp2(__ldcg(p.part_lse + base + s2) - all_ref[g]) * all_inv[g], p.part_o + (base + s2) * D + d);
+            if (p.out32) {
+                *reinterpret_cast<float4*>(p.out32 + ((int64_t)token * p.num_heads + head) * D + d) = val;
+            } else {
+                uint2 packed;
+                packed.x = pack_bf16(val.x, val.y);
+                packed.y = pack_bf16(val.z, val.w);
+                *reinterpret_cast<uint2*>(p.out + ((int64_t)token * p.num_heads + head) * D + d) = packed;
+            }
+        }
+        return;
+    }
     for (int idx = threadIdx.x; idx < gn * D; idx += DEC_WARPS * 32) {
         const int g = idx / D, d = idx - g * D;
         const int head = kvh * G + g0 + g;
         const int64_t base = ((int64_t)row * p.num_heads + head) * p.splits;
         float mm = -INFINITY;
         for (int s2 = 0; s2 < eff; ++s2) mm = fmaxf(mm, __ldcg(p.part_lse + base + s2));
-        if (SHARED) for (int s2 = 0; s2 < pre_n; ++s2) mm = fmaxf(mm, __ldcg(p.pre_lse + (pre_at + s2) * p.num_heads + head));      // the row's prefix's results come first
         float acc = 0.f, wsum = 0.f;
-        if (SHARED) {
-#pragma unroll 4
-            for (int s2 = 0; s2 < pre_n; ++s2) {
-                const float w = fast_exp2(__ldcg(p.pre_lse + (pre_at + s2) * p.num_heads + head) - (mm == -INFINITY ? 0.f : mm));
-                acc += w * __ldcg(p.pre_o + ((pre_at + s2) * p.num_heads + head) * D + d);
-                wsum += w;
-            }
-        }
         for (int s2 = 0; s2 < eff; ++s2) {
             const float lse = __ldcg(p.part_lse + base + s2);
             if (lse == -INFINITY) continue;

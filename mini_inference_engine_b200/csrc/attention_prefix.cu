@@ -235,11 +235,13 @@ static int launch_prefix(const PrefixParams& p, long long items, cudaStream_t st
 // Two chains of work run side by side, each with four softmax warps, a thread that issues its products, and its own S, P and O in tensor memory:
 //   S = Q K^T; the chain's threads move their rows of S into registers, write P = 2^(s - m), rounded to bfloat16, back, and
 //   O += P V with P as the left operand out of tensor memory and V as it lies.
-// Such a chain takes 4,400 cycles a step, four times what its products take; two fill one another's gaps.  With two tiles of pairs a chain owns a tile, and a
+// Such a chain takes 4,000 cycles a step (heads of 128), four times what its products take; two fill one another's gaps.  With two tiles of pairs a chain owns a tile, and a
 // step of the prefix serves both; with one the chains take the steps in turns over the same queries and leave a result each.
 // Keys and values come by TMA, a slot a copy, keys and values each with barriers of their own: keys of a later step arrive as soon as S is formed.
 // Tensor memory: heads of 64 S 2 x 128 columns, P 2 x 64, O 2 x 64; S of the next step is issued as soon as the rows are in registers.  Heads of 128: O takes
-// 2 x 128, and P lies over the S that it came from, so that S of the next step is issued behind this step's product with the values.
+// 2 x 128, and P lies over the S that it came from.  A step's S, P and product with the values then go in halves of 64 keys: S of the next step's first half is
+// formed under the softmax of this one's second (whole steps, S behind the product with the values: 51 -> 45 us for 64 rows behind 8,000 keys, 124 -> 110 for 256
+// behind 16,384).
 //
 // Values of one row must not reach another's output: slots' keys that are nobody's (in front of a row's own keys, behind its context) are made zero in
 // shared memory, and so are own values that are not finite, since 0 times those is not 0; the row is marked, and the joining kernel adds them to its output.
@@ -247,10 +249,8 @@ static int launch_prefix(const PrefixParams& p, long long items, cudaStream_t st
 #define PT_ROWS 128
 #define PT_KEYS 128
 #define PT_COST_START 7            // what starting and ending an item costs, in steps (3: 131 us for 256 rows behind 16,384 keys instead of 124)
-#ifndef TURNS
-#define TURNS 1
-#endif
-#define PT_WALK_PAIRS 128          // pairs on a key head up to which the kernel for any head size takes over: see mie_prefix_layout
+#define PT_WALK_PAIRS 128          // pairs on a key head up to which the kernel for any head size takes over (see mie_prefix_layout) ...
+#define PT_WALK_BYTES (16 << 20)   // ... unless heads are of 128 and there is this much to read
 #define PT_MOST_TILES 512          // tiles of rows that a launch can plan for ...
 #define PT_MOST_SEGMENTS 63        // ... and groups with the rows between them
 
@@ -722,7 +722,7 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 }
                 // (where P lies over S, scores that are here say that the product which read the P before them is done)
                 if (!OVER && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (n - 1) & 1, abort_p))) { ok = false; break; }
-                if (TURNS && both && j < npre) {                    // the chains take turns at the exponentials of the steps that both take part in
+                if (both && j < npre) {                    // the chains take turns at the exponentials of the steps that both take part in (118 us for 256 rows without)
                     const int turn = u == 0 ? n - 1 : n;
                     if (turn >= 0 && !__all_sync(0xffffffffu, mbar_wait(&exp_done[u ^ 1], turn & 1, abort_p))) { ok = false; break; }
                 }
@@ -742,11 +742,11 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 }
                 l_run = l_run * alpha + ((sm[0] + sm[1]) + (sm[2] + sm[3]));
                 __syncwarp();
-                if (TURNS && both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
+                if (both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
             } else {                                       // own keys of other warps' rows (of a prefix: none behind its end): weights of zero
                 if (!OVER && lane == 0) mbar_arrive(&s_free[u]);
                 if (!OVER && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (n - 1) & 1, abort_p))) { ok = false; break; }
-                if (TURNS && both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
+                if (both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
                 uint32_t none[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) none[i] = 0;
@@ -985,9 +985,12 @@ extern "C" int mie_prefix_layout(SharedArgs* a, int sms) {
     if (a->num_rows < 0 || a->num_kv_heads <= 0 || a->num_heads <= 0 || a->num_heads % a->num_kv_heads || a->head_dim < 16 || a->head_dim > 128 || a->head_dim % 16
         || sms <= 0 || a->page_size < 1 || (a->page_size & (a->page_size - 1))) return MIE_ERR_BAD_ARG;
     const int G = a->num_heads / a->num_kv_heads;
-    // Few pairs leave the walk's tiles of 128 empty, and it takes longer to begin.  Us, walk : the other two kernels -- 32 heads of 64 on 4, 2 rows behind 208 keys 11.2 : 9.8, 8
-    // behind 2,048 14.8 : 13.0, 16 16.0 : 14.0, 32 19.6 : 30.1; 32 of 128 on 8, 16 rows behind 4,000 25.3 : 21.4, 64 behind 8,000 53 : 84; 32 of 128 on 32, 33 rows in five groups 91 : 74.
-    for (a->walk = a->num_rows * (long long)G > PT_WALK_PAIRS; a->walk >= 0; --a->walk) {
+    // Few pairs leave the walk's tiles of 128 empty, and it takes longer to begin; what it gains grows with the keys and values that there are.  Us, walk : the other
+    // two kernels -- 32 heads of 64 on 4, 2 rows behind 208 keys 11.4 : 9.5, 8 behind 2,048 15.4 : 13.1, 16 16.0 : 14.3, 32 19.6 : 30; 32 on 32, 16 rows behind
+    // 3,000 35.9 : 30.2.  Heads of 128, 32 on 8: 16 rows behind 1,000 19.5 : 17.2, behind 4,000 21.2 : 21.6, behind 16,000 35 : 48, 64 behind 8,000 45 : 84;
+    // 32 on 32: 8 rows behind 2,000 21.4 : 23.5, 33 rows in five groups 69 : 74.
+    const double bytes = 4.0 * a->num_kv_heads * a->head_dim * (a->most_prefix + 0.5 * a->num_rows * a->most_own);
+    for (a->walk = a->num_rows * (long long)G > PT_WALK_PAIRS || (a->head_dim == 128 && bytes > PT_WALK_BYTES); a->walk >= 0; --a->walk) {
         const int pairs = a->walk ? PT_ROWS : PFX_PAIRS;
         a->chunks = (G + pairs - 1) / pairs;
         a->chunk_heads = (G + a->chunks - 1) / a->chunks;

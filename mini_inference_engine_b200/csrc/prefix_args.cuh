@@ -12,7 +12,8 @@ struct SharedArgs {
     long long q_stride, num_pages, most_slots;
     int table_stride, num_rows, groups, num_heads, num_kv_heads, head_dim, page_size, out_f32;
     int splits, stages, tma, min_part_tiles;                                      // the decode kernel's plan for the rows' own keys
-    int chunk_heads, chunks, tile_rows, places, walk;                             // mie_prefix_layout
+    int chunk_heads, chunks, tile_rows, places, walk;                             // mie_prefix_layout ...
+    int most_prefix, most_own;                                                    // ... which goes by these bounds on a prefix and on a row's own keys
     float scale;
 };
 

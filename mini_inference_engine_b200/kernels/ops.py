@@ -746,7 +746,7 @@ class _SharedArgs(ctypes.Structure):          # csrc/prefix_args.cuh
                                                 "out", "pre_o", "pre_lse", "pre_chunk", "row_info", "marks", "part_o", "part_lse", "counters")]
                 + [(n, ctypes.c_longlong) for n in ("q_stride", "num_pages", "most_slots")]
                 + [(n, ctypes.c_int) for n in ("table_stride", "num_rows", "groups", "num_heads", "num_kv_heads", "head_dim", "page_size", "out_f32", "splits",
-                                               "stages", "tma", "min_part_tiles", "chunk_heads", "chunks", "tile_rows", "places", "walk")]
+                                               "stages", "tma", "min_part_tiles", "chunk_heads", "chunks", "tile_rows", "places", "walk", "most_prefix", "most_own")]
                 + [("scale", ctypes.c_float)])
 
 
@@ -759,11 +759,11 @@ def _shared_libs():
 
 
 @functools.lru_cache(maxsize=256)
-def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_own: int,
+def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_prefix: int, max_own: int,
                  pages: int):
     """What a launch of these sizes keeps from call to call: its plan and its scratch memory, as the bytes of a _SharedArgs (and the tensors)."""
     a = _SharedArgs(num_rows=rows, groups=groups, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size,
-                    num_pages=pages)
+                    most_prefix=max_prefix, most_own=max_own, num_pages=pages)
     where = torch.device("cuda", device)
     _need(_shared_libs()[0].mie_prefix_layout(ctypes.byref(a), num_sms(where)) == 0, f"{num_heads} heads of {head_dim} on {num_kv_heads}: not taken")
     kept = [_workspace(where, "prefix_o", a.most_slots * num_heads * head_dim, torch.float32), _workspace(where, "prefix_lse", a.most_slots * num_heads, torch.float32),
@@ -844,8 +844,10 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     if groups == 0 or max_prefix == 0:                        # nothing is shared
         return decode_attention(q, q_stride, k_cache, v_cache, block_tables, row_q_start, row_q_len, row_ctx_len, out, num_heads, num_kv_heads, head_dim,
                                 page_size, scale, max_ctx=max_own)
-    # (own keys are planned for in powers of two: a plan serves many steps)
-    plan, walk, _ = _shared_plan(device, rows, groups, num_heads, num_kv_heads, head_dim, page_size, 1 << (max_own - 1).bit_length(), shape[0])
+    max_prefix = width * page_size if max_prefix is None else max(1, min(max_prefix, width * page_size))
+    # (lengths are planned for in powers of two: a plan serves many steps)
+    plan, walk, _ = _shared_plan(device, rows, groups, num_heads, num_kv_heads, head_dim, page_size, 1 << (max_prefix - 1).bit_length(),
+                                 1 << (max_own - 1).bit_length(), shape[0])
     a = _SharedArgs.from_buffer_copy(plan)
     a.q, a.k_cache, a.v_cache, a.out = at_q, at_k, at_v, at_out
     a.block_tables, a.row_q_start, a.row_q_len, a.row_ctx_len = _at(block_tables), _at(row_q_start), _at(row_q_len), _at(row_ctx_len)

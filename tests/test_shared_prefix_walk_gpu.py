@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 
 def walks(ops, c, **hints):
     """The case, run by the walk: its plan says so."""
-    return ops._shared_plan(torch.cuda.current_device(), c.rows, c.group_prefix.numel(), c.H, c.G, c.D, c.page, hints.get("max_own", 1), c.cache.shape[1])[1]
+    return ops._shared_plan(torch.cuda.current_device(), c.rows, c.group_prefix.numel(), c.H, c.G, c.D, c.page, hints["max_prefix"], hints["max_own"],
+                            c.cache.shape[1])[1]
 
 
 @pytest.mark.parametrize("D", [64, 128])
@@ -255,3 +256,20 @@ def test_groups_and_lengths_out_of_range_are_reported(ops, H, G, D):
         ops.range_report().zero_()
         sound = Case([(6, 100), (4, 20)], 30, H, G, D, 16, seed=D)
         sound.check(sound.run(ops, **sound.hints))            # the call after it is as it should be
+
+
+@pytest.mark.parametrize("D,groups,own", [(64, [(2, 6000), (1, 0)], 900), (80, [(3, 5000)], 700), (128, [(1, 9000), (2, 40)], 500)])
+def test_few_rows_with_many_own_keys(ops, D, groups, own):
+    """The kernel for any head size: a row's own keys in parts, behind a prefix in many ranges; a query that is no number shows in its row and head only."""
+    c = Case(groups, own, 8, 2, D, 16, seed=D)
+    assert not walks(ops, c, **c.hints)
+    out = c.run(ops, **c.hints)
+    c.check(out)
+    assert torch.equal(out, c.run(ops, **c.hints))
+    c.check(c.run(ops, dtype=torch.float32, **c.hints))
+    c.qkv[1, 3 * D + 1] = float("nan")
+    out = c.run(ops, **c.hints)
+    assert torch.isnan(out[1, 3]).all()
+    out[1, 3] = 0
+    assert torch.isfinite(out).all()
+    c.check(out, [0, 2])
