@@ -529,7 +529,7 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         later = place_of(STAGES);
     }
     // Softmax warps 2..5 (chain 0) and 6..9 (chain 1), a thread a pair: which, and its query, under the copies and the hand-out of tensor memory.  A query's 16-byte
-    // pieces go to neighbouring lanes (a lane its own query, behind the hand-out: 8,000 cycles a block).
+    // pieces go to neighbouring lanes (a lane its own query, behind the hand-out: 4 us more).
     const int u = warp >= 6 ? 1 : 0, q = warp & 3, r = q * 32 + lane;      // (the lanes of tensor memory that a warp reaches go by its number)
     const int in_tile = (both ? u * half : 0) + r / heads, my_row = row0 + in_tile, head = kvh * G + h0 + r % heads;
     const bool softmax = warp >= 2 && warp <= 9, pair = softmax && r / heads < half && in_tile < rows && plan.ctx[min(in_tile, rows - 1)] > 0;
@@ -539,13 +539,14 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         pdl_wait();
         uint4 v[LANES];
 #pragma unroll
-        for (int i = 0; i < LANES; ++i) {
+        for (int i = 0; i < LANES; ++i) {                  // (where there is no pair the first query is read, and zeros are stored: a branch a load put them one behind another, 5 us)
             const int64_t src = __shfl_sync(0xffffffffu, mine, i * AT_ONCE + lane / LANES);
-            v[i] = src >= 0 ? *reinterpret_cast<const uint4*>(p.q + src + lane % LANES * 8) : make_uint4(0, 0, 0, 0);
+            v[i] = *reinterpret_cast<const uint4*>(p.q + max((int64_t)0, src) + lane % LANES * 8);
         }
 #pragma unroll
         for (int i = 0; i < LANES; ++i) {
             const int to_r = q * 32 + i * AT_ONCE + lane / LANES, c = lane % LANES;
+            if (__shfl_sync(0xffffffffu, mine, i * AT_ONCE + lane / LANES) < 0) v[i] = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4*>(tiles + q_off(u) + (c >> 3) * SUB + to_r * 128 + (((c & 7) ^ (to_r & 7)) << 4)) = v[i];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
