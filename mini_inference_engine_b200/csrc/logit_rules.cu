@@ -16,7 +16,7 @@
 // order.  (Penalties worked out where the logits pass by: some lane of nearly every warp met a marked entry, and the warp went through the divisions of all
 // four of its group; 256 rows of 128,256 entries on texts of up to 8,000 tokens 97 us.)  A slice larger than the table takes several turns.
 // Which thread takes an entry differs from run to run, and the same call is to give the same bits: the settled entries of a round (4 tokens a thread) are
-// summed as integers, relative to the round's greatest, which no order changes (34.9 us for the choice of 200 rows; each thread to its own sum 32.3).
+// summed as integers, relative to the round's greatest, which no order changes (34.9 us for the choice of 200 rows; each thread to its own sum 32.6).
 // Choosing: the slices of a row are a thread-block cluster whose first block joins the winners and the sums that the others write into its shared
 // memory (the maximum of x' and the sum of exp(x' - maximum), in float32, joined pairwise).
 //
@@ -422,10 +422,11 @@ static int rules_table(int per) {
     const int words = (per / 2 + 8 + 3) & ~3;
     return words < RULES_TABLE ? words : RULES_TABLE;
 }
-// Slices a row and threads a block.  A round of blocks takes its chain of loads and barriers (6 us, and what more warps add to the barriers), 0.6 us for
-// 16 entries a thread and 1.5 us for eight tokens of text a thread (a row's text is taken as half as long as the slots are wide); the cut whose
-// rounds are over first.  Us, slices x threads: the choice for 200 rows of 50,001 entries, 1 x 1,024 31.7, 2 x 512 34.2, 4 x 512 41, 8 x 256 48; for 8 rows
-// of 32,000, 8 x 256 7.3, 8 x 1,024 8.9, 1 x 1,024 10.2; 256 rows of 128,256 written, texts of up to 8,000, 2 x 1,024 77, 4 x 512 80, 8 x 256 88.
+// Slices a row and threads a block: the cut whose rounds of blocks are over first, a round counted as 2 for its chain of loads and barriers and 0.4 for every 256
+// threads more in those, 0.3 for 16 entries a thread and 3 for eight tokens of text a thread (a row's text is taken as half as long as the slots are wide).  These
+// weights take, of twelve cuts measured for thirty shapes (1 to 500 rows, 32,000 to 151,936 entries, texts of 64 to 12,000), one that is 6% behind the best on the
+// average; 6, 0.4, 0.6 and 1.5 one 8% behind.  Us, slices x threads: the choice for 200 rows of 50,001 entries, 1 x 1,024 32.8, 1 x 512 35.0, 2 x 512 35.3, 8 x 256
+// 53; for 8 rows of 32,000, 8 x 256 7.8, 8 x 512 8.2, 1 x 1,024 11.1; 64 rows of 128,256 written, texts of up to 2,000, 4 x 512 18.3, 8 x 256 19.4, 2 x 1,024 18.5.
 struct RuleCut { int parts, threads; };
 static RuleCut rules_cut(int rows, int vocab, int width, bool choose) {
     RuleCut best = {1, 1024};
@@ -436,7 +437,7 @@ static RuleCut rules_cut(int rows, int vocab, int width, bool choose) {
             int fit = (int)(232448 / ((size_t)rules_table(per) * 4 + 2048));
             if (fit > RULES_SM_THREADS / threads) fit = RULES_SM_THREADS / threads;
             const int64_t places = (int64_t)fit * device_sm_count(), rounds = ((int64_t)rows * parts + places - 1) / places;
-            const double cost = (double)rounds * (6.0 + 0.4 * (threads / 256 - 1) + 0.6 * per / (16.0 * threads) + 1.5 * (width / 2) / (8.0 * threads));
+            const double cost = (double)rounds * (2.0 + 0.4 * (threads / 256 - 1) + 0.3 * per / (16.0 * threads) + 3.0 * (width / 2) / (8.0 * threads));
             if (cost < least) { least = cost; best = RuleCut{parts, threads}; }
         }
     }
