@@ -57,12 +57,12 @@ def rotates_in_decode(dtype, head_dim: int, ctx) -> bool:
     """Whether ``attention(..., rope=...)`` can rotate q and the new key itself and write the cache: a step of
     decoding rows only, on the tensor-core decode kernel, with a head size it rotates."""
     return (_backend == "auto" and dtype == torch.bfloat16 and head_dim <= 128 and head_dim % 32 == 0
-            and decode_only(ctx) and ctx.prefix is None)
+            and decode_only(ctx) and getattr(ctx, "prefix", None) is None)
 
 
 # Shared prefixes against ordinary decode attention, which reads a prefix once a row, by the bytes of keys and values that sharing saves a layer (SHARE_MIN_BYTES).
-# Us, ordinary : shared -- 32 heads of 64 on 4, 2 rows behind 208 keys 4.2 : 11.9, 8 behind 2,048 (15 MB) 10.0 : 15.8; 32 of 128 on 8, 64 behind 8,000 (2.1 GB) 376 : 62, 256 behind
-# 16,384 1,983 : 143; 32 of 128 on 32, 33 rows in five groups (0.9 GB) 159 : 76.
+# Us, ordinary : shared -- 32 heads of 64 on 4, 2 rows behind 208 keys 4.2 : 9.4, 8 behind 2,048 (15 MB) 10.0 : 13.0; 32 of 128 on 8, 64 behind 8,000 (2.1 GB) 376 : 43, 256 behind
+# 16,384 1,983 : 110; 32 of 128 on 32, 33 rows in five groups (0.9 GB) 159 : 69.
 SHARE_MIN_BYTES = 48 << 20
 
 
@@ -158,9 +158,10 @@ def attention(qkv, ctx, cache, out, num_heads, num_kv_heads, head_dim, scale, wi
                              "in steps of 32 up to 128)")
         return ops.decode_attention(*args, out, num_heads, num_kv_heads, head_dim, cache.page_size, scale, window,
                                     max_ctx=ctx.max_ctx_len, rope=rope)
-    if ctx.prefix is not None and fast and window == 0 and mods is None and decode_only(ctx):
-        return ops.shared_prefix_attention(*args, ctx.prefix.start, ctx.prefix.length, out, num_heads, num_kv_heads, head_dim, cache.page_size, scale,
-                                           max_prefix=ctx.prefix.max_prefix, max_own=ctx.prefix.max_own)
+    prefix = getattr(ctx, "prefix", None)
+    if prefix is not None and fast and window == 0 and mods is None and decode_only(ctx):
+        return ops.shared_prefix_attention(*args, prefix.start, prefix.length, out, num_heads, num_kv_heads, head_dim, cache.page_size, scale,
+                                           max_prefix=prefix.max_prefix, max_own=prefix.max_own)
     if not fast and _backend == "auto" and ops.attention_f32_takes(qkv, cache.k, cache.v, out, head_dim):
         return _attention_f32(args, ctx, out, num_heads, num_kv_heads, head_dim, cache.page_size, scale, window, mods, keep)
     if not fast:
