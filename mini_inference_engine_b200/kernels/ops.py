@@ -760,15 +760,22 @@ def _shared_libs():
 
 @functools.lru_cache(maxsize=256)
 def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_prefix: int, max_own: int,
-                 pages: int):
-    """What a launch of these sizes keeps from call to call: its plan and its scratch memory, as the bytes of a _SharedArgs (and the tensors)."""
+                 pages: int, stream: int):
+    """What a launch of these sizes keeps from call to call: its plan and its scratch memory, as the bytes of a _SharedArgs (and the tensors).  Every stream
+    has scratch memory of its own, so that calls on two do not meet; ``stream`` 0: the default stream, and captured launches."""
     a = _SharedArgs(num_rows=rows, groups=groups, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size,
                     most_prefix=max_prefix, most_own=max_own, num_pages=pages)
     where = torch.device("cuda", device)
     _need(_shared_libs()[0].mie_prefix_layout(ctypes.byref(a), num_sms(where)) == 0, f"{num_heads} heads of {head_dim} on {num_kv_heads}: not taken")
-    kept = [_workspace(where, "prefix_o", a.most_slots * num_heads * head_dim, torch.float32), _workspace(where, "prefix_lse", a.most_slots * num_heads, torch.float32),
-            _workspace(where, "prefix_chunk", 1, torch.int32), _workspace(where, "prefix_rows", 2 * rows, torch.int32),
-            _workspace(where, "prefix_marks", rows * num_kv_heads, torch.int32)]
+    own = f"@{stream}" if stream else ""
+
+    def scratch(name, numel, dtype=torch.float32, zero=False):
+        if zero and own:                                      # a launch captured later finds these cleared, outside its graph
+            _workspace(where, name, numel, dtype)
+        return _workspace(where, name + own, numel, dtype)
+
+    kept = [scratch("prefix_o", a.most_slots * num_heads * head_dim), scratch("prefix_lse", a.most_slots * num_heads), scratch("prefix_chunk", 1, torch.int32),
+            scratch("prefix_rows", 2 * rows, torch.int32), scratch("prefix_marks", rows * num_kv_heads, torch.int32, zero=True)]
     for name, t in zip(("pre_o", "pre_lse", "pre_chunk", "row_info", "marks"), kept):
         setattr(a, name, t.data_ptr())
     if not a.walk:                                            # the rows' own keys by the decode kernel behind
@@ -779,8 +786,8 @@ def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_hea
         a.tma = tma_ok and decode_uses_tma(blocks, head_dim)
         a.stages = decode_stages(blocks, max_own, a.splits, bool(a.tma), head_dim, clustered=False)
         if a.splits > 1:
-            more = [_workspace(where, "decode_part_o", rows * num_heads * a.splits * head_dim, torch.float32),
-                    _workspace(where, "decode_part_lse", rows * num_heads * a.splits, torch.float32), _workspace(where, "decode_counters", rows * units, torch.int32)]
+            more = [scratch("decode_part_o", rows * num_heads * a.splits * head_dim), scratch("decode_part_lse", rows * num_heads * a.splits),
+                    scratch("decode_counters", rows * units, torch.int32, zero=True)]
             a.part_o, a.part_lse, a.counters = (t.data_ptr() for t in more)
             kept += more
     return bytes(a), bool(a.walk), kept
@@ -812,8 +819,9 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     prefixes and on the keys behind them, for planning (a captured step's may be shorter); without them the block table's width bounds both.
 
     Two launches: the keys (prefixes in tiles of (row, head) pairs, and the rows' own), then what joins a row's partial results.  Rows with more than
-    one new token are skipped.  With other head sizes than 64 and 128, or pages below 8, slots of a row's last page behind its context must hold
-    finite values (see ``decode_uses_tma``)."""
+    one new token are skipped.  Slots of a row's last page behind its context must hold
+    finite values (see ``decode_uses_tma``).  Launches captured on any streams share scratch memory, as those of other kernels here do: their graphs are replayed one
+    behind the other."""
     _need(q.dtype == torch.bfloat16 == k_cache.dtype == v_cache.dtype and out.dtype in (torch.bfloat16, torch.float32),
           "attention over shared prefixes is bfloat16 (its output bfloat16 or float32)")
     i32 = torch.int32
@@ -847,7 +855,8 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     max_prefix = width * page_size if max_prefix is None else max(1, min(max_prefix, width * page_size))
     # (lengths are planned for in powers of two: a plan serves many steps)
     plan, walk, _ = _shared_plan(device, rows, groups, num_heads, num_kv_heads, head_dim, page_size, 1 << (max_prefix - 1).bit_length(),
-                                 1 << (max_own - 1).bit_length(), shape[0])
+                                 1 << (max_own - 1).bit_length(), shape[0],
+                                 0 if torch.cuda.is_current_stream_capturing() else raw_stream().value or 0)
     a = _SharedArgs.from_buffer_copy(plan)
     a.q, a.k_cache, a.v_cache, a.out = at_q, at_k, at_v, at_out
     a.block_tables, a.row_q_start, a.row_q_len, a.row_ctx_len = _at(block_tables), _at(row_q_start), _at(row_q_len), _at(row_ctx_len)
@@ -1014,6 +1023,7 @@ def sample(logits: torch.Tensor, temperature, request, position, seed: int, out:
         return out
     if rules is None:
         _need(logits.dtype == torch.float32 and (logits.stride(1) == 1 or vocab <= 1), "logits must be float32, a row's entries side by side")
+        _need(logits.is_cuda and logits.device.index == torch.cuda.current_device(), "logits must be on the current device")
         args = _NO_RULES
     else:
         args = rules.args(logits)

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 def walks(ops, c, **hints):
     """The case, run by the walk: its plan says so."""
     return ops._shared_plan(torch.cuda.current_device(), c.rows, c.group_prefix.numel(), c.H, c.G, c.D, c.page, hints["max_prefix"], hints["max_own"],
-                            c.cache.shape[1])[1]
+                            c.cache.shape[1], 0)[1]
 
 
 @pytest.mark.parametrize("D", [64, 128])
@@ -273,3 +273,22 @@ def test_few_rows_with_many_own_keys(ops, D, groups, own):
     out[1, 3] = 0
     assert torch.isfinite(out).all()
     c.check(out, [0, 2])
+
+
+def test_calls_on_two_streams_at_once(ops):
+    """Each stream's calls use scratch memory of their own."""
+    cases = [Case([(40, 900)], 200, 32, 2, 64, 16, seed=3), Case([(2, 3000)], 700, 8, 2, 64, 16, seed=4), Case([(17, 2000), (3, 100)], 100, 8, 8, 128, 16, seed=5)]
+    want = [c.run(ops, **c.hints) for c in cases]
+    for c, o in zip(cases, want):
+        c.check(o)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for turn in range(10):
+        got = []
+        for k in range(9):
+            i = (k + turn) % 3
+            with torch.cuda.stream(streams[k % 3]):
+                got.append((i, cases[i].run(ops, **cases[i].hints)))
+        torch.cuda.synchronize()
+        for i, o in got:
+            assert torch.equal(o, want[i]), (turn, i)
