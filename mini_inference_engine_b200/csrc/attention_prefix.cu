@@ -1006,7 +1006,8 @@ extern "C" int mie_prefix_layout(SharedArgs* a, int sms) {
 }
 
 extern "C" int mie_prefix_attention(const SharedArgs* a, cudaStream_t stream) {
-    if (a->num_rows <= 0 || (!a->walk && a->groups <= 0)) return 0;
+    if (a->num_rows <= 0) return 0;
+    if (a->groups <= 0 || (!a->walk && !a->own_keys)) return MIE_ERR_BAD_ARG;
     if (a->num_rows > 65535) return MIE_ERR_TOO_LARGE;
     WalkParams w = {};
     PrefixParams& p = w.b;
@@ -1024,17 +1025,18 @@ extern "C" int mie_prefix_attention(const SharedArgs* a, cudaStream_t stream) {
     const long long items = prefix_most_items(a->num_rows, a->walk ? a->groups + 2 : a->groups, p.groups.units, p.groups.tile_rows, p.groups.places);
     if (items > 0x7fffffffll) return MIE_ERR_TOO_LARGE;
     if (a->walk) return a->head_dim == 64 ? launch_walk<64>(w, a->out, a->out_f32 != 0, items, stream) : launch_walk<128>(w, a->out, a->out_f32 != 0, items, stream);
+    int rc = MIE_ERR_BAD_ARG;
     switch (a->head_dim) {
-        case 16: return launch_prefix<16>(p, items, stream);
-        case 32: return launch_prefix<32>(p, items, stream);
-        case 48: return launch_prefix<48>(p, items, stream);
-        case 64: return launch_prefix<64>(p, items, stream);
-        case 80: return launch_prefix<80>(p, items, stream);
-        case 96: return launch_prefix<96>(p, items, stream);
-        case 112: return launch_prefix<112>(p, items, stream);
-        case 128: return launch_prefix<128>(p, items, stream);
+        case 16: rc = launch_prefix<16>(p, items, stream); break;
+        case 32: rc = launch_prefix<32>(p, items, stream); break;
+        case 48: rc = launch_prefix<48>(p, items, stream); break;
+        case 64: rc = launch_prefix<64>(p, items, stream); break;
+        case 80: rc = launch_prefix<80>(p, items, stream); break;
+        case 96: rc = launch_prefix<96>(p, items, stream); break;
+        case 112: rc = launch_prefix<112>(p, items, stream); break;
+        case 128: rc = launch_prefix<128>(p, items, stream); break;
     }
-    return MIE_ERR_BAD_ARG;
+    return rc ? rc : a->own_keys(a, stream);
 }
 
 // Non-zero when a block of any launch so far gave up a bounded wait.

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 import math
 
 import torch
@@ -742,26 +743,28 @@ def decode_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, block_tab
 
 
 class _SharedArgs(ctypes.Structure):          # csrc/prefix_args.cuh
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k_cache", "v_cache", "block_tables", "row_q_start", "row_q_len", "row_ctx_len", "group_start", "group_prefix",
-                                                "out", "pre_o", "pre_lse", "pre_chunk", "row_info", "marks", "part_o", "part_lse", "counters")]
-                + [(n, ctypes.c_longlong) for n in ("q_stride", "num_pages", "most_slots")]
-                + [(n, ctypes.c_int) for n in ("table_stride", "num_rows", "groups", "num_heads", "num_kv_heads", "head_dim", "page_size", "out_f32", "splits",
-                                               "stages", "tma", "min_part_tiles", "chunk_heads", "chunks", "tile_rows", "places", "walk", "most_prefix", "most_own")]
-                + [("scale", ctypes.c_float)])
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k_cache", "v_cache", "block_tables", "row_q_start", "row_q_len", "row_ctx_len", "group_start", "group_prefix", "out")]
+                + [("q_stride", ctypes.c_longlong), ("table_stride", ctypes.c_int), ("out_f32", ctypes.c_int), ("scale", ctypes.c_float), ("walk", ctypes.c_int)]
+                + [(n, ctypes.c_void_p) for n in ("own_keys", "pre_o", "pre_lse", "pre_chunk", "row_info", "marks", "part_o", "part_lse", "counters")]
+                + [(n, ctypes.c_longlong) for n in ("num_pages", "most_slots")]
+                + [(n, ctypes.c_int) for n in ("num_rows", "groups", "num_heads", "num_kv_heads", "head_dim", "page_size", "splits", "stages", "tma", "min_part_tiles",
+                                               "chunk_heads", "chunks", "tile_rows", "places", "most_prefix", "most_own")])
+
+
+_shared_call = struct.Struct("10Pqiifi")                       # the fields that are a call's own, up to "walk"
 
 
 @functools.lru_cache(maxsize=None)
 def _shared_libs():
     first, second = load("attention_prefix"), load("attention_decode_shared")
-    for fn in (first.mie_prefix_attention, second.mie_decode_attention_shared):
-        fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    first.mie_prefix_attention.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
     return first, second
 
 
 @functools.lru_cache(maxsize=256)
 def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_prefix: int, max_own: int,
                  pages: int, stream: int):
-    """What a launch of these sizes keeps from call to call: its plan and its scratch memory, as the bytes of a _SharedArgs (and the tensors).  Every stream
+    """What a launch of these sizes keeps from call to call: its plan and its scratch memory, as the bytes of a _SharedArgs behind a call's own (and the tensors).  Every stream
     has scratch memory of its own, so that calls on two do not meet; ``stream`` 0: the default stream, and captured launches."""
     a = _SharedArgs(num_rows=rows, groups=groups, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size,
                     most_prefix=max_prefix, most_own=max_own, num_pages=pages)
@@ -779,6 +782,7 @@ def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_hea
     for name, t in zip(("pre_o", "pre_lse", "pre_chunk", "row_info", "marks"), kept):
         setattr(a, name, t.data_ptr())
     if not a.walk:                                            # the rows' own keys by the decode kernel behind
+        a.own_keys = ctypes.cast(_shared_libs()[1].mie_decode_attention_shared, ctypes.c_void_p).value
         units = num_kv_heads * -(-(num_heads // num_kv_heads) // 16)
         tma_ok = head_dim in (64, 128) and page_size >= 8
         a.splits, a.min_part_tiles = own_keys_plan(rows, units, max_own, tma_ok, head_dim)
@@ -790,7 +794,7 @@ def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_hea
                     scratch("decode_counters", rows * units, torch.int32, zero=True)]
             a.part_o, a.part_lse, a.counters = (t.data_ptr() for t in more)
             kept += more
-    return bytes(a), bool(a.walk), kept
+    return bytes(a)[_shared_call.size:], a.walk, kept
 
 
 def own_keys_plan(rows: int, kv_units: int, max_own: int, tma_ok: bool, head_dim: int) -> tuple[int, int]:
@@ -822,51 +826,47 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     one new token are skipped.  Slots of a row's last page behind its context must hold
     finite values (see ``decode_uses_tma``).  Launches captured on any streams share scratch memory, as those of other kernels here do: their graphs are replayed one
     behind the other."""
-    _need(q.dtype == torch.bfloat16 == k_cache.dtype == v_cache.dtype and out.dtype in (torch.bfloat16, torch.float32),
-          "attention over shared prefixes is bfloat16 (its output bfloat16 or float32)")
-    i32 = torch.int32
+    bf16, i32, f32 = torch.bfloat16, torch.int32, out.dtype == torch.float32
+    _need(q.dtype == bf16 == k_cache.dtype == v_cache.dtype and (f32 or out.dtype == bf16), "attention over shared prefixes is bfloat16 (its output bfloat16 or float32)")
     _need(block_tables.dtype == row_q_start.dtype == row_q_len.dtype == row_ctx_len.dtype == group_start.dtype == group_prefix.dtype == i32
           and block_tables.is_contiguous() and row_q_start.is_contiguous() and row_q_len.is_contiguous() and row_ctx_len.is_contiguous()
           and group_start.is_contiguous() and group_prefix.is_contiguous(), "block tables, rows and groups must be contiguous int32 tensors")
     rows, groups = row_q_len.numel(), group_prefix.numel()
     _need(num_kv_heads > 0 and num_heads % num_kv_heads == 0, "query heads must be a multiple of kv heads")
-    _need(head_dim % 16 == 0 and 16 <= head_dim <= 128, f"head_dim {head_dim}: attention over shared prefixes takes multiples of 16 from 16 to 128")
+    _need(head_dim % 16 == 0 and 16 <= head_dim <= 128, "attention over shared prefixes takes head sizes in multiples of 16 from 16 to 128")
     _need(page_size >= 1 and page_size & (page_size - 1) == 0, "the page size must be a power of two")
     shape = k_cache.shape
     _need(len(shape) == 4 and shape == v_cache.shape and shape[1:] == (num_kv_heads, page_size, head_dim) and k_cache.is_contiguous() and v_cache.is_contiguous(),
           "caches must be contiguous [pages, kv heads, page size, head_dim]")
-    _need(block_tables.dim() == 2 and block_tables.shape[0] >= rows and row_q_start.numel() >= rows and row_ctx_len.numel() >= rows,
+    at_q, at_k, at_v, at_out = _at(q), _at(k_cache), _at(v_cache), _at(out)
+    ints = (_at(block_tables), _at(row_q_start), _at(row_q_len), _at(row_ctx_len), _at(group_start), _at(group_prefix))
+    table = block_tables.shape
+    _need(len(table) == 2 and table[0] >= rows and row_q_start.numel() >= rows and row_ctx_len.numel() >= rows,
           "block_tables, row_q_start and row_ctx_len need an entry for every row")
     _need(group_start.numel() == groups + 1, "group_start has one entry more than group_prefix")
-    at_q, at_k, at_v, at_out = _at(q), _at(k_cache), _at(v_cache), _at(out)
     _need(q_stride % 8 == 0 and (at_q | at_k | at_v) % 16 == 0, "rows of q and the caches must begin on 16 bytes")
     _need(out.is_contiguous() and at_out % 16 == 0, "the output must be contiguous [tokens, heads, head_dim], 16-byte aligned")
-    _need(shape[0] * num_kv_heads * page_size < 1 << 31, "caches of 2^31 key rows and more are not taken")
+    pages, width = shape[0], table[1]
+    _need(pages * num_kv_heads * page_size < 1 << 31, "caches of 2^31 key rows and more are not taken")
     _need(scale > 0, "the scale of the scores must be positive")
     device = q.device.index
     _need(device == torch.cuda.current_device(), "the tensors must be on the current device")
     if rows == 0:
         return out
-    width = block_tables.shape[1]
-    max_own = width * page_size if max_own is None else max(1, min(max_own, width * page_size))
+    covered = width * page_size
+    max_own = covered if max_own is None else max(1, min(max_own, covered))
     if groups == 0 or max_prefix == 0:                        # nothing is shared
         return decode_attention(q, q_stride, k_cache, v_cache, block_tables, row_q_start, row_q_len, row_ctx_len, out, num_heads, num_kv_heads, head_dim,
                                 page_size, scale, max_ctx=max_own)
-    max_prefix = width * page_size if max_prefix is None else max(1, min(max_prefix, width * page_size))
+    max_prefix = covered if max_prefix is None else max(1, min(max_prefix, covered))
+    stream = _stream()
     # (lengths are planned for in powers of two: a plan serves many steps)
     plan, walk, _ = _shared_plan(device, rows, groups, num_heads, num_kv_heads, head_dim, page_size, 1 << (max_prefix - 1).bit_length(),
-                                 1 << (max_own - 1).bit_length(), shape[0],
-                                 0 if torch.cuda.is_current_stream_capturing() else raw_stream().value or 0)
-    a = _SharedArgs.from_buffer_copy(plan)
-    a.q, a.k_cache, a.v_cache, a.out = at_q, at_k, at_v, at_out
-    a.block_tables, a.row_q_start, a.row_q_len, a.row_ctx_len = _at(block_tables), _at(row_q_start), _at(row_q_len), _at(row_ctx_len)
-    a.group_start, a.group_prefix = _at(group_start), _at(group_prefix)
-    a.q_stride, a.table_stride, a.scale, a.out_f32 = q_stride, width, scale, out.dtype == torch.float32
-    first, second = _shared_libs()
-    at = ctypes.addressof(a)
-    _check(first.mie_prefix_attention(at, _stream()), "shared_prefix_attention (walk)" if walk else "shared_prefix_attention (prefixes)")
-    if not walk:
-        _check(second.mie_decode_attention_shared(at, _stream()), "shared_prefix_attention (own keys)")
+                                 1 << (max_own - 1).bit_length(), pages, 0 if torch.cuda.is_current_stream_capturing() else stream.value or 0)
+    _check(_shared_libs()[0].mie_prefix_attention(_shared_call.pack(at_q, at_k, at_v, *ints, at_out, q_stride, width, f32, scale, walk) + plan, stream),
+           "shared_prefix_attention")
+    global launches
+    launches += 1                                             # (two kernels)
     return out
 
 
@@ -1023,7 +1023,6 @@ def sample(logits: torch.Tensor, temperature, request, position, seed: int, out:
         return out
     if rules is None:
         _need(logits.dtype == torch.float32 and (logits.stride(1) == 1 or vocab <= 1), "logits must be float32, a row's entries side by side")
-        _need(logits.is_cuda and logits.device.index == torch.cuda.current_device(), "logits must be on the current device")
         args = _NO_RULES
     else:
         args = rules.args(logits)
@@ -1034,6 +1033,7 @@ def sample(logits: torch.Tensor, temperature, request, position, seed: int, out:
     _need(logprob is None or logprob.dtype == torch.float32, "logprob must be float32")
     _need(not append or (rules is not None and rules.history is not None), "append goes with rules that have a history")
     _ptr(logits)                                               # (refuses what is not on a CUDA device)
+    _need(rules is not None or logits.device.index == torch.cuda.current_device(), "logits must be on the current device")
     _check(_rules_lib().mie_sample_rules(args, logits.data_ptr(), logits.stride(0), _at(temperature), _at(request), _at(position), seed & ((1 << 64) - 1), _at(out),
                                          _at(logprob), int(append), rows, vocab, host_ptr, turn_ptr, stride, _stream()), "sample with rules")
     return out
