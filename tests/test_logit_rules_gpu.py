@@ -353,3 +353,35 @@ def test_the_same_call_gives_the_same_bits(ops, rows, vocab, width):
         now = (tokens.tolist(), lp.view(torch.int32).tolist())
         first = first or now
         assert now == first
+
+
+@pytest.mark.parametrize("vocab,width", [(700, 300), (50001, 4000), (140001, 9000)])
+@pytest.mark.parametrize("lift", [3.0, 4.5, 30.0, 500.0, None])
+def test_texts_far_above_the_rest(ops, vocab, width, lift):
+    """The text's tokens lead the others by ``lift`` (None: the mask leaves the text's alone): their sum is taken against their own greatest, and the same call
+    gives the same bits."""
+    rows = 3
+    s = Step(ops, rows, vocab, width=width, biases=0, seed=vocab)
+    s.total, s.rep, s.pres = [width, width - 7, width // 2], [1.0, 1.3, 0.8], [0.0, -0.4, 0.7]
+    if lift is not None:
+        for r in range(rows):
+            at = torch.tensor(sorted(set(s.text[s.slot[r]][:s.total[r]])))
+            s.logits[r, at] = s.logits[r, at].abs() + lift
+        s.mask_row = [-1, -1, -1]
+    else:
+        s.allowed = [sorted(set(s.text[s.slot[r]][:s.total[r]])) for r in range(rows)]
+        s.mask = [words_of(a, -(-vocab // 32)) for a in s.allowed]
+        s.mask_row = list(range(rows))
+    s.build()
+    logits, first = s.logits.to(DEV), None
+    for _ in range(10):
+        tokens, lp = s.choose(logits)
+        now = (tokens.tolist(), lp.view(torch.int32).tolist())
+        first = first or now
+        assert now == first
+    for r in range(rows):
+        want, bound = s.row(r)
+        best = int(tokens[r])
+        assert want[best] >= want.max() - 2 * float(bound.max())
+        want_lp = float(torch.log_softmax(want, 0)[best])
+        assert abs(float(lp[r]) - want_lp) <= logprob_bound(want) + float(bound.max()) * 2, (r, float(lp[r]), want_lp)
