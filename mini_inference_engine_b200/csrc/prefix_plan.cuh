@@ -72,7 +72,7 @@ __host__ __device__ __forceinline__ long long prefix_most_slots(int rows, int un
 
 #ifdef __CUDACC__
 // Steps a range, for every lane the same; by a whole warp: lane l weighs up cutting the longest prefix into l + 1 and l + 33 ranges.  A lane holds a
-// group (of up to 32: the host's arithmetic above for more); 13.3 -> 10 us for the two launches of a step of two rows behind 208 keys against every
+// group (of up to 32: the host's arithmetic above for more); 13.3 -> 11.7 us for the two launches of a step of two rows behind 208 keys against every
 // lane reading every group.
 __device__ __forceinline__ int prefix_chunk(const PrefixGroups& p) {
     const int lane = threadIdx.x & 31;
