@@ -2,7 +2,8 @@
 // entry points that differ in where the scratch memory comes from (attention_decode.cu: the
 // caller's; attention_decode_static.cu: a fixed array inside the library) and in whether a window keeps
 // the first keys in sight (attention_decode_kept.cu: the KEEP instances, compiled where a model asks for them), and for rows whose
-// first keys another kernel has dealt with (attention_decode_shared.cu: the SHARED instances).
+// first keys another kernel has dealt with (attention_decode_shared.cu: the SHARED instances), or lie where another row's block table says
+// (attention_decode_through.cu: the THROUGH instances).
 #pragma once
 #include "mma_common.cuh"
 #include "tcgen05_common.cuh"      // mbarrier, TMA copies, bounded waits, the tensor-map encoder
@@ -70,10 +71,13 @@ __device__ __forceinline__ uint32_t swz_tile_off(int row, int chunk) {
 // alone it is not (64 x 2048: 40.0 -> 42.9 us), so the caller chooses (ops.decode_uses_tma).
 // SHARED: a row of a group with a shared prefix walks its own keys only, those from the prefix's end on, and joins them with the partial
 // results that attention_prefix.cu left for the prefix (the splits merge through scratch memory then, never in a cluster).
-template <int D, int NSTAGE, bool TMA, bool KEEP, bool SHARED>
+// THROUGH: a row of such a group walks all of its keys, those of the prefix by the block table of the group's first row.
+enum { DEC_PLAIN = 0, DEC_SHARED = 1, DEC_THROUGH = 2 };
+template <int D, int NSTAGE, bool TMA, bool KEEP, int MODE>
 __global__ void __launch_bounds__(DEC_WARPS * 32)
 decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const DecodeParams p) {
+    constexpr bool SHARED = MODE == DEC_SHARED, THROUGH = MODE == DEC_THROUGH;
     constexpr int DP = D + 8;                    // padded row: ldmatrix rows fall into different banks
     constexpr int KSTEPS = D / 16, NBLK = D / 8;
     constexpr int PARTS = (D + 63) / 64;                           // 64-column parts of a head (TMA layout)
@@ -102,6 +106,8 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     // value (and the queries) afterwards.
     pdl_launch_dependents();
     const int row = blockIdx.z;
+    if (THROUGH && blockIdx.x + blockIdx.y + blockIdx.z == 0)
+        for (int g = threadIdx.x; g < p.groups.groups; g += DEC_WARPS * 32) check_group(p.groups, g, p.report);
     if (p.row_q_len[row] != 1) {                                   // another kernel's row
         pdl_wait();                                                // no block ends before the kernel in front has: later kernels rely on it
         return;
@@ -111,17 +117,23 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     const int kvh = blockIdx.y / p.chunks, chunk = blockIdx.y - kvh * p.chunks;
     const int g0 = chunk * 16, gn = min(16, G - g0);               // query heads of this block within the group
     const int split = blockIdx.x;
-    const int ctx = SHARED ? max(0, min(p.row_ctx_len[row], p.groups.most_keys)) : p.row_ctx_len[row];
+    const int ctx = SHARED || THROUGH ? max(0, min(p.row_ctx_len[row], p.groups.most_keys)) : p.row_ctx_len[row];
     const int token = p.row_q_start[row];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int quad = lane >> 2, tq = lane & 3;
 
     __shared__ PrefixPart s_part;                                  // SHARED: the row's group (rows 0: it has none)
-    int prefix = 0;
-    if (SHARED) {
+    int prefix = 0, leader = row;
+    bool young = false;                                            // THROUGH: a row of the group writes a key of the prefix in this step
+    if (SHARED || THROUGH) {
         for (int g = 0; g < p.groups.groups; ++g) {
             const PrefixPart t = prefix_group(p.groups, g);
-            if (row >= t.first_row && row < t.first_row + t.rows) { prefix = t.keys; break; }
+            if (row >= t.first_row && row < t.first_row + t.rows) {
+                prefix = t.keys;
+                leader = t.first_row;
+                if (THROUGH) for (int r = t.first_row + threadIdx.x; r < t.first_row + t.rows; r += DEC_WARPS * 32) young |= writes_prefix(p.row_q_len[r], p.row_ctx_len[r], prefix);
+                break;
+            }
         }
         if (prefix > ctx || ctx != p.row_ctx_len[row]) {           // a context that ends inside its prefix, or beyond its block table
             if (threadIdx.x == 0 && split == 0 && blockIdx.y == 0) range_report(p.report, MIE_RANGE_POSITION, MIE_K_ATTENTION_DECODE, row, p.row_ctx_len[row]);
@@ -189,15 +201,28 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     const int rest = ntiles - kept_mine, first_page = rest > 0 ? tile_key(kept_mine) >> p.page_shift : 0, page0 = first_page - kept_pages;
     const int n_pages = kept_pages + (rest > 0 ? ((min(ctx, tile_key(ntiles - 1) + DEC_TILE) - 1) >> p.page_shift) - first_page + 1 : 0);
     const int64_t page_limit = p.check_pages > 0 ? p.check_pages : ((int64_t)1 << 40);
+    // THROUGH: whole pages of the prefix lie where the group's first row says; where it ends inside a page, that page's first keys too (tail_page)
+    const int* lead = THROUGH ? p.block_tables + (int64_t)leader * p.table_stride : nullptr;
+    // (a row without own keys has no entry of its own for that page)
+    const bool alone = THROUGH && ctx <= prefix;
+    const int lead_pages = THROUGH ? (alone ? prefix + p.page_size - 1 : prefix) >> p.page_shift : 0, tail0 = lead_pages << p.page_shift;
+    const bool tail = THROUGH && leader != row && prefix > tail0;
+    auto page_of = [&](int e) {
+        if (THROUGH && e < lead_pages) return checked_page(lead[e], page_limit, p.report, MIE_K_ATTENTION_PREFIX, e);
+        return checked_page(table[e], page_limit, p.report, MIE_K_ATTENTION_DECODE, e);
+    };
+    const int tail_page = tail ? checked_page(lead[lead_pages], page_limit, p.report, MIE_K_ATTENTION_PREFIX, lead_pages) : 0;
     for (int i = threadIdx.x; i < min(n_pages, DEC_PAGE_SLOTS); i += DEC_WARPS * 32) {
         const int e = i + (i < kept_pages ? kept_page0 : page0);
-        s_pages[i] = checked_page(table[e], page_limit, p.report, MIE_K_ATTENTION_DECODE, e);
+        s_pages[i] = page_of(e);
     }
     auto page_at = [&](int key, int base) {                        // base: kept_page0 for a kept tile's key, else page0
         const int e = key >> p.page_shift, pi = e - base;
-        return pi < DEC_PAGE_SLOTS ? s_pages[pi] : checked_page(table[e], page_limit, p.report, MIE_K_ATTENTION_DECODE, e);
+        return pi < DEC_PAGE_SLOTS ? s_pages[pi] : page_of(e);
     };
-    __syncthreads();
+    if (THROUGH) {
+        if (__syncthreads_or(young)) pdl_wait();
+    } else __syncthreads();
     constexpr int CHUNKS_PER_ROW = D / 8;                          // 16-byte pieces per key
     const int rows_per_copy = min(p.page_size, DEC_TILE);          // TMA: one copy = one page (or a 64-row piece of it)
     auto load_tile = [&](int t, int stage) {
@@ -227,7 +252,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
             const int r = idx / CHUNKS_PER_ROW, c = (idx - r * CHUNKS_PER_ROW) * 8;
             const int key = k0 + r;
             if (key < ctx && (!SHARED || key >= first_key)) {
-                const int page = page_at(key, base);
+                const int page = tail && key >= tail0 && key < prefix ? tail_page : page_at(key, base);
                 const int64_t src = (((int64_t)page * p.num_kv_heads + kvh) * p.page_size + (key & (p.page_size - 1))) * D + c;
                 cp_async16(kd + r * DP + c, p.k_cache + src);
                 cp_async16(vd + r * DP + c, p.v_cache + src);
@@ -329,6 +354,23 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
             }
             __syncthreads();
         }
+        if (THROUGH && TMA && tail && tile_key(t) < prefix && tile_key(t) + DEC_TILE > tail0) {
+            // the prefix's last keys: a copy by TMA brought the row's own page, whose slots for them may hold anything
+            const int from = max(tail0, tile_key(t)), n = min(prefix, tile_key(t) + DEC_TILE) - from;
+            for (int i = threadIdx.x; i < n * 2 * CHUNKS_PER_ROW; i += DEC_WARPS * 32) {
+                const int which = i / (n * CHUNKS_PER_ROW), at = i - which * n * CHUNKS_PER_ROW, k = at / CHUNKS_PER_ROW, c = at - k * CHUNKS_PER_ROW, r = from + k - tile_key(t);
+                const int64_t src = (((int64_t)tail_page * p.num_kv_heads + kvh) * p.page_size + (from + k - tail0)) * D + c * 8;
+                const uint4 v = __ldcg(reinterpret_cast<const uint4*>((which ? p.v_cache : p.k_cache) + src));
+                *reinterpret_cast<uint4*>(tma_tiles + (size_t)stage * 2 * KV_TILE_BYTES + which * KV_TILE_BYTES + swz_tile_off(r, c)) = v;
+            }
+            __syncthreads();
+        }
+        if (THROUGH && TMA && alone && leader != row && tile_key(t) + DEC_TILE > ctx) {      // behind them, the first row's own values: not this row's
+            const int from = max(0, ctx - tile_key(t));
+            for (int i = threadIdx.x; i < (DEC_TILE - from) * CHUNKS_PER_ROW; i += DEC_WARPS * 32)
+                *reinterpret_cast<uint4*>(tma_tiles + (size_t)stage * 2 * KV_TILE_BYTES + KV_TILE_BYTES + swz_tile_off(from + i / CHUNKS_PER_ROW, i % CHUNKS_PER_ROW)) = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+        }
         if (SHARED && TMA && tile0 + t == 0 && lo < first_key) {   // the first page's slots in front of the own keys may hold anything: 0 * NaN is NaN
             for (int i = threadIdx.x; i < (first_key - lo) * CHUNKS_PER_ROW; i += DEC_WARPS * 32)
                 *reinterpret_cast<uint4*>(tma_tiles + (size_t)stage * 2 * KV_TILE_BYTES + KV_TILE_BYTES + swz_tile_off(i / CHUNKS_PER_ROW, i % CHUNKS_PER_ROW)) = make_uint4(0, 0, 0, 0);
@@ -391,7 +433,8 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float mm = m[i >> 1];
-                        pv[n][i] = mm == -INFINITY ? 0.f : fast_exp2(s[n][i] - mm);
+                        if (MODE == DEC_PLAIN) pv[n][i] = mm == -INFINITY ? 0.f : fast_exp2(s[n][i] - mm);
+                        else pv[n][i] = fast_exp2(s[n][i] - (mm == -INFINITY ? 0.f : mm));      // (scores that are no numbers show in the sum)
                         sum[i >> 1] += pv[n][i];
                     }
                 pf[0] = pack_bf16(pv[0][0], pv[0][1]);
@@ -454,10 +497,10 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
             f[w] = (mm == -INFINITY || m_s[w][g] == -INFINITY) ? 0.f : fast_exp2(m_s[w][g] - mm);
             ll += f[w] * l_s[w][g];
         }
-        const float inv = ll > 0.f ? __frcp_rn(ll) : SHARED && ll != 0.f ? ll : 0.f;
+        const float inv = ll > 0.f ? __frcp_rn(ll) : MODE != DEC_PLAIN && ll != 0.f ? ll : 0.f;
 #pragma unroll
         for (int w = 0; w < DEC_WARPS; ++w) f_s[w][g] = f[w] * inv;
-        c_lse[g] = ll > 0.f ? mm + __log2f(ll) : SHARED && ll != 0.f ? ll : -INFINITY;           // base-2 log-sum-exp of this block's part (SHARED: no number stays none)
+        c_lse[g] = ll > 0.f ? mm + __log2f(ll) : MODE != DEC_PLAIN && ll != 0.f ? ll : -INFINITY;           // base-2 log-sum-exp of this block's part (shared prefixes: no number stays none)
     }
     // Merging the splits inside a cluster: (head, four dimensions) items go round the blocks, item i to
     // block i % S.  Every block sends its normalised partial of an item straight to the item's owner
@@ -642,8 +685,9 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
             acc += w * __ldcg(p.part_o + (base + s2) * D + d);
             wsum += w;
         }
-        if (p.out32) p.out32[((int64_t)token * p.num_heads + head) * D + d] = wsum > 0.f ? acc / wsum : 0.f;
-        else p.out[((int64_t)token * p.num_heads + head) * D + d] = __float2bfloat16_rn(wsum > 0.f ? acc / wsum : 0.f);
+        const float val = wsum > 0.f ? acc / wsum : MODE != DEC_PLAIN && wsum != 0.f ? wsum : 0.f;
+        if (p.out32) p.out32[((int64_t)token * p.num_heads + head) * D + d] = val;
+        else p.out[((int64_t)token * p.num_heads + head) * D + d] = __float2bfloat16_rn(val);
     }
 }
 
@@ -662,7 +706,7 @@ static int make_decode_map(CUtensorMap* map, const void* ptr, uint64_t rows, int
     return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
 }
 
-template <int D, int NSTAGE, bool TMA, bool KEEP, bool SHARED>
+template <int D, int NSTAGE, bool TMA, bool KEEP, int MODE>
 static int launch_decode_stages(const DecodeParams& p, const DecodeMaps& maps, int num_rows, cudaStream_t stream) {
     // at least the four-warp merge buffer (4 x 16 x D float32) must fit
     size_t smem = TMA ? (size_t)NSTAGE * 2 * ((D + 63) / 64) * 8192 + 1024 : (size_t)NSTAGE * 2 * DEC_TILE * (D + 8) * sizeof(bf16);
@@ -671,36 +715,36 @@ static int launch_decode_stages(const DecodeParams& p, const DecodeMaps& maps, i
     DecodeParams pp = p;
     pp.recv_offset = (uint32_t)((smem + 15) & ~size_t(15));
     if (p.cluster) smem = pp.recv_offset + (16 * (D / 4) + 8) * sizeof(float4) + 8 * 16 * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(decode_attention_kernel<D, NSTAGE, TMA, KEEP, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(decode_attention_kernel<D, NSTAGE, TMA, KEEP, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
     const dim3 grid(p.splits, p.num_kv_heads * p.chunks, num_rows);
     const dim3 cluster(p.cluster ? p.splits : 1, 1, 1);
-    return launch_kernel_cluster(decode_attention_kernel<D, NSTAGE, TMA, KEEP, SHARED>, grid, dim3(DEC_WARPS * 32), smem, stream, cluster,
+    return launch_kernel_cluster(decode_attention_kernel<D, NSTAGE, TMA, KEEP, MODE>, grid, dim3(DEC_WARPS * 32), smem, stream, cluster,
                                  maps.k, maps.v, pp);
 }
 
 // Tiles in flight per block.  Few tiles per block (short contexts, many splits): two stages, so that
 // more blocks share an SM and hide one another's latencies.  Many tiles per block: a deeper ring.
-template <int D, bool TMA, bool KEEP, bool SHARED>
+template <int D, bool TMA, bool KEEP, int MODE>
 static int launch_decode_tma(const DecodeParams& p, const DecodeMaps& maps, int num_rows, cudaStream_t stream) {
-    if (p.stages <= 2) return launch_decode_stages<D, 2, TMA, KEEP, SHARED>(p, maps, num_rows, stream);
-    if (p.stages == 3 || D > 64) return launch_decode_stages<D, 3, TMA, KEEP, SHARED>(p, maps, num_rows, stream);
-    return launch_decode_stages<D, 4, TMA, KEEP, SHARED>(p, maps, num_rows, stream);
+    if (p.stages <= 2) return launch_decode_stages<D, 2, TMA, KEEP, MODE>(p, maps, num_rows, stream);
+    if (p.stages == 3 || D > 64) return launch_decode_stages<D, 3, TMA, KEEP, MODE>(p, maps, num_rows, stream);
+    return launch_decode_stages<D, 4, TMA, KEEP, MODE>(p, maps, num_rows, stream);
 }
 
-template <int D, bool KEEP, bool SHARED>
+template <int D, bool KEEP, int MODE>
 static int launch_decode(const DecodeParams& p, const DecodeMaps& maps, int num_rows, cudaStream_t stream) {
     if constexpr (D == 64 || D == 128) {
-        if (maps.use) return launch_decode_tma<D, true, KEEP, SHARED>(p, maps, num_rows, stream);
+        if (maps.use) return launch_decode_tma<D, true, KEEP, MODE>(p, maps, num_rows, stream);
     }
-    return launch_decode_tma<D, false, KEEP, SHARED>(p, maps, num_rows, stream);
+    return launch_decode_tma<D, false, KEEP, MODE>(p, maps, num_rows, stream);
 }
 
 
 // Checks the sizes, fills the parameter block and launches.  With splits > 1 and all three scratch
 // pointers null, the splits (2, 4 or 8) form a thread-block cluster and merge through distributed
 // shared memory; with scratch given, any number of splits merges through it.
-template <bool KEEP, bool SHARED = false>
+template <bool KEEP, int MODE = DEC_PLAIN>
 static int decode_attention_launch(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
                                    const int* block_tables, int table_stride, const int* row_q_start,
                                    const int* row_q_len, const int* row_ctx_len, int num_rows, void* out,
@@ -717,7 +761,8 @@ static int decode_attention_launch(const void* q, int64_t q_stride, const void* 
     if (num_kv_heads <= 0 || num_heads % num_kv_heads) return MIE_ERR_BAD_ARG;
     if (page_size < 1 || (page_size & (page_size - 1))) return MIE_ERR_BAD_ARG;
     const bool cluster = splits > 1 && !part_o && !part_lse && !counters;     // no scratch given: merge inside a cluster
-    if (SHARED && (cluster || !groups || window != 0 || (groups->groups > 0 && (!pre_o || !pre_lse || !pre_chunk)))) return MIE_ERR_BAD_ARG;
+    if (MODE == DEC_SHARED && (cluster || (groups && groups->groups > 0 && (!pre_o || !pre_lse || !pre_chunk)))) return MIE_ERR_BAD_ARG;
+    if (MODE != DEC_PLAIN && (!groups || window != 0)) return MIE_ERR_BAD_ARG;
     if (splits < 1 || (splits > 1 && !cluster && (!part_o || !part_lse || !counters))) return MIE_ERR_BAD_ARG;
     if (cluster && splits != 2 && splits != 4 && splits != 8) return MIE_ERR_BAD_ARG;
     if (num_rows > 65535) return MIE_ERR_TOO_LARGE;
@@ -761,14 +806,14 @@ static int decode_attention_launch(const void* q, int64_t q_stride, const void* 
         p.error = g_error_dev;
     }
     switch (head_dim) {
-        case 16: return launch_decode<16, KEEP, SHARED>(p, maps, num_rows, stream);
-        case 32: return launch_decode<32, KEEP, SHARED>(p, maps, num_rows, stream);
-        case 48: return launch_decode<48, KEEP, SHARED>(p, maps, num_rows, stream);
-        case 64: return launch_decode<64, KEEP, SHARED>(p, maps, num_rows, stream);
-        case 80: return launch_decode<80, KEEP, SHARED>(p, maps, num_rows, stream);
-        case 96: return launch_decode<96, KEEP, SHARED>(p, maps, num_rows, stream);
-        case 112: return launch_decode<112, KEEP, SHARED>(p, maps, num_rows, stream);
-        case 128: return launch_decode<128, KEEP, SHARED>(p, maps, num_rows, stream);
+        case 16: return launch_decode<16, KEEP, MODE>(p, maps, num_rows, stream);
+        case 32: return launch_decode<32, KEEP, MODE>(p, maps, num_rows, stream);
+        case 48: return launch_decode<48, KEEP, MODE>(p, maps, num_rows, stream);
+        case 64: return launch_decode<64, KEEP, MODE>(p, maps, num_rows, stream);
+        case 80: return launch_decode<80, KEEP, MODE>(p, maps, num_rows, stream);
+        case 96: return launch_decode<96, KEEP, MODE>(p, maps, num_rows, stream);
+        case 112: return launch_decode<112, KEEP, MODE>(p, maps, num_rows, stream);
+        case 128: return launch_decode<128, KEEP, MODE>(p, maps, num_rows, stream);
     }
     return MIE_ERR_BAD_ARG;
 }

@@ -9,9 +9,7 @@
 #include "mma_common.cuh"
 #include "tcgen05_common.cuh"
 #include "prefix_plan.cuh"
-#include "range_check.cuh"
 
-#define MIE_K_ATTENTION_PREFIX 16      // this kernel's number in the range report (csrc/range_check.cuh)
 #define PFX_WARPS 4
 #define PFX_PAIRS 64
 #define PFX_TILE 64
@@ -34,15 +32,7 @@ __device__ __forceinline__ float exp2_fast(float x) {      // two units in the l
     return y;
 }
 
-// Does a row's step write a key of its prefix (its newest key is the prefix's last, say)?
-__device__ __forceinline__ bool writes_prefix(int len, int ctx, int keys) { return len > 0 && ctx - len < keys; }
 __device__ __forceinline__ bool writes_prefix(const PrefixParams& p, int row, int keys) { return writes_prefix(p.row_q_len[row], p.row_ctx_len[row], keys); }
-// Reports a group whose rows are none of the step's, or go back, and a prefix that is negative or longer than a block table.
-__device__ __forceinline__ void check_group(const PrefixGroups& p, int g, int* report) {
-    const int a = p.start[g], b = p.start[g + 1], keys = p.prefix[g];
-    if (a < 0 || a > b || b > p.num_rows) range_report(report, MIE_RANGE_ROW, MIE_K_ATTENTION_PREFIX, g, a < 0 || a > b ? a : b);
-    else if (b > a && (keys < 0 || keys > p.most_keys)) range_report(report, MIE_RANGE_POSITION, MIE_K_ATTENTION_PREFIX, a, keys);
-}
 
 template <int D>
 __global__ void __launch_bounds__(PFX_WARPS * 32)
@@ -987,7 +977,7 @@ extern "C" int mie_prefix_layout(SharedArgs* a, int sms) {
         || sms <= 0 || a->page_size < 1 || (a->page_size & (a->page_size - 1))) return MIE_ERR_BAD_ARG;
     const int G = a->num_heads / a->num_kv_heads;
     // Few pairs leave the walk's tiles of 128 empty, and it takes longer to begin; what it gains grows with the keys and values that there are.  Us, walk : the other
-    // two kernels -- 32 heads of 64 on 4, 2 rows behind 208 keys 11.4 : 9.5, 8 behind 2,048 15.4 : 13.1, 16 16.0 : 14.3, 32 19.6 : 30; 32 on 32, 16 rows behind
+    // two kernels -- 32 heads of 64 on 4, 8 rows behind 2,048 15.4 : 13.1, 16 16.0 : 14.3, 32 19.6 : 30; 32 on 32, 16 rows behind
     // 3,000 35.9 : 30.2.  Heads of 128, 32 on 8: 16 rows behind 1,000 19.5 : 17.2, behind 4,000 21.2 : 21.6, behind 16,000 35 : 48, 64 behind 8,000 45 : 84;
     // 32 on 32: 8 rows behind 2,000 21.4 : 23.5, 33 rows in five groups 69 : 74.
     const double bytes = 4.0 * a->num_kv_heads * a->head_dim * (a->most_prefix + 0.5 * a->num_rows * a->most_own);

@@ -11,7 +11,7 @@ struct SharedArgs {
     long long q_stride;
     int table_stride, out_f32;
     float scale;
-    int walk;                                                                     // 1: prefix and own keys in one walk; 0: a kernel for the prefixes, then ...
+    int walk;                                                                     // 2: row by row (attention_decode_through.cu); 1: prefix and own keys in one walk; 0: a kernel for the prefixes, then ...
     int (*own_keys)(const SharedArgs*, cudaStream_t);                             // ... this one for own keys (mie_decode_attention_shared, another library's)
     float* pre_o; float* pre_lse; int* pre_chunk; int* row_info; int* marks;      // scratch: partial results of ranges, how prefixes are cut, a row's results, rows marked
     float* part_o; float* part_lse; int* counters;                                // scratch of the decode kernel (splits > 1); counters and marks are left zero

@@ -8,6 +8,8 @@
 #pragma once
 #include "common.cuh"
 
+#define MIE_K_ATTENTION_PREFIX 16      // what reads prefixes, in the range report (csrc/range_check.cuh)
+
 #define PREFIX_STEP 128
 #define PREFIX_MAX_SPLITS 64
 #define PREFIX_COST_START 3        // what starting and ending an item costs, in steps
@@ -71,6 +73,17 @@ __host__ __device__ __forceinline__ long long prefix_most_slots(int rows, int un
 }
 
 #ifdef __CUDACC__
+#include "range_check.cuh"
+
+// Does a row's step write a key of its prefix (its newest key is the prefix's last, say)?
+__device__ __forceinline__ bool writes_prefix(int len, int ctx, int keys) { return len > 0 && ctx - len < keys; }
+// Reports a group whose rows are none of the step's, or go back, and a prefix that is negative or longer than a block table.
+__device__ __forceinline__ void check_group(const PrefixGroups& p, int g, int* report) {
+    const int a = p.start[g], b = p.start[g + 1], keys = p.prefix[g];
+    if (a < 0 || a > b || b > p.num_rows) range_report(report, MIE_RANGE_ROW, MIE_K_ATTENTION_PREFIX, g, a < 0 || a > b ? a : b);
+    else if (b > a && (keys < 0 || keys > p.most_keys)) range_report(report, MIE_RANGE_POSITION, MIE_K_ATTENTION_PREFIX, a, keys);
+}
+
 // Steps a range, for every lane the same; by a whole warp: lane l weighs up cutting the longest prefix into l + 1 and l + 33 ranges.  A lane holds a
 // group (of up to 32: the host's arithmetic above for more); 13.3 -> 11.7 us for the two launches of a step of two rows behind 208 keys against every
 // lane reading every group.

@@ -61,7 +61,7 @@ def rotates_in_decode(dtype, head_dim: int, ctx) -> bool:
 
 
 # Shared prefixes against ordinary decode attention, which reads a prefix once a row, by the bytes of keys and values that sharing saves a layer (SHARE_MIN_BYTES).
-# Us, ordinary : shared -- 32 heads of 64 on 4, 2 rows behind 208 keys 4.2 : 9.4, 8 behind 2,048 (15 MB) 10.0 : 13.0; 32 of 128 on 8, 64 behind 8,000 (2.1 GB) 376 : 43, 256 behind
+# Us, ordinary : shared -- 32 heads of 64 on 4, 2 rows behind 208 keys 4.2 : 4.3, 8 behind 2,048 (15 MB) 10.0 : 11.1; 32 of 128 on 8, 64 behind 8,000 (2.1 GB) 376 : 43, 256 behind
 # 16,384 1,983 : 110; 32 of 128 on 32, 33 rows in five groups (0.9 GB) 159 : 69.
 SHARE_MIN_BYTES = 48 << 20
 

@@ -533,7 +533,8 @@ def set_prefill_pairs(mode: int = -1) -> None:
 def check_tc_errors() -> None:
     """Raises if a block of a tensor-core kernel gave up a bounded wait (call after a synchronise)."""
     for name, fn in (("attention_prefill_tc", "mie_prefill_attention_tc"), ("attention_decode", "mie_decode_attention"),
-                     ("attention_decode_kept", "mie_decode_attention_kept"), ("attention_decode_shared", "mie_decode_attention_shared"), ("attention_prefix", "mie_prefix_attention")):
+                     ("attention_decode_kept", "mie_decode_attention_kept"), ("attention_decode_shared", "mie_decode_attention_shared"),
+                     ("attention_decode_through", "mie_decode_attention_through"), ("attention_prefix", "mie_prefix_attention")):
         lib = build._libs.get(name)
         if lib is not None and getattr(lib, fn + "_error")():
             getattr(lib, fn + "_clear_error")()
@@ -756,9 +757,19 @@ _shared_call = struct.Struct("10Pqiifi")                       # the fields that
 
 @functools.lru_cache(maxsize=None)
 def _shared_libs():
-    first, second = load("attention_prefix"), load("attention_decode_shared")
-    first.mie_prefix_attention.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
-    return first, second
+    libs = load("attention_prefix"), load("attention_decode_shared"), load("attention_decode_through")
+    for fn in (libs[0].mie_prefix_attention, libs[2].mie_decode_attention_through):
+        fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+    return libs
+
+
+# Rows of a group one by one (each reads the prefix through the first row's block table; the second to ask finds it in L2) against the group at once, by the bytes of keys and values
+# that taking them at once would save, and by the keys that a block would walk.  Us, one by one : at once -- 32 heads of 64 on 4, 2 rows behind 208 4.3 : 9.9, behind 2,000 (2 MB)
+# 6.3 : 11.6, behind 8,000 (8 MB, 1,000 keys a block) 20.4 : 15.5, 8 behind 2,048 (14 MB) 11.1 : 13.0, 16 (30 MB) 20.1 : 14.0; 32 of 128 on 8, 2 behind 4,000 (16 MB) 15.2 : 19.1,
+# 8 behind 1,000 (27 MB) 12.9 : 14.6, 4 behind 4,000 (47 MB) 18.1 : 19.0, 16 behind 1,000 (59 MB) 19.3 : 17.1; 32 on 32, 2 behind 2,000 (31 MB) 17.8 : 19.8, 4 (94 MB) 30 : 21;
+# 24 of 96 on 4, 12 behind 999 (16 MB) 12.2 : 14.6.
+PREFIX_ONE_BY_ONE_BYTES = (20 << 20, 48 << 20)                # heads below 96, others
+PREFIX_ONE_BY_ONE_KEYS = 640
 
 
 @functools.lru_cache(maxsize=256)
@@ -781,19 +792,31 @@ def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_hea
             scratch("prefix_rows", 2 * rows, torch.int32), scratch("prefix_marks", rows * num_kv_heads, torch.int32, zero=True)]
     for name, t in zip(("pre_o", "pre_lse", "pre_chunk", "row_info", "marks"), kept):
         setattr(a, name, t.data_ptr())
-    if not a.walk:                                            # the rows' own keys by the decode kernel behind
+    units = num_kv_heads * -(-(num_heads // num_kv_heads) // 16)
+    tma_ok = head_dim in (64, 128) and page_size >= 8
+    merge = "scratch"
+    splits, how, min_part_tiles = decode_plan(rows, units, max_prefix + max_own, tma_ok, head_dim)
+    if ((rows - 1) * max_prefix * num_kv_heads * head_dim * 4 <= PREFIX_ONE_BY_ONE_BYTES[head_dim >= 96]
+            and max_prefix + max_own <= PREFIX_ONE_BY_ONE_KEYS * splits):
+        a.walk, most = 2, max_prefix + max_own
+        a.splits, merge, a.min_part_tiles = splits, how, min_part_tiles
+        if merge == "cluster":
+            a.min_part_tiles = 0
+        blocks = rows * units * a.splits
+        a.tma = tma_ok and (merge == "scratch" or decode_uses_tma(blocks, head_dim))
+        a.stages = decode_stages(blocks, most, a.splits, bool(a.tma), head_dim, clustered=merge == "cluster")
+    elif not a.walk:                                          # the rows' own keys by the decode kernel behind
         a.own_keys = ctypes.cast(_shared_libs()[1].mie_decode_attention_shared, ctypes.c_void_p).value
-        units = num_kv_heads * -(-(num_heads // num_kv_heads) // 16)
-        tma_ok = head_dim in (64, 128) and page_size >= 8
         a.splits, a.min_part_tiles = own_keys_plan(rows, units, max_own, tma_ok, head_dim)
         blocks = rows * units * a.splits
         a.tma = tma_ok and decode_uses_tma(blocks, head_dim)
         a.stages = decode_stages(blocks, max_own, a.splits, bool(a.tma), head_dim, clustered=False)
-        if a.splits > 1:
-            more = [scratch("decode_part_o", rows * num_heads * a.splits * head_dim), scratch("decode_part_lse", rows * num_heads * a.splits),
-                    scratch("decode_counters", rows * units, torch.int32, zero=True)]
-            a.part_o, a.part_lse, a.counters = (t.data_ptr() for t in more)
-            kept += more
+    if a.splits > 1 and merge == "scratch":
+        more = [scratch("decode_part_o", rows * num_heads * a.splits * head_dim), scratch("decode_part_lse", rows * num_heads * a.splits),
+                scratch("decode_counters", rows * units, torch.int32, zero=True)]
+        for name, t in zip(("part_o", "part_lse", "counters"), more):
+            setattr(a, name, t.data_ptr())
+        kept += more
     return bytes(a)[_shared_call.size:], a.walk, kept
 
 
@@ -822,8 +845,8 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     overlap; rows of no group share nothing.  A row's context (``row_ctx_len``) includes its prefix.  ``max_prefix`` and ``max_own``: bounds on the
     prefixes and on the keys behind them, for planning (a captured step's may be shorter); without them the block table's width bounds both.
 
-    Two launches: the keys (prefixes in tiles of (row, head) pairs, and the rows' own), then what joins a row's partial results.  Rows with more than
-    one new token are skipped.  Slots of a row's last page behind its context must hold
+    Two launches: the keys (prefixes in tiles of (row, head) pairs, and the rows' own), then what joins a row's partial results; one, row by row, where
+    little is shared (``PREFIX_ONE_BY_ONE_BYTES``).  Rows with more than one new token are skipped.  Slots of a row's last page behind its context must hold
     finite values (see ``decode_uses_tma``).  Launches captured on any streams share scratch memory, as those of other kernels here do: their graphs are replayed one
     behind the other."""
     bf16, i32, f32 = torch.bfloat16, torch.int32, out.dtype == torch.float32
@@ -863,8 +886,11 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     # (lengths are planned for in powers of two: a plan serves many steps)
     plan, walk, _ = _shared_plan(device, rows, groups, num_heads, num_kv_heads, head_dim, page_size, 1 << (max_prefix - 1).bit_length(),
                                  1 << (max_own - 1).bit_length(), pages, 0 if torch.cuda.is_current_stream_capturing() else stream.value or 0)
-    _check(_shared_libs()[0].mie_prefix_attention(_shared_call.pack(at_q, at_k, at_v, *ints, at_out, q_stride, width, f32, scale, walk) + plan, stream),
-           "shared_prefix_attention")
+    args = _shared_call.pack(at_q, at_k, at_v, *ints, at_out, q_stride, width, f32, scale, walk) + plan
+    if walk == 2:
+        _check(_shared_libs()[2].mie_decode_attention_through(args, stream), "shared_prefix_attention (row by row)")
+        return out
+    _check(_shared_libs()[0].mie_prefix_attention(args, stream), "shared_prefix_attention")
     global launches
     launches += 1                                             # (two kernels)
     return out

@@ -8,10 +8,20 @@ from test_shared_prefix_gpu import DEV, Case, ops  # noqa: F401  (the fixture)
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def at_once(monkeypatch):
+    """Groups are taken at once however little they share."""
+    from mini_inference_engine_b200.kernels import ops
+    monkeypatch.setattr(ops, "PREFIX_ONE_BY_ONE_BYTES", (-1, -1))
+    ops._shared_plan.cache_clear()
+    yield
+    ops._shared_plan.cache_clear()
+
+
 def walks(ops, c, **hints):
     """The case, run by the walk: its plan says so."""
     return ops._shared_plan(torch.cuda.current_device(), c.rows, c.group_prefix.numel(), c.H, c.G, c.D, c.page, hints["max_prefix"], hints["max_own"],
-                            c.cache.shape[1], 0)[1]
+                            c.cache.shape[1], 0)[1] == 1
 
 
 @pytest.mark.parametrize("D", [64, 128])
