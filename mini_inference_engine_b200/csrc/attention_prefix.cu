@@ -1,7 +1,8 @@
 // Attention of decoding rows over keys that they share: every (row, query head) pair of a group against the group's prefix, computed once for
 // all rows, in bfloat16 with float32 scores, softmax statistics and sums.  Leaves, for a pair and a range of keys,
 //     o = sum_j 2^(s_j - m) v_j / l   and   m + log2 l,     l = sum_j 2^(s_j - m),  s_j = scale log2(e) q . k_j
-// which a kernel behind joins with the pair's other ranges.  prefix_plan.cuh says how the work is cut.
+// which a kernel behind joins with the pair's other ranges.  prefix_plan.cuh says how the work is cut.  (Where little is shared the rows go one by one:
+// attention_decode_through.cu.)
 //
 // Two ways.  Heads of 64 and 128 on pages of 8 positions or more: tcgen05, prefix and own keys in one walk, below.  Any head size in steps of 16: a
 // block takes 64 pairs, 16 a warp (mma.sync m16n8k16), and walks its range of the prefix in tiles of 64 keys that arrive by cp.async, two in flight; a tile
@@ -855,7 +856,22 @@ prefix_join_kernel(const WalkParams wp, bf16* __restrict__ out, float* __restric
     const int row = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
     const int2 info = __ldcg(wp.row_info + row);
     const int S = min(info.y, 2 * PREFIX_MAX_SPLITS);
-    if (p.row_q_len[row] != 1 || p.row_ctx_len[row] <= 0 || head >= p.num_heads) return;      // (a row of more than one new token is left alone)
+    if (p.row_q_len[row] != 1 || head >= p.num_heads) return;      // (a row of more than one new token is left alone)
+    const int64_t at = ((int64_t)p.row_q_start[row] * p.num_heads + head) * D + lane * E;
+    auto write = [&](const float* acc) {
+        if (out32) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) out32[at + e] = acc[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(out + at + e) = __floats2bfloat162_rn(acc[e], acc[e + 1]);
+        }
+    };
+    if (p.row_ctx_len[row] <= 0) {                         // no keys at all: no range may have been planned for the row
+        const float none[E] = {};
+        write(none);
+        return;
+    }
     if (S <= 0 || (int64_t)info.x + S > p.most_slots) return;
     const int kvh = head / (p.num_heads / p.num_kv_heads);
     int* mark = wp.marks + (int64_t)row * p.num_kv_heads + kvh;
@@ -930,14 +946,7 @@ prefix_join_kernel(const WalkParams wp, bf16* __restrict__ out, float* __restric
         __syncwarp();
         if (lane == 0) atomicSub(mark, 1);                 // the last of the key head's query heads leaves it 0
     }
-    const int64_t at = ((int64_t)p.row_q_start[row] * p.num_heads + head) * D + lane * E;
-    if (out32) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) out32[at + e] = acc[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(out + at + e) = __floats2bfloat162_rn(acc[e], acc[e + 1]);
-    }
+    write(acc);
 }
 
 static int prefix_map(CUtensorMap* map, const void* ptr, uint64_t rows, int head_dim, int box_rows) {

@@ -21,7 +21,7 @@
 // memory (the maximum of x' and the sum of exp(x' - maximum), in float32, joined pairwise).
 //
 // Bound: the bytes of the logits (read once, written once by `apply`) for many rows, the chain row -> text -> table -> logits -> list -> cluster for few:
-// slices are cut so that all blocks run at once where that is possible (rules_parts).
+// slices are cut by what a round of blocks costs (rules_cut).
 #include <limits.h>
 
 #include "choice.cuh"

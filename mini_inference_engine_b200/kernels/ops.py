@@ -842,7 +842,7 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     ``group_start`` int32 [groups + 1]: group g is the rows group_start[g] .. group_start[g + 1] - 1; ``group_prefix`` int32 [groups]: its rows share that
     many first keys, which lie where the block table of the group's FIRST row says (the other rows' table entries for them are not followed, but
     where a prefix ends inside a page every row's own entry for that page holds its keys from there on).  0: the rows share nothing.  Groups do not
-    overlap; rows of no group share nothing.  A row's context (``row_ctx_len``) includes its prefix.  ``max_prefix`` and ``max_own``: bounds on the
+    overlap; rows of no group share nothing.  A row's context (``row_ctx_len``) includes its prefix; a row without any keys gives zeros.  ``max_prefix`` and ``max_own``: bounds on the
     prefixes and on the keys behind them, for planning (a captured step's may be shorter); without them the block table's width bounds both.
 
     Two launches: the keys (prefixes in tiles of (row, head) pairs, and the rows' own), then what joins a row's partial results; one, row by row, where

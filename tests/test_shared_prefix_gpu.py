@@ -303,3 +303,17 @@ def test_refusals(ops):
     refused("16 bytes", qkv=c.qkv[:, 1:])
     refused("every row", ctx_len=c.ctx_len[:2])
     c.check(c.run(ops))
+
+
+@pytest.mark.parametrize("D", [64, 128, 80])
+@pytest.mark.parametrize("groups,own", [([(3, 0), (2, 50)], [0, 5, 0, 0, 3]), ([(2, 0), (9, 0)], [0] * 11), ([(9, 0), (1, 0)], [0, 0, 0, 300, 0, 0, 1, 0, 0, 0])])
+def test_rows_without_any_keys_give_zeros(ops, D, groups, own):
+    c = Case(groups, own, 32, 2, D, 16, seed=D)
+    other = Case([(20, 300)], 100, 32, 2, D, 16, seed=1)
+    for hints in (c.hints, dict(max_prefix=64, max_own=c.hints["max_own"])):
+        other.run(ops, **other.hints)                         # (other results in the scratch memory)
+        out = c.run(ops, **hints)
+        c.check(out, [r for r in range(c.rows) if c.ctx[r]])
+        for r in range(c.rows):
+            if not c.ctx[r]:
+                assert (out[r] == 0).all(), r
