@@ -206,11 +206,24 @@ prefix_attention_kernel(const PrefixParams p) {
     }
 }
 
+// The shared memory of a kernel, asked for once a device (`granted`: the kernel's devices).
+template <typename K>
+static int grant_shared(K kernel, size_t bytes, unsigned long long& granted) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return (int)e;
+    if (device <= 63 && (__atomic_load_n(&granted, __ATOMIC_RELAXED) >> device & 1)) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device <= 63) __atomic_fetch_or(&granted, 1ull << device, __ATOMIC_RELAXED);
+    return (int)e;
+}
+
 template <int D>
 static int launch_prefix(const PrefixParams& p, long long items, cudaStream_t stream) {
     const size_t smem = (size_t)4 * PFX_TILE * (D + 8) * sizeof(bf16);
-    cudaError_t e = cudaFuncSetAttribute(prefix_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
+    static unsigned long long granted = 0;
+    const int rc = grant_shared(prefix_attention_kernel<D>, smem, granted);
+    if (rc) return rc;
     return launch_kernel(prefix_attention_kernel<D>, dim3((unsigned)items), dim3(PFX_WARPS * 32), smem, stream, p);
 }
 
@@ -967,8 +980,8 @@ static int launch_walk(WalkParams p, void* out, bool out_f32, long long items, c
     const uint64_t rows = (uint64_t)p.b.num_pages * p.b.num_kv_heads * p.b.page_size;
     const int box = p.b.page_size < PT_KEYS ? p.b.page_size : PT_KEYS;
     if ((rc = prefix_map(&mk, p.b.k_cache, rows, D, box)) || (rc = prefix_map(&mv, p.b.v_cache, rows, D, box))) return rc;
-    const cudaError_t e = cudaFuncSetAttribute(prefix_walk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PT_SMEM<D>);
-    if (e != cudaSuccess) return (int)e;
+    static unsigned long long granted = 0;
+    if ((rc = grant_shared(prefix_walk_kernel<D>, PT_SMEM<D>, granted))) return rc;
     if ((rc = launch_kernel(prefix_walk_kernel<D>, dim3((unsigned)items), dim3(PT_THREADS), PT_SMEM<D>, stream, mk, mv, p))) return rc;
     return launch_kernel(prefix_join_kernel<D>, dim3(p.b.groups.num_rows, (p.b.num_heads + JOIN_WARPS - 1) / JOIN_WARPS), dim3(JOIN_WARPS * 32), 0, stream, p,
                          out_f32 ? nullptr : (bf16*)out, out_f32 ? (float*)out : nullptr);

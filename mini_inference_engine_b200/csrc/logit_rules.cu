@@ -431,12 +431,13 @@ struct RuleCut { int parts, threads; };
 static RuleCut rules_cut(int rows, int vocab, int width, bool choose) {
     RuleCut best = {1, 1024};
     double least = 1e30;
+    const int sms = device_sm_count();
     for (int threads = 256; threads <= 1024; threads *= 2) {
         for (int parts = 1; parts <= (choose ? RULES_MAX_PARTS : 64); parts *= 2) {
             const int per = ((vocab + parts - 1) / parts + 3) & ~3;
             int fit = (int)(232448 / ((size_t)rules_table(per) * 4 + 2048));
             if (fit > RULES_SM_THREADS / threads) fit = RULES_SM_THREADS / threads;
-            const int64_t places = (int64_t)fit * device_sm_count(), rounds = ((int64_t)rows * parts + places - 1) / places;
+            const int64_t places = (int64_t)fit * sms, rounds = ((int64_t)rows * parts + places - 1) / places;
             const double cost = (double)rounds * (2.0 + 0.4 * (threads / 256 - 1) + 0.3 * per / (16.0 * threads) + 3.0 * (width / 2) / (8.0 * threads));
             if (cost < least) { least = cost; best = RuleCut{parts, threads}; }
         }
@@ -448,8 +449,16 @@ template <int T>
 static int launch_rules_threads(const RuleParams& p, bool choose, int parts, cudaStream_t stream) {
     const size_t smem = p.history || p.bias_tokens ? (size_t)p.table * 4 : 0;
     auto kernel = !choose ? logit_rules_kernel<T, false, false> : parts > 1 ? logit_rules_kernel<T, true, true> : logit_rules_kernel<T, true, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RULES_TABLE * 4);
+    static unsigned long long allowed[3] = {0, 0, 0};      // a kernel's devices on which it may have that much shared memory
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
+    unsigned long long* on = &allowed[!choose ? 0 : parts > 1 ? 1 : 2];
+    if (device > 63 || !(__atomic_load_n(on, __ATOMIC_RELAXED) >> device & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RULES_TABLE * 4);
+        if (e != cudaSuccess) return (int)e;
+        if (device <= 63) __atomic_fetch_or(on, 1ull << device, __ATOMIC_RELAXED);
+    }
     return launch_kernel_cluster(kernel, dim3(parts, p.rows), dim3(T), smem, stream, dim3(choose ? parts : 1, 1, 1), p);
 }
 

@@ -859,7 +859,8 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     _need(head_dim % 16 == 0 and 16 <= head_dim <= 128, "attention over shared prefixes takes head sizes in multiples of 16 from 16 to 128")
     _need(page_size >= 1 and page_size & (page_size - 1) == 0, "the page size must be a power of two")
     shape = k_cache.shape
-    _need(len(shape) == 4 and shape == v_cache.shape and shape[1:] == (num_kv_heads, page_size, head_dim) and k_cache.is_contiguous() and v_cache.is_contiguous(),
+    pages = shape[0] if shape else 0
+    _need(shape == (pages, num_kv_heads, page_size, head_dim) and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous(),
           "caches must be contiguous [pages, kv heads, page size, head_dim]")
     at_q, at_k, at_v, at_out = _at(q), _at(k_cache), _at(v_cache), _at(out)
     ints = (_at(block_tables), _at(row_q_start), _at(row_q_len), _at(row_ctx_len), _at(group_start), _at(group_prefix))
@@ -869,10 +870,10 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     _need(group_start.numel() == groups + 1, "group_start has one entry more than group_prefix")
     _need(q_stride % 8 == 0 and (at_q | at_k | at_v) % 16 == 0, "rows of q and the caches must begin on 16 bytes")
     _need(out.is_contiguous() and at_out % 16 == 0, "the output must be contiguous [tokens, heads, head_dim], 16-byte aligned")
-    pages, width = shape[0], table[1]
+    width = table[1]
     _need(pages * num_kv_heads * page_size < 1 << 31, "caches of 2^31 key rows and more are not taken")
     _need(scale > 0, "the scale of the scores must be positive")
-    device = q.device.index
+    device = q.get_device()
     _need(device == torch.cuda.current_device(), "the tensors must be on the current device")
     if rows == 0:
         return out
@@ -1032,14 +1033,14 @@ def sample(logits: torch.Tensor, temperature, request, position, seed: int, out:
     rows, vocab = logits.shape
     _need(temperature.dtype == torch.float32 and request.dtype == torch.int64 and position.dtype == torch.int32
           and out.dtype == torch.int32, "sampling argument types")
-    host_ptr, stride = ctypes.c_void_p(0), 0
+    host_ptr, stride = None, 0
     if host_out is not None:
         _need(host_out.dtype == torch.int32 and host_out.dim() == 2 and host_out.is_pinned() and host_out.is_contiguous()
               and host_out.shape[1] >= rows, "host_out must be a pinned int32 tensor [turns, n >= rows]")
         if host_turn is not None:
             _need(host_turn.is_cuda and host_turn.dtype == torch.int32 and host_turn.numel() >= 1, "host_turn must be a device int32 tensor")
         host_ptr, stride = ctypes.c_void_p(host_out.data_ptr()), host_out.shape[1]
-    turn_ptr = _ptr(host_turn) if host_out is not None else ctypes.c_void_p(0)
+    turn_ptr = _ptr(host_turn) if host_out is not None else None
     if rules is None and logprob is None:
         _need(not append, "append goes with rules")
         _need(logits.dtype == torch.float32 and logits.is_contiguous(), "logits must be contiguous float32")
@@ -1053,9 +1054,9 @@ def sample(logits: torch.Tensor, temperature, request, position, seed: int, out:
     else:
         args = rules.args(logits)
     _need(vocab > 0, "an empty vocabulary has no token")
-    for t, name in ((temperature, "temperature"), (request, "request"), (position, "position"), (out, "out"), (logprob, "logprob")):
-        if t is not None:
-            _need(t.is_contiguous() and t.numel() >= rows, f"{name} must be contiguous, one entry a row")
+    _need(temperature.is_contiguous() and temperature.numel() >= rows and request.is_contiguous() and request.numel() >= rows
+          and position.is_contiguous() and position.numel() >= rows and out.is_contiguous() and out.numel() >= rows
+          and (logprob is None or (logprob.is_contiguous() and logprob.numel() >= rows)), "temperature, request, position, out and logprob must be contiguous, one entry a row")
     _need(logprob is None or logprob.dtype == torch.float32, "logprob must be float32")
     _need(not append or (rules is not None and rules.history is not None), "append goes with rules that have a history")
     _ptr(logits)                                               # (refuses what is not on a CUDA device)
