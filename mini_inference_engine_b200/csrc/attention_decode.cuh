@@ -715,15 +715,8 @@ static int launch_decode_stages(const DecodeParams& p, const DecodeMaps& maps, i
     DecodeParams pp = p;
     pp.recv_offset = (uint32_t)((smem + 15) & ~size_t(15));
     if (p.cluster) smem = pp.recv_offset + (16 * (D / 4) + 8) * sizeof(float4) + 8 * 16 * sizeof(float);
-    static int granted[64] = {0};                                  // shared memory that this kernel may have, by device
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
+    cudaError_t e = cudaFuncSetAttribute(decode_attention_kernel<D, NSTAGE, TMA, KEEP, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    if (device > 63 || __atomic_load_n(&granted[device], __ATOMIC_RELAXED) < (int)smem) {
-        e = cudaFuncSetAttribute(decode_attention_kernel<D, NSTAGE, TMA, KEEP, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return (int)e;
-        if (device <= 63) __atomic_store_n(&granted[device], (int)smem, __ATOMIC_RELAXED);
-    }
     const dim3 grid(p.splits, p.num_kv_heads * p.chunks, num_rows);
     const dim3 cluster(p.cluster ? p.splits : 1, 1, 1);
     return launch_kernel_cluster(decode_attention_kernel<D, NSTAGE, TMA, KEEP, MODE>, grid, dim3(DEC_WARPS * 32), smem, stream, cluster,
