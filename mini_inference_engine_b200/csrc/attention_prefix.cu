@@ -672,6 +672,13 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             seen_lo = at + (prefix - own_begin);
             seen_hi = at + (plan.ctx[in_tile] - own_begin);
         }
+        // The chains take turns at the exponentials of the steps that both take part in (118 us for 256 rows without): half n of chain 0 behind half n - 1 of chain 1,
+        // that behind half n of chain 0.  Every half takes its turn, one without keys too: a chain that went on without would complete a second phase of its
+        // barrier, and the other, if it had not asked for the first by then, would wait for a parity that does not come again.
+        auto take_turn = [&](int j, int n) {
+            const int turn = u == 0 ? n - 1 : n;
+            return !(both && j < npre) || turn < 0 || __all_sync(0xffffffffu, mbar_wait(&exp_done[u ^ 1], turn & 1, abort_p)) != 0;
+        };
         float m_run = -INFINITY, l_run = 0.f;
         int used = 0;
         for (int j = 0; j < J && ok; ++j) {
@@ -727,10 +734,7 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 }
                 // (where P lies over S, scores that are here say that the product which read the P before them is done)
                 if (!OVER && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (n - 1) & 1, abort_p))) { ok = false; break; }
-                if (both && j < npre) {                    // the chains take turns at the exponentials of the steps that both take part in (118 us for 256 rows without)
-                    const int turn = u == 0 ? n - 1 : n;
-                    if (turn >= 0 && !__all_sync(0xffffffffu, mbar_wait(&exp_done[u ^ 1], turn & 1, abort_p))) { ok = false; break; }
-                }
+                if (!take_turn(j, n)) { ok = false; break; }
                 const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
                 float sm[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -751,6 +755,7 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             } else {                                       // own keys of other warps' rows (of a prefix: none behind its end): weights of zero
                 if (!OVER && lane == 0) mbar_arrive(&s_free[u]);
                 if (!OVER && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[u], (n - 1) & 1, abort_p))) { ok = false; break; }
+                if (!take_turn(j, n)) { ok = false; break; }
                 if (both && j < npre && lane == 0) mbar_arrive(&exp_done[u]);
                 uint32_t none[16];
 #pragma unroll
