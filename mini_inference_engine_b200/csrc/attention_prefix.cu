@@ -451,18 +451,10 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const int npre = max(0, min(J, pre_steps - x0));       // the first npre of this item's steps are the prefix's
     // own slots go by lists, one a tile of pairs: list l's begin at list0[l], and take list_steps[l] steps, turn by turn while both have some
     const int list0[2] = {0, both ? plan.own_first[half] : 0}, list_end[2] = {both ? plan.own_first[half] : plan.own_first[rows], plan.own_first[rows]};
-    const int steps0 = (list_end[0] + W - 1) >> ws, steps1 = both ? (list_end[1] - list0[1] + W - 1) >> ws : 0, turns = min(steps0, steps1);
-    struct OwnStep { int list, k; };                       // the k-th step of a list
-    auto own_step = [&](int j) {
-        const int x = x0 + j - pre_steps;
-        if (x < 2 * turns) return OwnStep{x & 1, x >> 1};
-        return OwnStep{steps1 > steps0 ? 1 : 0, x - turns};
-    };
-    // does chain c take part in step j?
-    auto active = [&](int c, int j) {
-        if (!both) return (j & 1) == c;
-        return j < npre || own_step(j).list == c;
-    };
+    const int steps0 = (list_end[0] + W - 1) >> ws, steps1 = both ? (list_end[1] - list0[1] + W - 1) >> ws : 0;
+    const WalkSteps steps = {J, npre, x0 - pre_steps, steps0, steps1, both};
+    auto own_step = [&](int j) { return walk_own_step(steps, j); };
+    auto active = [&](int c, int j) { return walk_takes_part(steps, c, j); };
     // the row of the tile of rows that an own slot belongs to
     auto owner = [&](int slot) {
         int lo = 0, hi = rows - 1;                         // the last row whose first slot is not behind it
@@ -612,7 +604,8 @@ prefix_walk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             };
             auto scores = [&](int j, int h) {              // S of half h of step j, once its keys are here
                 const int st = j % STAGES;
-                if (h == 0) ok = wait_for(&k_full[st], (j / STAGES) & 1);
+                // (behind steps of the other chain alone: once that is done with all of its own, what lay here before has come; the values' waits lie behind this one)
+                if (h == 0) ok = (!walk_behind_other(steps, mu, j, STAGES) || wait_for(&o_full[mu ^ 1], 0)) && wait_for(&k_full[st], (j / STAGES) & 1);
                 if (!ok) return;
                 tc_fence_after();
                 if (issuer) {

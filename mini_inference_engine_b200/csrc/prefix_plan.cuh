@@ -29,6 +29,27 @@ __host__ __device__ __forceinline__ void prefix_range(int steps, int splits, int
     n = base + (s < more ? 1 : 0);
 }
 
+// The steps of an item of the walk over prefix and own keys (attention_prefix.cu): J of them, the first npre the prefix's.  With two tiles of pairs (`both`) a chain owns a tile:
+// both chains take part in a step of the prefix; the own keys of a tile are a list (steps0 and steps1 steps), and the lists take turns while both have steps left.
+// With one tile the chains take the steps in turns.
+struct WalkSteps { int J, npre, own0, steps0, steps1; bool both; };        // own0 + j: own step j's place among those of the whole walk
+struct OwnStep { int list, k; };                                           // the k-th step of a list
+__host__ __device__ __forceinline__ OwnStep walk_own_step(const WalkSteps& w, int j) {
+    const int x = w.own0 + j, turns = min(w.steps0, w.steps1);
+    if (x < 2 * turns) return OwnStep{x & 1, x >> 1};
+    return OwnStep{w.steps1 > w.steps0 ? 1 : 0, x - turns};
+}
+// Does chain c take part in step j?
+__host__ __device__ __forceinline__ bool walk_takes_part(const WalkSteps& w, int c, int j) {
+    if (!w.both) return (j & 1) == c;
+    return j < w.npre || walk_own_step(w, j).list == c;
+}
+// Step j lies where step j - stages lay.  A chain that took part in that one knows that its keys and values have come; where the other chain alone did (the lists' turns have just
+// ended), a wait for step j's could take the phase before it for its own.  The other chain has no step behind j then.
+__host__ __device__ __forceinline__ bool walk_behind_other(const WalkSteps& w, int c, int j, int stages) {
+    return w.both && j - stages >= w.npre && walk_own_step(w, j - stages).list != c;
+}
+
 __host__ __device__ __forceinline__ PrefixPart prefix_group(const PrefixGroups& p, int g) {
     PrefixPart t = {};
     const int a = max(0, min(p.start[g], p.num_rows)), b = max(a, min(p.start[g + 1], p.num_rows));
