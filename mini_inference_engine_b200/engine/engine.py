@@ -149,11 +149,10 @@ class LLMEngine:
         self._portion_slot = most
         self._sampled = torch.zeros(most + 8, dtype=torch.int32, device=self.device)   # the last step's tokens, on the device
         self._turn = 0
-        self._in_flight = None
         self.rules = RuleBook(self.device, self.cfg.max_model_len, self.vocab_size)
         self._logprobs = self._pinned_logprobs = None        # made when a request first asks for them
         self.can_share = self.cache.can_share() and not layout.state         # whether requests can share pages
-        self.prefixes: list = []                 # the prefixes that requests may begin with (``add_prefix``)
+        self._host_state()
         self._shared_graphs: dict = {}           # (bucket, context bound) -> captured decode step over shared prefixes, or None: it has run once
         self._bytes_per_key = max((2 * n.num_kv_heads * n.head_dim * torch.empty((), dtype=dtype).element_size()
                                    for _, n in layout.kv.values()), default=0)
@@ -173,6 +172,12 @@ class LLMEngine:
             self._capture_cuda_graphs()
         if self.cfg.warm_up_prompt_step:
             self._warm_up_prompt_step()
+
+    def _host_state(self) -> None:
+        """What the host keeps between steps."""
+        self._in_flight = None
+        self._unreported: list = []              # requests that have ended and that no step has returned yet
+        self.prefixes: list = []                 # the prefixes that requests may begin with (``add_prefix``)
 
     @torch.inference_mode()
     def _warm_up_prompt_step(self):
@@ -453,20 +458,23 @@ class LLMEngine:
         if not self.cache.can_reserve(p.cache, len(p.token_ids), watermark=self.scheduler.watermark):
             raise ValueError(f"a prefix of {pages} pages, {min(q.num_free for q in self.cache.pools)} free")
         try:
-            arr = np.asarray(p.token_ids, dtype=np.int32)
-            for a in range(0, arr.size, self.cfg.max_num_batched_tokens):
-                part = arr[a:a + self.cfg.max_num_batched_tokens]
-                self.cache.reserve(p.cache, part.size)
-                ctx = self.runner.builder.build([self.runner.make_row(p.cache, part, ())])
-                ctx.token_feedback = self._sampled
-                self.model.step(ctx)
-                self.cache.advance(p.cache, part.size)
+            self._compute_prefix(p)
         except BaseException:
             self.cache.free(p.cache)
             raise
         self.cache.pin(p.cache)
         self.prefixes.append(p)
         return p
+
+    def _compute_prefix(self, p: Prefix) -> None:
+        arr = np.asarray(p.token_ids, dtype=np.int32)
+        for a in range(0, arr.size, self.cfg.max_num_batched_tokens):
+            part = arr[a:a + self.cfg.max_num_batched_tokens]
+            self.cache.reserve(p.cache, part.size)
+            ctx = self.runner.builder.build([self.runner.make_row(p.cache, part, ())])
+            ctx.token_feedback = self._sampled
+            self.model.step(ctx)
+            self.cache.advance(p.cache, part.size)
 
     def release_prefix(self, prefix: Prefix) -> None:
         """No further request begins with ``prefix``; its pages go back when the last that does has ended."""
@@ -520,25 +528,25 @@ class LLMEngine:
         return seq
 
     # ------------------------------------------------------------------ grammars
-    def _ask_grammars(self) -> list:
-        """Before a step: what every live request's grammar allows next.  A grammar reads the tokens so far, so the step in flight is read first.  Returns
-        the requests that end here (their grammar allows nothing), beside those that ended with the step that was read."""
+    def _ask_grammars(self) -> None:
+        """Before a step: what every live request's grammar allows next.  A grammar reads the tokens so far, so the step in flight is read first.  The requests
+        that end here (their grammar allows nothing) are reported beside those that ended with the step that was read: by this step, or, where a
+        grammar fails, by the next."""
         if not any(s.params.grammar is not None for s in (*self.scheduler.running, *self.scheduler.waiting)):
-            return []
-        finished = self.drain()
+            return
+        self._unreported += self.drain()
         for s in (*self.scheduler.running, *self.scheduler.waiting):
             if s.params.grammar is None or s.mask_at == len(s.token_ids):
                 continue
             try:
                 s.mask = mask_words(s.params.grammar.allowed(list(s.output_ids)), self.vocab_size)
-            except BaseException:            # the request goes, the others and the engine stay as they are
+            except BaseException:            # the request goes (the exception is its report), the others and the engine stay as they are
                 self._end_now(s)
                 raise
             s.mask_at = len(s.token_ids)
             if s.mask is not None and not s.mask.any():
                 self._end_now(s)
-                finished.append(s)
-        return finished
+                self._unreported.append(s)
 
     def _end_now(self, seq) -> None:
         seq.finish_time = time.perf_counter()
@@ -547,7 +555,7 @@ class LLMEngine:
 
     # ------------------------------------------------------------------ one engine step
     def has_work(self) -> bool:
-        return self.scheduler.has_work() or self._in_flight is not None
+        return self.scheduler.has_work() or self._in_flight is not None or bool(self._unreported)
 
     @torch.inference_mode()
     def step(self) -> list:
@@ -559,15 +567,16 @@ class LLMEngine:
         -(k+1) in the batch means "entry k of the previous step's samples"), so nothing but the stop
         rules waits for the host: a request that ends by count is known beforehand, one that ends by
         EOS runs one step too many, whose token is dropped."""
-        finished = self._ask_grammars()
+        self._ask_grammars()
         launched = self._launch()
         if self._in_flight is not None:
-            finished += self._complete(self._in_flight)
+            self._unreported += self._complete(self._in_flight)
         self._in_flight = launched
         # nothing to run ahead of: read the step's tokens now (also keeps the reference's loop
         # `while engine.scheduler.has_work(): engine.step()` complete)
         if launched is not None and (not self.cfg.overlap_steps or not self.scheduler.has_work()):
-            finished += self.drain()
+            self._unreported += self.drain()
+        finished, self._unreported = self._unreported, []
         return finished
 
     def drain(self) -> list:
@@ -691,8 +700,12 @@ class LLMEngine:
             done_event = torch.cuda.Event()
             done_event.record()
 
-        # bookkeeping that does not need the tokens: progress, the place each token will take, and the
-        # requests that end by count with this step
+        ending = self._advance(batch, sample_seqs)
+        return _InFlight(sample_seqs, [s.num_tokens - 1 for s in sample_seqs], ending, sources, logprob_sources, done_event)
+
+    def _advance(self, batch, sample_seqs) -> list:
+        """Bookkeeping that does not need a launched step's tokens: progress, the place each token will take, and the requests that end by count
+        with this step, which are returned."""
         self.num_steps += 1
         for seq, n in batch:
             self.cache.advance(seq.cache, n)
@@ -705,7 +718,7 @@ class LLMEngine:
                 self.scheduler.finish(seq)                 # its pages may go to the next step: that one runs after this one
                 self._ended(seq)
                 ending.append(seq)
-        return _InFlight(sample_seqs, [s.num_tokens - 1 for s in sample_seqs], ending, sources, logprob_sources, done_event)
+        return ending
 
     def _complete(self, fl) -> list:
         with _nvtx_range("sample"):
