@@ -175,6 +175,7 @@ class LLMEngine:
 
     def _host_state(self) -> None:
         """What the host keeps between steps."""
+        self.scheduler.ended = self._ended
         self._in_flight = None
         self._unreported: list = []              # requests that have ended and that no step has returned yet
         self.prefixes: list = []                 # the prefixes that requests may begin with (``add_prefix``)
@@ -490,7 +491,7 @@ class LLMEngine:
         self.cache.free(prefix.cache)
 
     def _ended(self, seq) -> None:
-        """What a request that has ended holds beside its pages goes back."""
+        """What a request that has ended, whoever ended it, holds beside its pages goes back (the scheduler calls it)."""
         self.rules.release(seq)
         if seq.prefix is not None:
             prefix, seq.prefix = seq.prefix, None
@@ -551,7 +552,6 @@ class LLMEngine:
     def _end_now(self, seq) -> None:
         seq.finish_time = time.perf_counter()
         self.scheduler.finish(seq)
-        self._ended(seq)
 
     # ------------------------------------------------------------------ one engine step
     def has_work(self) -> bool:
@@ -716,7 +716,6 @@ class LLMEngine:
             total = len(seq.token_ids)
             if total - seq.prompt_len >= seq.params.max_tokens or total >= max_len:
                 self.scheduler.finish(seq)                 # its pages may go to the next step: that one runs after this one
-                self._ended(seq)
                 ending.append(seq)
         return ending
 
@@ -746,7 +745,6 @@ class LLMEngine:
                 seq.ended_by_eos = True
                 seq.finish_time = now
                 self.scheduler.finish(seq)
-                self._ended(seq)
                 finished.append(seq)
         return finished
 

@@ -62,6 +62,7 @@ class Scheduler:
         self.waiting: deque = deque()
         self.running: list = []          # in order of admission: the last one is the first to be pushed out
         self.num_preemptions = 0
+        self.ended = None                # called with every request that ``finish`` ends: what it holds beside its ``RequestCache`` goes back
         # pages an admission must leave free (a hundredth of the pool, at least one): room for the
         # running requests' next pages (inference_engine/scheduler.py:29-30)
         self.watermark = max(1, min(p.num_pages for p in cache.pools) // 100)
@@ -159,3 +160,5 @@ class Scheduler:
         elif seq.status is Status.WAITING and seq in self.waiting:
             self.waiting.remove(seq)
         seq.status = Status.FINISHED
+        if self.ended is not None:
+            self.ended(seq)

@@ -42,3 +42,22 @@ def test_a_grammar_that_fails_hides_nobody_else(overlap, first):
     assert raised == 1 and got == [good] and len(good.output_ids) == 3 and len(bad.output_ids) == 3 and bad.finish_time is not None
     assert good.output_ids == [3, 4, 5]
     whole(eng)
+
+
+@pytest.mark.parametrize("when", ["waiting", "running"])
+def test_a_request_that_is_ended_early_gives_everything_back(when):
+    """``scheduler.finish`` ends a request wherever it is: its prefix and its rules' slot go back too."""
+    eng = HostEngine(40, overlap_steps=False)
+    p = eng.add_prefix(list(range(40)))
+    assert eng.computed == [32]
+    s = eng.add_request(list(range(40)), SamplingParams(max_tokens=9, repetition_penalty=1.2), prefix=p)
+    if when == "running":
+        eng.step()
+        eng.rules._held[s.seq_id] = 0
+        eng.rules._free.clear()
+    eng.scheduler.finish(s)
+    assert p.users == 0 and not eng.has_work() and eng.rules._free == ([0] if when == "running" else [])
+    eng.scheduler.finish(s)                                   # once more: nothing happens
+    assert p.users == 0
+    eng.release_prefix(p)
+    whole(eng)
