@@ -12,11 +12,13 @@ from __future__ import annotations
 import contextlib
 import os
 import time
+from collections import deque
 from dataclasses import dataclass
 
 import numpy as np
 import torch
 
+from ..cache.manager import RequestCache
 from ..config import EngineConfig, load_config
 from ..kernels import gemm_tc, ops
 from ..kernels.attention import captured_context_bounds, sharing_pays
@@ -450,14 +452,10 @@ class LLMEngine:
             raise ValueError(f"a prefix of {len(ids)} tokens fills no page of {self.cfg.block_size}")
         if len(ids) > self.cfg.max_model_len:
             raise ValueError(f"prefix of {len(ids)} tokens exceeds max_model_len {self.cfg.max_model_len}")
+        refused = self._no_room_for_prefix(pages)
+        if refused:
+            raise ValueError(refused)
         p = Prefix(ids[:pages * self.cfg.block_size])
-        live = list(self.scheduler.running) + list(self.scheduler.waiting)
-        for s in live:
-            most = min(s.prompt_len + s.params.max_tokens, self.cfg.max_model_len)
-            if not self.scheduler.can_ever_fit(most, s.prefix_pages, pinned=pages):
-                raise ValueError(f"a prefix of {pages} pages would leave request {s.seq_id} too few")
-        if not self.cache.can_reserve(p.cache, len(p.token_ids), watermark=self.scheduler.watermark):
-            raise ValueError(f"a prefix of {pages} pages, {min(q.num_free for q in self.cache.pools)} free")
         try:
             self._compute_prefix(p)
         except BaseException:
@@ -466,6 +464,15 @@ class LLMEngine:
         self.cache.pin(p.cache)
         self.prefixes.append(p)
         return p
+
+    def _no_room_for_prefix(self, pages: int) -> str | None:
+        """Why a prefix of so many pages cannot be held now; None where it can."""
+        for s in (*self.scheduler.running, *self.scheduler.waiting):
+            if not self.scheduler.can_ever_fit(self._most_positions(s.prompt_len, s.params), s.prefix_pages, pinned=pages):
+                return f"a prefix of {pages} pages would leave request {s.seq_id} too few"
+        if not self.cache.can_reserve(RequestCache(), pages * self.cfg.block_size, watermark=self.scheduler.watermark):
+            return f"a prefix of {pages} pages, {min(q.num_free for q in self.cache.pools)} free"
+        return None
 
     def _compute_prefix(self, p: Prefix) -> None:
         arr = np.asarray(p.token_ids, dtype=np.int32)
@@ -499,13 +506,31 @@ class LLMEngine:
             if prefix.closed and not prefix.users:
                 self._free_prefix(prefix)
 
-    def add_request(self, prompt, params: SamplingParams | None = None, prefix: Prefix | None = None) -> Sequence:
-        """``prefix``: what the prompt begins with, from ``add_prefix``; the request shares its pages (all of them that lie in front of the prompt's
-        last token)."""
+    def _checked(self, prompt, params: SamplingParams | None) -> tuple:
+        """A request's prompt and options as they are run; ValueError for those that are not taken."""
         ids = self._prompt_ids(prompt)
         params = params or SamplingParams()
         if params.logit_bias and max(params.logit_bias) >= self.vocab_size:
             raise ValueError(f"logit_bias names token {max(params.logit_bias)}, outside the vocabulary [0, {self.vocab_size})")
+        if len(ids) > self.cfg.max_model_len:
+            raise ValueError(f"prompt of {len(ids)} tokens exceeds max_model_len {self.cfg.max_model_len}")
+        if len(ids) + params.max_tokens > self.cfg.max_model_len:     # inference_engine/engine.py:126-127
+            params = SamplingParams(**{**params.__dict__, "max_tokens": max(1, self.cfg.max_model_len - len(ids))})
+        return ids, params
+
+    def _most_positions(self, prompt_len: int, params: SamplingParams) -> int:
+        return min(prompt_len + params.max_tokens, self.cfg.max_model_len)
+
+    def _refuse_what_never_fits(self, prompt_len: int, params: SamplingParams, shared: int = 0) -> None:
+        most = self._most_positions(prompt_len, params)
+        if not self.scheduler.can_ever_fit(most, shared):
+            raise ValueError(f"a request of {most} positions can never fit the cache "
+                             f"({self.cache.pools[0].num_usable} usable pages of {self.cfg.block_size}, {self.cache.pinned[0]} held by prefixes)")
+
+    def add_request(self, prompt, params: SamplingParams | None = None, prefix: Prefix | None = None) -> Sequence:
+        """``prefix``: what the prompt begins with, from ``add_prefix``; the request shares its pages (all of them that lie in front of the prompt's
+        last token)."""
+        ids, params = self._checked(prompt, params)
         shared = 0
         if prefix is not None:
             if prefix not in self.prefixes:
@@ -513,14 +538,7 @@ class LLMEngine:
             shared = min(len(prefix.token_ids), len(ids) - 1) // self.cfg.block_size
             if ids[:len(prefix.token_ids)] != prefix.token_ids[:len(ids)]:
                 raise ValueError("the prompt does not begin with the prefix")
-        if len(ids) > self.cfg.max_model_len:
-            raise ValueError(f"prompt of {len(ids)} tokens exceeds max_model_len {self.cfg.max_model_len}")
-        if len(ids) + params.max_tokens > self.cfg.max_model_len:     # inference_engine/engine.py:126-127
-            params = SamplingParams(**{**params.__dict__, "max_tokens": max(1, self.cfg.max_model_len - len(ids))})
-        most = min(len(ids) + params.max_tokens, self.cfg.max_model_len)
-        if not self.scheduler.can_ever_fit(most, shared):
-            raise ValueError(f"a request of {most} positions can never fit the cache "
-                             f"({self.cache.pools[0].num_usable} usable pages of {self.cfg.block_size}, {self.cache.pinned[0]} held by prefixes)")
+        self._refuse_what_never_fits(len(ids), params, shared)
         seq = Sequence(ids, params)
         if shared:
             seq.prefix, seq.prefix_pages = prefix, shared
@@ -749,34 +767,47 @@ class LLMEngine:
         return finished
 
     # ------------------------------------------------------------------ offline API
+    def _add_answers(self, asked: deque, n: int, seqs: list, arrival: float) -> None:
+        """Adds ``n`` answers to each of the next prompts (``asked``, from the front), behind its pages, for as long as there are places for them and
+        room for the pages beside the requests that live.  With no request alive there is: what is asked for fits alone."""
+        while asked and len(self.scheduler.running) + len(self.scheduler.waiting) < self.cfg.max_num_seqs:
+            ids, sp = asked[0]
+            pages = (len(ids) - 1) // self.cfg.block_size          # all in front of the last token
+            prefix = None
+            if pages:
+                if self.has_work() and (self._no_room_for_prefix(pages)
+                                        or not self.scheduler.can_ever_fit(self._most_positions(len(ids), sp), pages, pinned=pages)):
+                    return
+                prefix = self.add_prefix(ids[:pages * self.cfg.block_size])
+            asked.popleft()
+            try:
+                for _ in range(n):
+                    seqs.append(self.add_request(ids, sp, prefix=prefix))
+                    seqs[-1].arrival_time = arrival
+            finally:
+                if prefix is not None:                             # (held by the requests that begin with it)
+                    self.release_prefix(prefix)
+
     def generate(self, prompts, params=None, decode_text: bool = True, n: int = 1) -> list:
         """``n`` answers to every prompt, one behind another in the result; with more than one, the answers to a prompt share its pages where the
-        model allows it (``add_prefix``)."""
+        model allows it (``add_prefix``).  A prompt's pages are computed and held once its answers' turn comes: prompts that do not fit the cache side by
+        side wait for those in front.  What cannot be run at all is refused with ValueError before anything is added."""
         if not isinstance(params, list):
             params = [params or SamplingParams()] * len(prompts)
         if len(params) != len(prompts):
             raise ValueError("one SamplingParams per prompt")
         if n < 1:
             raise ValueError(f"n must be at least 1, got {n}")
-        seqs, prefixes = [], []
-        try:
-            for p, sp in zip(prompts, params):
-                prefix = None
-                if n > 1 and self.can_share:
-                    ids = self._prompt_ids(p)
-                    whole = (len(ids) - 1) // self.cfg.block_size * self.cfg.block_size
-                    if whole:
-                        try:
-                            prefix = self.add_prefix(ids[:whole])
-                        except ValueError:                     # no room to hold it beside the requests: every answer computes its own
-                            prefix = None
-                        else:
-                            prefixes.append(prefix)
-                seqs += [self.add_request(p, sp, prefix=prefix) for _ in range(n)]
-        finally:
-            for prefix in prefixes:                            # (held by the requests that begin with it)
-                self.release_prefix(prefix)
-        while self.has_work():
+        arrival = time.perf_counter()
+        asked = deque(self._checked(p, sp) for p, sp in zip(prompts, params))
+        for ids, sp in asked:
+            self._refuse_what_never_fits(len(ids), sp)
+        seqs: list = []
+        if n == 1 or not self.can_share:
+            seqs = [self.add_request(ids, sp) for ids, sp in asked for _ in range(n)]
+            asked.clear()
+        while asked or self.has_work():
+            self._add_answers(asked, n, seqs, arrival)
             self.step()
         outs = []
         for s in seqs:

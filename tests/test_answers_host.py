@@ -61,3 +61,57 @@ def test_a_request_that_is_ended_early_gives_everything_back(when):
     assert p.users == 0
     eng.release_prefix(p)
     whole(eng)
+
+
+def prompts_of(count, tokens):
+    return [[(i * 31 + k) % 4096 for k in range(tokens)] for i in range(count)]
+
+
+def check_outputs(outs, prompts, n, tokens):
+    assert [o.prompt_len for o in outs] == [len(p) for p in prompts for _ in range(n)]
+    assert all(o.output_ids == list(range(o.prompt_len, o.prompt_len + tokens)) for o in outs)        # (the model's answers)
+
+
+@pytest.mark.parametrize("overlap", [True, False])
+@pytest.mark.parametrize("blocks,count", [(100, 12), (60, 5), (42, 3)])
+def test_more_prompts_than_the_cache_holds_prefixes_for(overlap, blocks, count):
+    """Requests of 40 pages, ten of them their prompt's: they fit one after another, and so do their prefixes."""
+    prompts = prompts_of(count, 165)
+    eng = HostEngine(blocks, overlap_steps=overlap, max_model_len=1024)
+    outs = eng.generate(prompts, SamplingParams(max_tokens=475, ignore_eos=True), n=2)
+    check_outputs(outs, prompts, 2, 475)
+    assert eng.computed == [160] * count and all(o.ttft >= 0 and o.latency >= o.ttft for o in outs)
+    whole(eng)
+
+
+def test_every_place_is_filled():
+    """Prompts are taken up to the most requests that run at once, short ones (no whole page) among them."""
+    prompts = [p[:t] for p, t in zip(prompts_of(12, 40), (40, 16, 17, 3, 40, 33, 40, 40, 1, 40, 18, 40))]
+    eng = HostEngine(200, max_num_seqs=9)
+    outs = eng.generate(prompts, SamplingParams(max_tokens=6, ignore_eos=True), n=3)
+    check_outputs(outs, prompts, 3, 6)
+    assert len(eng.ran[0]) == 9 and eng.computed == [32, 16, 32, 32, 32, 32, 32, 16, 32]
+    whole(eng)
+
+
+def test_answers_beside_a_prefix_that_is_held():
+    """Pages that a user's prefix holds are not the answers'."""
+    eng = HostEngine(60, max_model_len=1024)
+    p = eng.add_prefix(list(range(160)))
+    prompts = prompts_of(4, 165)
+    outs = eng.generate(prompts, SamplingParams(max_tokens=475, ignore_eos=True), n=2)
+    check_outputs(outs, prompts, 2, 475)
+    with pytest.raises(ValueError, match="never fit"):
+        eng.generate(prompts_of(2, 165) + prompts_of(1, 320), SamplingParams(max_tokens=600, ignore_eos=True), n=2)
+    eng.release_prefix(p)
+    whole(eng)
+
+
+@pytest.mark.parametrize("n", [1, 2])
+@pytest.mark.parametrize("bad,match", [([], "empty"), ([5000], "vocabulary"), ([1] * 2000, "max_model_len"), ([1] * 990, "never fit")])
+def test_nothing_is_added_when_a_prompt_is_refused(n, bad, match):
+    eng = HostEngine(50, max_model_len=1024)
+    with pytest.raises(ValueError, match=match):
+        eng.generate(prompts_of(2, 40) + [bad], SamplingParams(max_tokens=4), n=n)
+    assert not eng.has_work() and eng.computed == []
+    whole(eng)
