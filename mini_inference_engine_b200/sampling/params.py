@@ -4,8 +4,14 @@ draws from torch's global generator, unseeded, so its sampled runs cannot be rep
 the reference does not have: penalties for repeated tokens, biases, a grammar, log-probabilities."""
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
+
+
+def _single(x) -> float:
+    """x as the float32 that the kernels get (beyond their range: infinite)."""
+    return ctypes.c_float(x).value
 
 
 @dataclass
@@ -26,16 +32,17 @@ class SamplingParams:
     def __post_init__(self):
         if self.temperature < 0:
             raise ValueError(f"temperature must be >= 0, got {self.temperature}")
-        if not (self.repetition_penalty > 0 and math.isfinite(self.repetition_penalty)):
-            raise ValueError(f"repetition_penalty must be positive and finite, got {self.repetition_penalty}")
+        # (all of them as float32: 1e300 is infinite there, and 1e-46 is 0)
+        if not (_single(self.repetition_penalty) > 0 and math.isfinite(_single(self.repetition_penalty))):
+            raise ValueError(f"repetition_penalty must be positive and finite in float32, got {self.repetition_penalty}")
         for name in ("presence_penalty", "frequency_penalty"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} must be finite, got {getattr(self, name)}")
+            if not math.isfinite(_single(getattr(self, name))):
+                raise ValueError(f"{name} must be finite in float32, got {getattr(self, name)}")
         for t, b in (self.logit_bias or {}).items():
             if int(t) != t or t < 0:
                 raise ValueError(f"logit_bias: {t!r} is not a token id")
-            if math.isnan(b) or b == math.inf:
-                raise ValueError(f"logit_bias of token {t}: a finite number or -inf, got {b}")
+            if math.isnan(b) or _single(b) == math.inf:
+                raise ValueError(f"logit_bias of token {t}: a finite number in float32 or -inf, got {b}")
         if self.grammar is not None and not callable(getattr(self.grammar, "allowed", None)):
             raise ValueError("a grammar has a method allowed(output_ids)")
 

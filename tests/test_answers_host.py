@@ -115,3 +115,17 @@ def test_nothing_is_added_when_a_prompt_is_refused(n, bad, match):
         eng.generate(prompts_of(2, 40) + [bad], SamplingParams(max_tokens=4), n=n)
     assert not eng.has_work() and eng.computed == []
     whole(eng)
+
+
+@pytest.mark.parametrize("given", [dict(repetition_penalty=1e-46), dict(repetition_penalty=1e39), dict(presence_penalty=-1e39), dict(frequency_penalty=1e300),
+                                   dict(logit_bias={3: 1e39})])
+def test_numbers_that_float32_does_not_hold_are_refused(given):
+    """The kernels' numbers are float32: a repetition penalty of 0 or infinity there makes NaN of some logits."""
+    with pytest.raises(ValueError, match="float32"):
+        SamplingParams(**given)
+
+
+def test_numbers_at_the_ends_of_float32_are_taken():
+    most, least = 3.4028234e38, 1e-45
+    SamplingParams(repetition_penalty=most, presence_penalty=-most, frequency_penalty=most, logit_bias={3: most, 4: -most, 5: -1e300})
+    SamplingParams(repetition_penalty=least)
