@@ -510,8 +510,10 @@ class LLMEngine:
         """A request's prompt and options as they are run; ValueError for those that are not taken."""
         ids = self._prompt_ids(prompt)
         params = params or SamplingParams()
-        if params.logit_bias and max(params.logit_bias) >= self.vocab_size:
-            raise ValueError(f"logit_bias names token {max(params.logit_bias)}, outside the vocabulary [0, {self.vocab_size})")
+        if params.logit_bias:                    # (a copy of its own: the device takes the list at the request's first token, and its length at every one)
+            params = SamplingParams(**{**params.__dict__, "logit_bias": dict(params.logit_bias)})
+            if max(params.logit_bias) >= self.vocab_size:
+                raise ValueError(f"logit_bias names token {max(params.logit_bias)}, outside the vocabulary [0, {self.vocab_size})")
         if len(ids) > self.cfg.max_model_len:
             raise ValueError(f"prompt of {len(ids)} tokens exceeds max_model_len {self.cfg.max_model_len}")
         if len(ids) + params.max_tokens > self.cfg.max_model_len:     # inference_engine/engine.py:126-127

@@ -129,3 +129,15 @@ def test_numbers_at_the_ends_of_float32_are_taken():
     most, least = 3.4028234e38, 1e-45
     SamplingParams(repetition_penalty=most, presence_penalty=-most, frequency_penalty=most, logit_bias={3: most, 4: -most, 5: -1e300})
     SamplingParams(repetition_penalty=least)
+
+
+def test_a_request_keeps_the_biases_that_it_was_added_with():
+    """What the caller does to its dictionary afterwards does not reach a request: its list is on the device by then, as long as it was."""
+    eng = HostEngine(40)
+    given = SamplingParams(max_tokens=3, logit_bias={3: 1.0})
+    s = eng.add_request([1, 2], given)
+    given.logit_bias.update({4: 2.0, 10 ** 6: 1.0})
+    assert s.params.logit_bias == {3: 1.0}
+    given.logit_bias = {3: float("nan")}
+    with pytest.raises(ValueError, match="logit_bias"):
+        eng.add_request([1, 2], given)
