@@ -180,6 +180,7 @@ class LLMEngine:
         self.scheduler.ended = self._ended
         self._in_flight = None
         self._unreported: list = []              # requests that have ended and that no step has returned yet
+        self._under_grammar: dict = {}           # live requests with a grammar, by id: a step without any looks at no request for it
         self.prefixes: list = []                 # the prefixes that requests may begin with (``add_prefix``)
 
     @torch.inference_mode()
@@ -218,7 +219,7 @@ class LLMEngine:
     def _choose_under_rules(self, seqs, logits, extras, at: int, turn: int, host_out):
         """The tokens of ``seqs`` once more where some have rules, chosen from a step's logits under them: over the tokens that the step itself chose.
         ``at``: the rows' first place among the sampled tokens.  Returns the pinned row that receives the log-probabilities, or None."""
-        if not any(s.params.has_rules for s in seqs):
+        if not any(s.has_rules for s in seqs):
             return None
         k = len(seqs)
         lp = None
@@ -500,6 +501,7 @@ class LLMEngine:
     def _ended(self, seq) -> None:
         """What a request that has ended, whoever ended it, holds beside its pages goes back (the scheduler calls it)."""
         self.rules.release(seq)
+        self._under_grammar.pop(seq.seq_id, None)
         if seq.prefix is not None:
             prefix, seq.prefix = seq.prefix, None
             prefix.users -= 1
@@ -545,6 +547,8 @@ class LLMEngine:
         if shared:
             seq.prefix, seq.prefix_pages = prefix, shared
             prefix.users += 1
+        if params.grammar is not None:
+            self._under_grammar[seq.seq_id] = seq
         self.scheduler.add(seq)
         return seq
 
@@ -553,11 +557,11 @@ class LLMEngine:
         """Before a step: what every live request's grammar allows next.  A grammar reads the tokens so far, so the step in flight is read first.  The requests
         that end here (their grammar allows nothing) are reported beside those that ended with the step that was read: by this step, or, where a
         grammar fails, by the next."""
-        if not any(s.params.grammar is not None for s in (*self.scheduler.running, *self.scheduler.waiting)):
+        if not self._under_grammar:
             return
         self._unreported += self.drain()
-        for s in (*self.scheduler.running, *self.scheduler.waiting):
-            if s.params.grammar is None or s.mask_at == len(s.token_ids):
+        for s in tuple(self._under_grammar.values()):
+            if s.mask_at == len(s.token_ids):
                 continue
             try:
                 s.mask = mask_words(s.params.grammar.allowed(list(s.output_ids)), self.vocab_size)
@@ -706,7 +710,7 @@ class LLMEngine:
                 self.h2d_bytes += buf.nbytes
                 logits = self.model.step(ctx)
                 lp = None
-                if any(s.params.has_rules for s in sample_seqs):
+                if any(s.has_rules for s in sample_seqs):
                     lp = self._choose_under_rules(sample_seqs, logits, ctx.extras, 0, turn, self._pinned_tokens)
                 elif sample_seqs and not self.sampler.sample_step(logits, ctx.extras, self._sampled[:k], row_seeds, seeds,
                                                                   host_out=self._pinned_tokens):

@@ -30,6 +30,7 @@ class Sequence:
         # turning two thousand Python integers into numbers again at every step
         self.prompt_array = np.asarray(self.token_ids, dtype=np.int32)
         self.params = params
+        self.has_rules = params.has_rules        # asked of every row at every step
         self.cache = RequestCache()
         self.status = Status.WAITING
         self.num_preemptions = 0

@@ -87,7 +87,7 @@ class RuleBook:
         masks = []
         for i, s in enumerate(seqs):
             p = s.params
-            if not p.has_rules:
+            if not s.has_rules:
                 continue
             ints[:4, i] = self.admit(s), s.prompt_len, len(s.token_ids), len(p.logit_bias or ())
             reals[:, i] = p.repetition_penalty, p.presence_penalty, p.frequency_penalty

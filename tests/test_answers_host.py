@@ -141,3 +141,33 @@ def test_a_request_keeps_the_biases_that_it_was_added_with():
     given.logit_bias = {3: float("nan")}
     with pytest.raises(ValueError, match="logit_bias"):
         eng.add_request([1, 2], given)
+
+
+def test_a_step_without_grammars_looks_at_no_request_for_them():
+    """However many wait: a step's host work goes by the rows it runs."""
+    eng = HostEngine(40, max_num_seqs=2, overlap_steps=False)
+    for _ in range(50):
+        eng.add_request([1, 2], SamplingParams(max_tokens=3))
+    asked = []
+
+    class Params:
+        def __getattribute__(self, name):
+            asked.append(name)
+            return getattr(SamplingParams(max_tokens=3), name)
+
+    for s in list(eng.scheduler.waiting)[2:]:
+        s.params = Params()
+    eng.step()
+    assert asked == []
+
+
+def test_grammars_are_asked_for_as_long_as_their_requests_live():
+    eng = HostEngine(40)
+    first, second = eng.add_request([1, 2], SamplingParams(max_tokens=3, grammar=Upto(9))), eng.add_request([1, 2], SamplingParams(max_tokens=9, grammar=Upto(5)))
+    early = eng.add_request([1, 2], SamplingParams(max_tokens=9, grammar=Upto(9)))
+    eng.scheduler.finish(early)
+    assert list(eng._under_grammar) == [first.seq_id, second.seq_id]
+    while eng.has_work():
+        eng.step()
+    assert not eng._under_grammar and len(first.output_ids) == 3 and len(second.output_ids) == 5 and early.mask_at == -1
+    whole(eng)
