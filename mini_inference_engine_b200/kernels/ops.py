@@ -874,7 +874,9 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     _need(pages * num_kv_heads * page_size < 1 << 31, "caches of 2^31 key rows and more are not taken")
     _need(scale > 0, "the scale of the scores must be positive")
     device = q.get_device()
-    _need(device == torch.cuda.current_device(), "the tensors must be on the current device")
+    _need(torch.cuda.current_device() == device == k_cache.get_device() == v_cache.get_device() == out.get_device() == block_tables.get_device()
+          == row_q_start.get_device() == row_q_len.get_device() == row_ctx_len.get_device() == group_start.get_device() == group_prefix.get_device(),
+          "the tensors must be on the current device")
     if rows == 0:
         return out
     covered = width * page_size
@@ -1060,7 +1062,9 @@ def sample(logits: torch.Tensor, temperature, request, position, seed: int, out:
     _need(logprob is None or logprob.dtype == torch.float32, "logprob must be float32")
     _need(not append or (rules is not None and rules.history is not None), "append goes with rules that have a history")
     _ptr(logits)                                               # (refuses what is not on a CUDA device)
-    _need(rules is not None or logits.device.index == torch.cuda.current_device(), "logits must be on the current device")
+    _need(torch.cuda.current_device() == logits.get_device() == temperature.get_device() == request.get_device() == position.get_device() == out.get_device()
+          and (logprob is None or logprob.get_device() == logits.get_device())
+          and (host_ptr is None or host_turn is None or host_turn.get_device() == logits.get_device()), "the tensors must be on the current device")
     _check(_rules_lib().mie_sample_rules(args, logits.data_ptr(), logits.stride(0), _at(temperature), _at(request), _at(position), seed & ((1 << 64) - 1), _at(out),
                                          _at(logprob), int(append), rows, vocab, host_ptr, turn_ptr, stride, _stream()), "sample with rules")
     return out
