@@ -12,6 +12,7 @@ from __future__ import annotations
 import contextlib
 import os
 import time
+import weakref
 from collections import deque
 from dataclasses import dataclass
 
@@ -177,7 +178,9 @@ class LLMEngine:
 
     def _host_state(self) -> None:
         """What the host keeps between steps."""
-        self.scheduler.ended = self._ended
+        # (weakly: an engine that only the garbage collector could end might end, graphs and all, in the middle of another's capture)
+        ended = weakref.WeakMethod(self._ended)
+        self.scheduler.ended = lambda seq: ended()(seq)
         self._in_flight = None
         self._unreported: list = []              # requests that have ended and that no step has returned yet
         self._under_grammar: dict = {}           # live requests with a grammar, by id: a step without any looks at no request for it

@@ -171,3 +171,22 @@ def test_grammars_are_asked_for_as_long_as_their_requests_live():
         eng.step()
     assert not eng._under_grammar and len(first.output_ids) == 3 and len(second.output_ids) == 5 and early.mask_at == -1
     whole(eng)
+
+
+def test_an_engine_ends_with_its_last_reference():
+    """Nothing waits for the garbage collector, which may run while another engine captures its graphs: graphs that end then break that capture."""
+    import gc
+    import weakref
+    gc.collect()
+    gc.disable()
+    try:
+        eng = HostEngine(40)
+        eng.generate(prompts_of(2, 40), SamplingParams(max_tokens=3, grammar=Upto(2)), n=2)
+        p = eng.add_prefix(list(range(40)))
+        s = eng.add_request(list(range(40)), prefix=p)
+        eng.step()
+        gone = weakref.ref(eng)
+        del eng
+        assert gone() is None and s.prefix is p
+    finally:
+        gc.enable()
