@@ -772,21 +772,41 @@ PREFIX_ONE_BY_ONE_BYTES = (20 << 20, 48 << 20)                # heads below 96, 
 PREFIX_ONE_BY_ONE_KEYS = 640
 
 
+class _NoScratch(Exception):
+    """Scratch memory that starts cleared would have to be made inside a capture."""
+
+
+def _cleared(where, name: str, numel: int) -> tuple:
+    """(scratch tensor of int32 that starts cleared, whether it was made just now)."""
+    there = _workspaces.get((str(where), name))
+    ready = there is not None and there.numel() >= numel
+    if not ready and torch.cuda.is_current_stream_capturing():
+        raise _NoScratch
+    return _workspace(where, name, numel, torch.int32), not ready
+
+
 @functools.lru_cache(maxsize=256)
 def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_prefix: int, max_own: int,
                  pages: int, stream: int):
     """What a launch of these sizes keeps from call to call: its plan and its scratch memory, as the bytes of a _SharedArgs behind a call's own (and the tensors).  Every stream
-    has scratch memory of its own, so that calls on two do not meet; ``stream`` 0: the default stream, and captured launches."""
+    has scratch memory of its own, so that calls on two do not meet; ``stream`` 0: the default stream, and captured launches; -1: one captured launch alone, whose scratch is its
+    graph's and cleared at every replay (memory made inside a capture is not clear before the first)."""
     a = _SharedArgs(num_rows=rows, groups=groups, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size,
                     most_prefix=max_prefix, most_own=max_own, num_pages=pages)
     where = torch.device("cuda", device)
     _need(_shared_libs()[0].mie_prefix_layout(ctypes.byref(a), num_sms(where)) == 0, f"{num_heads} heads of {head_dim} on {num_kv_heads}: not taken")
-    own = f"@{stream}" if stream else ""
+    own, fresh = f"@{stream}" if stream > 0 else "", False
 
     def scratch(name, numel, dtype=torch.float32, zero=False):
-        if zero and own:                                      # a launch captured later finds these cleared, outside its graph
-            _workspace(where, name, numel, dtype)
-        return _workspace(where, name + own, numel, dtype)
+        nonlocal fresh
+        if stream < 0:
+            return (torch.zeros if zero else torch.empty)(max(1, numel), dtype=dtype, device=where)
+        if not zero:
+            return _workspace(where, name + own, numel, dtype)
+        for n in ((name, name + own) if own else (name,)):    # (a launch captured later finds the first cleared, outside its graph)
+            t, made = _cleared(where, n, numel)
+            fresh |= made
+        return t
 
     kept = [scratch("prefix_o", a.most_slots * num_heads * head_dim), scratch("prefix_lse", a.most_slots * num_heads), scratch("prefix_chunk", 1, torch.int32),
             scratch("prefix_rows", 2 * rows, torch.int32), scratch("prefix_marks", rows * num_kv_heads, torch.int32, zero=True)]
@@ -817,6 +837,8 @@ def _shared_plan(device: int, rows: int, groups: int, num_heads: int, num_kv_hea
         for name, t in zip(("part_o", "part_lse", "counters"), more):
             setattr(a, name, t.data_ptr())
         kept += more
+    if fresh:                                                 # whoever uses it next may do so on another stream
+        torch.cuda.current_stream(where).synchronize()
     return bytes(a)[_shared_call.size:], a.walk, kept
 
 
@@ -847,8 +869,8 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
 
     Two launches: the keys (prefixes in tiles of (row, head) pairs, and the rows' own), then what joins a row's partial results; one, row by row, where
     little is shared (``PREFIX_ONE_BY_ONE_BYTES``).  Rows with more than one new token are skipped.  Slots of a row's last page behind its context must hold
-    finite values (see ``decode_uses_tma``).  Launches captured on any streams share scratch memory, as those of other kernels here do: their graphs are replayed one
-    behind the other."""
+    finite values (see ``decode_uses_tma``).  Launches captured on any streams share scratch memory with one another and with calls on the default stream, as those of
+    other kernels here do: such graphs are replayed one behind the other, and behind those calls."""
     bf16, i32, f32 = torch.bfloat16, torch.int32, out.dtype == torch.float32
     _need(q.dtype == bf16 == k_cache.dtype == v_cache.dtype and (f32 or out.dtype == bf16), "attention over shared prefixes is bfloat16 (its output bfloat16 or float32)")
     _need(block_tables.dtype == row_q_start.dtype == row_q_len.dtype == row_ctx_len.dtype == group_start.dtype == group_prefix.dtype == i32
@@ -887,8 +909,11 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     max_prefix = covered if max_prefix is None else max(1, min(max_prefix, covered))
     stream = _stream()
     # (lengths are planned for in powers of two: a plan serves many steps)
-    plan, walk, _ = _shared_plan(device, rows, groups, num_heads, num_kv_heads, head_dim, page_size, 1 << (max_prefix - 1).bit_length(),
-                                 1 << (max_own - 1).bit_length(), pages, 0 if torch.cuda.is_current_stream_capturing() else stream.value or 0)
+    sizes = (device, rows, groups, num_heads, num_kv_heads, head_dim, page_size, 1 << (max_prefix - 1).bit_length(), 1 << (max_own - 1).bit_length(), pages)
+    try:
+        plan, walk, _kept = _shared_plan(*sizes, 0 if torch.cuda.is_current_stream_capturing() else stream.value or 0)
+    except _NoScratch:
+        plan, walk, _kept = _shared_plan.__wrapped__(*sizes, -1)
     args = _shared_call.pack(at_q, at_k, at_v, *ints, at_out, q_stride, width, f32, scale, walk) + plan
     if walk == 2:
         _check(_shared_libs()[2].mie_decode_attention_through(args, stream), "shared_prefix_attention (row by row)")
