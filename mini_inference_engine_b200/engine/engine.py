@@ -22,7 +22,7 @@ import torch
 from ..cache.manager import RequestCache
 from ..config import EngineConfig, load_config
 from ..kernels import gemm_tc, ops
-from ..kernels.attention import captured_context_bounds, sharing_pays
+from ..kernels.attention import captured_context_bounds, sharing_pays, sharing_weight
 from ..models.decoder import DecoderModel
 from ..parts.base import Runtime
 from ..sampling.params import SamplingParams
@@ -157,8 +157,7 @@ class LLMEngine:
         self.can_share = self.cache.can_share() and not layout.state         # whether requests can share pages
         self._host_state()
         self._shared_graphs: dict = {}           # (bucket, context bound) -> captured decode step over shared prefixes, or None: it has run once
-        self._bytes_per_key = max((2 * n.num_kv_heads * n.head_dim * torch.empty((), dtype=dtype).element_size()
-                                   for _, n in layout.kv.values()), default=0)
+        self._kv_shape = max(((n.num_kv_heads, n.head_dim) for _, n in layout.kv.values()), key=lambda s: s[0] * s[1], default=(0, 0))      # of the widest layer
         self.graphs: dict = {}                   # (bucket, context bound) -> captured decode step
         self.graph_sizes: list = []
         self.graph_bounds: list = []             # the context bounds the buckets were captured for, ascending
@@ -298,9 +297,13 @@ class LLMEngine:
         if self.dtype != torch.bfloat16:
             return None
         groups = shared_groups(dseqs, self.cfg.block_size)
-        if not groups or len(groups) > self.SHARED_GROUPS or not sharing_pays(groups, self._bytes_per_key):
+        if not groups or len(groups) > self.SHARED_GROUPS:
             return None
-        return groups
+        heads, head_dim = self._kv_shape
+        per_key = 2 * 2 * heads * head_dim
+        own = sum(s.cache.num_computed + 1 for s in dseqs) - sum(n * positions for n, _, positions in groups)
+        weight = sharing_weight(head_dim, heads, len(dseqs), own * per_key, sum(positions for _, _, positions in groups) * per_key)
+        return groups if sharing_pays(groups, per_key, weight) else None
 
     def _decode_shared(self, drows, extras, groups, context: int):
         """Runs a decode step whose rows share prefixes: from its bucket's graph, which is captured the second time the bucket occurs (the first time

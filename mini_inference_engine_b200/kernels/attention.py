@@ -60,16 +60,30 @@ def rotates_in_decode(dtype, head_dim: int, ctx) -> bool:
             and decode_only(ctx) and getattr(ctx, "prefix", None) is None)
 
 
-# Shared prefixes against ordinary decode attention, which reads a prefix once a row, by the bytes of keys and values that sharing saves a layer (SHARE_MIN_BYTES).
-# Us, ordinary : shared -- 32 heads of 64 on 4, 2 rows behind 208 keys 4.2 : 4.3, 8 behind 2,048 (15 MB) 10.0 : 11.1; 32 of 128 on 8, 64 behind 8,000 (2.1 GB) 376 : 43, 256 behind
-# 16,384 1,983 : 110; 32 of 128 on 32, 33 rows in five groups (0.9 GB) 159 : 69.
-SHARE_MIN_BYTES = 48 << 20
+# Shared prefixes against ordinary decode attention, which reads a prefix once a row: what sharing saves is the bytes of keys and values that are not read again, SHARE_MIN_BYTES of
+# them a layer at least.  What it costs beside that goes by the head size (``sharing_weight``).  Both sides as the engine runs them: the context's bound for every length, from 33 rows on
+# ordinary attention rotates queries and keys itself and sharing leaves that to a launch of its own, layers' caches in turns.  The weights are those of a grid that take the least time
+# over 5,100 steps (4 to 256 rows in 1 to 8 groups, 64 to 14,000 shared and up to 4,000 own keys, eleven head shapes): attention takes 1.5 % longer than by the better of the two on the
+# average and up to 1.4 times as long as by the other (3,100 steps that the grid did not see: 1.9 %, and 1.6 times); by 48 MB alone, whatever the rest, 5 % and 3.6 times (32 heads of 64 on 32, 256 rows of up to 3,000 own keys behind 112: 566 : 2,059).  Us, ordinary : shared -- 32 heads of 64 on 4: 64 rows behind 784
+# keys (48 MB) 14.6 : 19.9, behind 2,352 (144 MB) 31 : 23, of 900 own keys 39 : 37; 256 rows behind 592 (147 MB) 37 : 33, of 900 own keys 66 : 94; 32 heads of 128 on 8: 16 rows
+# behind 832 (49 MB) 15.0 : 18.2, behind 1,648 (97 MB) 24 : 18; 64 behind 8,000 (2.1 GB) 376 : 43; 32 of 128 on 32: 32 rows behind 112 (54 MB) 25 : 31, behind 304 (147 MB) 39 : 32.
+SHARE_MIN_BYTES = 64 << 20
 
 
-def sharing_pays(groups, bytes_per_key: int) -> bool:
+def sharing_weight(head_dim: int, num_kv_heads: int, rows: int, own_bytes: float, prefix_bytes: float) -> float:
+    """How many times SHARE_MIN_BYTES sharing must save a step of that many rows, with ``own_bytes`` of keys and values behind the prefixes and ``prefix_bytes`` of the prefixes
+    themselves (each once)."""
+    if head_dim == 64:                            # the walk reads keys that few pairs see slower than ordinary attention does
+        return 0.78 + own_bytes / (36.6 * 2 ** 20) + prefix_bytes / (42.7 * 2 ** 20) + rows * num_kv_heads / 1600
+    if head_dim == 128:
+        return 1.03 + own_bytes / (91 << 20)
+    return 0.66 + own_bytes / (640 << 20) + rows * num_kv_heads / 1600       # own keys by the same kernel; a block a row and a key head more
+
+
+def sharing_pays(groups, bytes_per_key: int, weight: float = 1.0) -> bool:
     """Whether a step of single tokens whose rows share prefixes -- ``groups`` as (rows, ..., positions) -- is attended over with them shared; ``bytes_per_key``
-    of keys and values in a layer."""
-    return sum((g[0] - 1) * g[-1] for g in groups) * bytes_per_key >= SHARE_MIN_BYTES
+    of keys and values in a layer, ``weight``: ``sharing_weight``."""
+    return sum((g[0] - 1) * g[-1] for g in groups) * bytes_per_key >= SHARE_MIN_BYTES * weight
 
 
 # float32: tiles of (token, head) pairs (csrc/attention_f32.cu) against a warp a pair.  A tile takes as long with one pair as with 64, a walk of keys shared out over up to eight
