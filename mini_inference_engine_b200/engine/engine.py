@@ -570,7 +570,7 @@ class LLMEngine:
             if s.mask_at == len(s.token_ids):
                 continue
             try:
-                s.mask = mask_words(s.params.grammar.allowed(list(s.output_ids)), self.vocab_size)
+                s.mask = mask_words(s.params.grammar.allowed(list(s.output_ids)), self.vocab_size, s.params.banned())
             except BaseException:            # the request goes (the exception is its report), the others and the engine stay as they are
                 self._end_now(s)
                 raise

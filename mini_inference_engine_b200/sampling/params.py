@@ -26,7 +26,7 @@ class SamplingParams:
     frequency_penalty: float = 0.0      # ... and this once for every time that it holds them
     logit_bias: dict | None = None      # token id -> what is added to its logit (-inf: a ban)
     grammar: object | None = None       # has allowed(output_ids) -> token ids, or one truth value an entry of the vocabulary (or None: all),
-                                        # asked before every token; where it allows nothing, the request ends
+                                        # asked before every token; where it allows nothing (but what logit_bias bans), the request ends
     logprobs: bool = False              # the output's logprobs: of every token, under the rules and before the temperature
 
     def __post_init__(self):
@@ -45,6 +45,10 @@ class SamplingParams:
                 raise ValueError(f"logit_bias of token {t}: a finite number in float32 or -inf, got {b}")
         if self.grammar is not None and not callable(getattr(self.grammar, "allowed", None)):
             raise ValueError("a grammar has a method allowed(output_ids)")
+
+    def banned(self) -> list:
+        """Tokens whose bias leaves them no chance."""
+        return [int(t) for t, b in (self.logit_bias or {}).items() if _single(b) == -math.inf]
 
     @property
     def has_rules(self) -> bool:

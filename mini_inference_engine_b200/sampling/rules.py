@@ -9,9 +9,9 @@ import torch
 from ..kernels import ops
 
 
-def mask_words(allowed, vocab: int):
-    """A grammar's answer as int32 words of one bit an entry (ops.LogitRules); None: everything may follow.  Raises ValueError for an answer
-    that fits no vocabulary."""
+def mask_words(allowed, vocab: int, banned=()):
+    """A grammar's answer as int32 words of one bit an entry (ops.LogitRules), less the ``banned`` entries; None: everything may follow.  Raises
+    ValueError for an answer that fits no vocabulary."""
     if allowed is None:
         return None
     words = -(-vocab // 32)
@@ -25,6 +25,7 @@ def mask_words(allowed, vocab: int):
         if given.ndim != 1 or not np.issubdtype(given.dtype, np.integer) or given.min() < 0 or given.max() >= vocab:
             raise ValueError(f"a grammar allows token ids in [0, {vocab}), or one truth value an entry")
         bits[given] = True
+    bits[list(banned)] = False
     return np.packbits(bits, bitorder="little").view(np.int32)
 
 

@@ -190,3 +190,18 @@ def test_an_engine_ends_with_its_last_reference():
         assert gone() is None and s.prefix is p
     finally:
         gc.enable()
+
+
+def test_a_grammar_that_allows_only_what_is_banned_allows_nothing():
+    """Else the choice, with nothing left to choose from, would return a token that the grammar forbids."""
+    class Only:
+        def allowed(self, ids):
+            return [5, 7] if len(ids) < 2 else [5]
+
+    eng = HostEngine(40)
+    out, = eng.generate([[1, 2]], SamplingParams(max_tokens=9, grammar=Only(), logit_bias={5: -1e300, 7: -2.0}))
+    assert len(out.output_ids) == 2
+    eng.add_request([1, 2], SamplingParams(max_tokens=9, grammar=Only(), logit_bias={5: float("-inf")}))
+    eng.step()
+    s, = eng.scheduler.running
+    assert s.mask.tolist()[0] == 1 << 7 and not s.mask[1:].any()
