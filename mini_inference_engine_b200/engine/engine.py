@@ -179,7 +179,13 @@ class LLMEngine:
         """What the host keeps between steps."""
         # (weakly: an engine that only the garbage collector could end might end, graphs and all, in the middle of another's capture)
         ended = weakref.WeakMethod(self._ended)
-        self.scheduler.ended = lambda seq: ended()(seq)
+
+        def tell(seq):
+            engine_hears = ended()
+            if engine_hears is not None:
+                engine_hears(seq)
+
+        self.scheduler.ended = tell
         self._in_flight = None
         self._unreported: list = []              # requests that have ended and that no step has returned yet
         self._under_grammar: dict = {}           # live requests with a grammar, by id: a step without any looks at no request for it

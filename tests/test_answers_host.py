@@ -185,9 +185,10 @@ def test_an_engine_ends_with_its_last_reference():
         p = eng.add_prefix(list(range(40)))
         s = eng.add_request(list(range(40)), prefix=p)
         eng.step()
-        gone = weakref.ref(eng)
+        gone, scheduler = weakref.ref(eng), eng.scheduler
         del eng
         assert gone() is None and s.prefix is p
+        scheduler.finish(s)                                   # nobody is left to hear of it
     finally:
         gc.enable()
 
