@@ -14,7 +14,7 @@ import os
 import time
 import weakref
 from collections import deque
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 import torch
@@ -525,13 +525,13 @@ class LLMEngine:
         ids = self._prompt_ids(prompt)
         params = params or SamplingParams()
         if params.logit_bias:                    # (a copy of its own: the device takes the list at the request's first token, and its length at every one)
-            params = SamplingParams(**{**params.__dict__, "logit_bias": dict(params.logit_bias)})
+            params = replace(params, logit_bias=dict(params.logit_bias))
             if max(params.logit_bias) >= self.vocab_size:
                 raise ValueError(f"logit_bias names token {max(params.logit_bias)}, outside the vocabulary [0, {self.vocab_size})")
         if len(ids) > self.cfg.max_model_len:
             raise ValueError(f"prompt of {len(ids)} tokens exceeds max_model_len {self.cfg.max_model_len}")
         if len(ids) + params.max_tokens > self.cfg.max_model_len:     # inference_engine/engine.py:126-127
-            params = SamplingParams(**{**params.__dict__, "max_tokens": max(1, self.cfg.max_model_len - len(ids))})
+            params = replace(params, max_tokens=max(1, self.cfg.max_model_len - len(ids)))
         return ids, params
 
     def _most_positions(self, prompt_len: int, params: SamplingParams) -> int:

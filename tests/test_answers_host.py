@@ -206,3 +206,20 @@ def test_a_grammar_that_allows_only_what_is_banned_allows_nothing():
     eng.step()
     s, = eng.scheduler.running
     assert s.mask.tolist()[0] == 1 << 7 and not s.mask[1:].any()
+
+
+def test_options_of_a_class_of_the_callers_own():
+    """A copy of a request's options is of their own class."""
+    from dataclasses import dataclass
+
+    @dataclass
+    class Named(SamplingParams):
+        name: str = ""
+
+        def __post_init__(self):
+            super().__post_init__()
+            self.seen = True
+
+    eng = HostEngine(400, max_model_len=64)
+    s = eng.add_request([1] * 60, Named(max_tokens=50, logit_bias={3: 1.0}, name="a"))
+    assert isinstance(s.params, Named) and s.params.name == "a" and s.params.max_tokens == 4 and s.params.seen
