@@ -142,8 +142,9 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     }
     // this block's part of the context: the range [lo, ctx) cut into `splits` parts of whole tiles
     const int first_key = SHARED ? prefix : mask_first_key(ctx - 1, p.window);      // sliding window, or the start of the query's block of positions
-    // (own keys: tiles from the start of their first page on, so that no earlier page of the row's table is asked for)
-    const int lo = SHARED ? prefix & ~(min(p.page_size, DEC_TILE) - 1) : first_key & ~(DEC_TILE - 1);
+    // (own keys: tiles from the start of their first page on, so that no earlier page of the row's table is asked for; without any, no tile: the row's
+    // table has no page for them)
+    const int lo = SHARED ? (ctx > prefix ? prefix & ~(min(p.page_size, DEC_TILE) - 1) : ctx) : first_key & ~(DEC_TILE - 1);
     const int kept = KEEP ? mask_kept_tiles(p.keep, lo, DEC_TILE) : 0;       // tiles of kept keys in front of the window's
     const int tiles_total = kept + (ctx - lo + DEC_TILE - 1) / DEC_TILE;
     // The grid is laid out for the longest context the launch may meet; a row is cut into as many parts as
