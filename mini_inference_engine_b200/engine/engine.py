@@ -661,6 +661,7 @@ class LLMEngine:
         with _nvtx_range("forward"):
             b = self.runner.builder
             sources, logprob_sources = [], []
+            sampled_for = []                                   # the requests of ``sources``' tokens, in their order: not always the batch's
             if use_graph or (portion_graph and decoding):      # ---- the requests that decode, from their bucket's graph
                 drows = [rows[i] for i in decoding]
                 dseqs = [batch[i][0] for i in decoding]
@@ -682,6 +683,7 @@ class LLMEngine:
                 lp = self._choose_under_rules(dseqs, logits, extras, 0, turn, self._pinned_tokens)
                 sources.append((self._pinned_tokens[turn], len(dseqs)))
                 logprob_sources.append((lp, len(dseqs)))
+                sampled_for += dseqs
                 for k, seq in enumerate(dseqs):
                     seq.pending_index = k
             if use_graph:
@@ -711,6 +713,7 @@ class LLMEngine:
                     lp = self._choose_under_rules(pseqs, logits, ctx.extras, self._portion_slot, turn, self._pinned_portion)
                     sources.append((self._pinned_portion[turn], 1))
                     logprob_sources.append((lp, 1))
+                    sampled_for += pseqs
                     pseq.pending_index = self._portion_slot
             else:                                              # ---- any other mix: one batch, launched kernel by kernel
                 k = len(sample_seqs)
@@ -729,6 +732,7 @@ class LLMEngine:
                     self._pinned_tokens[turn, :k].copy_(self._sampled[:k], non_blocking=True)   # this rare way copies
                 sources.append((self._pinned_tokens[turn], k))
                 logprob_sources.append((lp, k))
+                sampled_for += sample_seqs
                 for k2, seq in enumerate(sample_seqs):
                     seq.pending_index = k2
             self._turn = turn
@@ -736,8 +740,8 @@ class LLMEngine:
             done_event = torch.cuda.Event()
             done_event.record()
 
-        ending = self._advance(batch, sample_seqs)
-        return _InFlight(sample_seqs, [s.num_tokens - 1 for s in sample_seqs], ending, sources, logprob_sources, done_event)
+        ending = self._advance(batch, sampled_for)
+        return _InFlight(sampled_for, [s.num_tokens - 1 for s in sampled_for], ending, sources, logprob_sources, done_event)
 
     def _advance(self, batch, sample_seqs) -> list:
         """Bookkeeping that does not need a launched step's tokens: progress, the place each token will take, and the requests that end by count
