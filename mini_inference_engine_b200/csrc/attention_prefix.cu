@@ -234,18 +234,20 @@ static int launch_prefix(const PrefixParams& p, long long items, cudaStream_t st
 // 128 keys of one) a slot, where a pair sees its own row's keys only; a step holds own keys of one tile, and the tiles take turns.  An item is a range of steps
 // of such a walk; it leaves o and m + log2 l of its keys for every pair (-inf where a pair saw none), and a second kernel joins the ranges of a row.  Own keys
 // that way cost their bytes and little else: attended over by the decode kernel behind a kernel for the prefixes, 64 rows of up to 512 own keys behind 8,000
-// took 62 us, 256 rows of up to 96 behind 16,384 143 us, of which 40 and 54 were the decode kernel's.
+// took 62 us, 256 rows of up to 96 behind 16,384 143 us, of which 40 and 54 were the decode kernel's.  (Rows of many hundred own keys behind short prefixes are not
+// what the walk is for: 32 heads of 64 on 4, 256 rows of up to 900 behind 400 94 us, ordinary decode attention 58; kernels/attention.py: sharing_weight.)
 //
 // Two chains of work run side by side, each with four softmax warps, a thread that issues its products, and its own S, P and O in tensor memory:
 //   S = Q K^T; the chain's threads move their rows of S into registers, write P = 2^(s - m), rounded to bfloat16, back, and
 //   O += P V with P as the left operand out of tensor memory and V as it lies.
+// (m follows the running maximum in jumps of 2^8 only: the sums take the weights unrounded, and the greatest weight, which need not be 1, is rounded like the others.)
 // Such a chain takes 4,000 cycles a step (heads of 128), four times what its products take; two fill one another's gaps.  With two tiles of pairs a chain owns a tile, and a
 // step of the prefix serves both; with one the chains take the steps in turns over the same queries and leave a result each.
 // Keys and values come by TMA, a slot a copy, keys and values each with barriers of their own: keys of a later step arrive as soon as S is formed.
 // Tensor memory: heads of 64 S 2 x 128 columns, P 2 x 64, O 2 x 64; S of the next step is issued as soon as the rows are in registers.  Heads of 128: O takes
 // 2 x 128, and P lies over the S that it came from.  A step's S, P and product with the values then go in halves of 64 keys: S of the next step's first half is
 // formed under the softmax of this one's second (whole steps, S behind the product with the values: 51 -> 45 us for 64 rows behind 8,000 keys, 124 -> 110 for 256
-// behind 16,384).
+// behind 16,384; 43 and 113 now).
 //
 // Values of one row must not reach another's output: slots' keys that are nobody's (in front of a row's own keys, behind its context) are made zero in
 // shared memory, and so are own values that are not finite, since 0 times those is not 0; the row is marked, and the joining kernel adds them to its output.

@@ -296,7 +296,7 @@ class LLMEngine:
         return self.graphs[bs, next(c for c in self.graph_bounds if c >= context)]
 
     # ------------------------------------------------------------------ CUDA graphs of decode steps over shared prefixes
-    SHARED_GROUPS = 8        # prefixes that the rows of a step may share between them; with more, every row reads its own pages
+    SHARED_GROUPS = 8        # prefixes that the rows of a step may share between them; with more, every row reads all of its pages itself
 
     def _shared_step(self, dseqs):
         """The groups of decoding rows that share a prefix, if the step is to read those once a group; else None."""
@@ -454,7 +454,7 @@ class LLMEngine:
     @torch.inference_mode()
     def add_prefix(self, prompt) -> Prefix:
         """Computes the keys and values of ``prompt`` (as many of its tokens as fill whole pages) once, for requests that begin with it
-        (``add_request(..., prefix=)``): they share the pages, and steps in which many rows share them read them once.  The pages are held until
+        (``add_request(..., prefix=)``): they share the pages, and steps in which many rows share them read them once (``generate``).  The pages are held until
         ``release_prefix``.  Refused with ValueError where a layer keeps a window, a block of positions or a state, and where the
         pages would leave a request that waits or runs too few ever to end."""
         ids = self._prompt_ids(prompt)
@@ -812,7 +812,8 @@ class LLMEngine:
 
     def generate(self, prompts, params=None, decode_text: bool = True, n: int = 1) -> list:
         """``n`` answers to every prompt, one behind another in the result; with more than one, the answers to a prompt share its pages where the
-        model allows it (``add_prefix``).  A prompt's pages are computed and held once its answers' turn comes: prompts that do not fit the cache side by
+        model allows it (``add_prefix``), and steps read them once for all of a prompt's answers where that pays, for up to
+        ``SHARED_GROUPS`` prompts at a time (with more, every answer reads them by itself).  A prompt's pages are computed and held once its answers' turn comes: prompts that do not fit the cache side by
         side wait for those in front.  What cannot be run at all is refused with ValueError before anything is added."""
         if not isinstance(params, list):
             params = [params or SamplingParams()] * len(prompts)

@@ -60,13 +60,15 @@ def rotates_in_decode(dtype, head_dim: int, ctx) -> bool:
             and decode_only(ctx) and getattr(ctx, "prefix", None) is None)
 
 
-# Shared prefixes against ordinary decode attention, which reads a prefix once a row: what sharing saves is the bytes of keys and values that are not read again, SHARE_MIN_BYTES of
-# them a layer at least.  What it costs beside that goes by the head size (``sharing_weight``).  Both sides as the engine runs them: the context's bound for every length, from 33 rows on
-# ordinary attention rotates queries and keys itself and sharing leaves that to a launch of its own, layers' caches in turns.  The weights are those of a grid that take the least time
-# over 5,100 steps (4 to 256 rows in 1 to 8 groups, 64 to 14,000 shared and up to 4,000 own keys, eleven head shapes): attention takes 1.5 % longer than by the better of the two on the
-# average and up to 1.4 times as long as by the other (3,100 steps that the grid did not see: 1.9 %, and 1.6 times); by 48 MB alone, whatever the rest, 5 % and 3.6 times (32 heads of 64 on 32, 256 rows of up to 3,000 own keys behind 112: 566 : 2,059).  Us, ordinary : shared -- 32 heads of 64 on 4: 64 rows behind 784
-# keys (48 MB) 14.6 : 19.9, behind 2,352 (144 MB) 31 : 23, of 900 own keys 39 : 37; 256 rows behind 592 (147 MB) 37 : 33, of 900 own keys 66 : 94; 32 heads of 128 on 8: 16 rows
-# behind 832 (49 MB) 15.0 : 18.2, behind 1,648 (97 MB) 24 : 18; 64 behind 8,000 (2.1 GB) 376 : 43; 32 of 128 on 32: 32 rows behind 112 (54 MB) 25 : 31, behind 304 (147 MB) 39 : 32.
+# Shared prefixes against ordinary decode attention, which reads a prefix once a row: what sharing saves is the bytes of keys and values that are not read again,
+# SHARE_MIN_BYTES of them a layer at least.  What it costs beside that goes by the head size (``sharing_weight``).  Both sides as the engine runs them: the context's bound
+# for every length, from 33 rows on ordinary attention rotates queries and keys itself and sharing leaves that to a launch of its own, layers' caches in turns.  The weights
+# are those of a grid that take the least time over 5,100 steps (4 to 256 rows in 1 to 8 groups, 64 to 14,000 shared and up to 4,000 own keys, eleven head shapes):
+# attention takes 1.5 % longer than by the better of the two on the average and up to 1.4 times as long as by the other (3,100 steps that the grid did not see: 1.9 %, and
+# 1.6 times); by 48 MB alone, whatever the rest, 5 % and 3.6 times (32 heads of 64 on 32, 256 rows of up to 3,000 own keys behind 112: 566 : 2,059).  Us, ordinary : shared
+# -- 32 heads of 64 on 4: 64 rows behind 784 keys (48 MB) 14.6 : 19.9, behind 2,352 (144 MB) 31 : 23, of 900 own keys 39 : 37; 256 rows behind 592 (147 MB) 37 : 33, of 900
+# own keys 66 : 94; 32 heads of 128 on 8: 16 rows behind 832 (49 MB) 15.0 : 18.2, behind 1,648 (97 MB) 24 : 18; 64 behind 8,000 (2.1 GB) 376 : 43; 32 of 128 on 32: 32 rows
+# behind 112 (54 MB) 25 : 31, behind 304 (147 MB) 39 : 32.
 SHARE_MIN_BYTES = 64 << 20
 
 
