@@ -884,8 +884,14 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     pages = shape[0] if shape else 0
     _need(shape == (pages, num_kv_heads, page_size, head_dim) and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous(),
           "caches must be contiguous [pages, kv heads, page size, head_dim]")
-    at_q, at_k, at_v, at_out = _at(q), _at(k_cache), _at(v_cache), _at(out)
-    ints = (_at(block_tables), _at(row_q_start), _at(row_q_len), _at(row_ctx_len), _at(group_start), _at(group_prefix))
+    device = q.get_device()
+    if not (device == k_cache.get_device() == v_cache.get_device() == out.get_device() == block_tables.get_device() == row_q_start.get_device()
+            == row_q_len.get_device() == row_ctx_len.get_device() == group_start.get_device() == group_prefix.get_device()) or device < 0:
+        for t in (q, k_cache, v_cache, out, block_tables, row_q_start, row_q_len, row_ctx_len, group_start, group_prefix):
+            _at(t)                                            # (refuses what is not on a CUDA device)
+        _need(False, "the tensors must be on the current device")
+    at_q, at_k, at_v, at_out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    ints = (block_tables.data_ptr(), row_q_start.data_ptr(), row_q_len.data_ptr(), row_ctx_len.data_ptr(), group_start.data_ptr(), group_prefix.data_ptr())
     table = block_tables.shape
     _need(len(table) == 2 and table[0] >= rows and row_q_start.numel() >= rows and row_ctx_len.numel() >= rows,
           "block_tables, row_q_start and row_ctx_len need an entry for every row")
@@ -895,10 +901,7 @@ def shared_prefix_attention(q: torch.Tensor, q_stride: int, k_cache, v_cache, bl
     width = table[1]
     _need(pages * num_kv_heads * page_size < 1 << 31, "caches of 2^31 key rows and more are not taken")
     _need(scale > 0, "the scale of the scores must be positive")
-    device = q.get_device()
-    _need(torch.cuda.current_device() == device == k_cache.get_device() == v_cache.get_device() == out.get_device() == block_tables.get_device()
-          == row_q_start.get_device() == row_q_len.get_device() == row_ctx_len.get_device() == group_start.get_device() == group_prefix.get_device(),
-          "the tensors must be on the current device")
+    _need(device == torch.cuda.current_device(), "the tensors must be on the current device")
     if rows == 0:
         return out
     covered = width * page_size

@@ -52,3 +52,10 @@ def test_log_probabilities(stray):
     t = {k: on(v, int(k == stray)) for k, v in t.items()}
     with pytest.raises(ops.KernelError, match="current device"):
         ops.sample(t["logits"], t["temperature"], t["request"], t["position"], 0, t["out"], logprob=t["logprob"])
+
+
+def test_host_tensors():
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="CUDA tensors only"):
+        ops.shared_prefix_attention(bf(2, 64), 64, bf(3, 1, 16, 16), bf(3, 1, 16, 16), i(2, 2), i(2), i(2), i(2), i(2), i(1), bf(2, 2, 16), 2, 1, 16, 16, 0.25)
